@@ -48,7 +48,7 @@ class BahWeights(C.Structure):
     ]
 
 
-_p, _i, _f, _ll = C.c_void_p, C.c_int, C.c_float, C.c_longlong
+_p, _i, _f, _d, _ll = C.c_void_p, C.c_int, C.c_float, C.c_double, C.c_longlong
 
 # name -> (restype, argtypes); must list every function include/icap_hip.h declares.
 SIGNATURES = {
@@ -195,6 +195,13 @@ SIGNATURES = {
     "icap_conv_wgrad_gather_f32": (_i, [_p, _i, _p] + [_i] * 13 + [_p, _p, _p]),
     "icap_conv_wgrad_gather_ws_floats": (_ll, [_i, _i, _i, _i, _i]),
     "icap_im2col_f32": (_i, [_p] + [_i] * 11 + [_p, _p]),
+    "icap_attention_packed_ws_bytes": (_ll, [_i] * 6),
+    "icap_attention_packed_fwd": (_i, [_i] + [_p] * 7 + [_i] * 6 + [_ll] * 6 + [_f, _i, _p, _ll, _p]),
+    "icap_attention_packed_bwd": (_i, [_i] + [_p] * 11 + [_i] * 6 + [_ll] * 8 + [_f, _i, _p, _p]),
+    "icap_linear_ce_ws_bytes": (_ll, [_i] * 5),
+    "icap_linear_ce_fwd": (_i, [_i, _p, _ll, _p, _ll, _p, _p, _i, _i, _i, _ll, _i, _p, _p, _p, _p, _ll, _p]),
+    "icap_linear_ce_bwd": (_i, [_i, _p, _ll, _p, _ll, _p, _p, _i, _i, _i, _ll] + [_p] * 7 + [_ll, _p]),
+    "icap_adamw_tensors": (_i, [_i] + [_p] * 9 + [_i] * 3 + [_d] * 6 + [C.c_ulonglong, _p, _p]),
 }
 
 _lib = None

@@ -5,6 +5,7 @@
 #include <stdio.h>
 #include <mutex>
 #include "decode.hpp"
+#include "packed.hpp"
 #include "../../include/icap_hip.h"
 
 namespace icap {
@@ -200,6 +201,54 @@ static inline long long align4(long long n) { return (n + 3) & ~3LL; }
         const int rc_ = (expr);   \
         if (rc_ != ICAP_OK) return rc_; \
     } while (0)
+
+long long linear_ce_ws_bytes(int, int, int, int, int);
+int linear_ce_fwd(int, const void*, long long, const void*, long long, const void*, const long long*, int, int, int, long long, int, float*, float*,
+                  float*, void*, long long, hipStream_t);
+int linear_ce_bwd(int, const void*, long long, const void*, long long, const void*, const long long*, int, int, int, long long, const float*,
+                  const float*, const float*, void*, void*, void*, void*, long long, hipStream_t);
+int adamw_tensors(int, void* const*, const void* const*, void* const*, void* const*, float* const*, float* const*, const long long*, const int*,
+                  const int*, int, int, int, double, double, double, double, double, double, unsigned long long, const int*, hipStream_t);
+
+// ---------------------------------------------------------------- attention over packed sequences: checks, and the share of keys
+static int attention_check(const char* what, int dtype, const AttnArgs& a) {
+    if (dtype < DT_F32 || dtype > DT_F16) { set_error("%s: unknown type %d", what, dtype); return ICAP_ERR_ARG; }
+    if (a.seqs <= 0 || a.tokens_q < 0 || a.tokens_k < 0 || a.heads <= 0 || a.kv_heads <= 0 || a.heads % a.kv_heads || a.dim <= 0 || !a.cu_q || !a.cu_k ||
+        (a.tokens_q && (!a.q || !a.lse)) || (a.tokens_k && (!a.k || !a.v))) {
+        set_error("%s: null tensor, or sizes (sequences and heads from 1, heads a multiple of key heads)", what);
+        return ICAP_ERR_ARG;
+    }
+    if (a.dim > 128 || a.dim % 8) { set_error("%s: head dimension %d must be a multiple of 8, at most 128", what, a.dim); return ICAP_ERR_LIMIT; }
+    // hidden places are -inf before the scale is applied, and the largest score is taken before it
+    if (!(a.scale > 0.f && a.scale < INFINITY)) { set_error("%s: the scale must be positive and finite", what); return ICAP_ERR_ARG; }
+    const int e = dtype == DT_F32 ? 4 : 8;
+    if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || a.q_tok % e || a.q_head % e || a.k_tok % e || a.k_head % e || a.v_tok % e || a.v_head % e) {
+        set_error("%s: q, k, v must be 16-byte aligned, their strides multiples of 16 bytes", what);
+        return ICAP_ERR_ALIGN;
+    }
+    // rows (tokens x heads) and workgroups are counted in 32 bits
+    if ((long long)a.tokens_q * a.heads > (1ll << 30) || (long long)a.tokens_k * a.kv_heads > (1ll << 30) || a.seqs > (1 << 24) ||
+        ((long long)a.seqs + 1) * a.kv_heads > (1ll << 30)) {
+        set_error("%s: tokens x heads beyond 2^30", what);
+        return ICAP_ERR_LIMIT;
+    }
+    return ICAP_OK;
+}
+
+// Keys are split when the rows alone give fewer workgroups than the card holds (256 CUs, four one-wave workgroups each):
+// only where one wave covers a sequence's rows (single tokens), so that the partial results stay small.
+static int attention_splits(int seqs, int tokens_q, int tokens_k, int heads, int kv_heads) {
+    const long long rows = (long long)tokens_q * (heads / kv_heads) / seqs;
+    if (rows > 16) return 1;
+    const long long wgs = (long long)seqs * kv_heads, longest = tokens_k;       // the longest sequence may hold them all
+    long long s = (1024 + wgs - 1) / wgs;
+    if (s > longest / 128) s = longest / 128;
+    return (int)(s < 1 ? 1 : (s > 32 ? 32 : s));
+}
+
+static long long attention_ws(int splits, int tokens_q, int heads, int dim) {
+    return splits > 1 ? (long long)splits * tokens_q * heads * (dim + 1) * 4 : 0;
+}
 
 }  // namespace icap
 
@@ -1030,6 +1079,86 @@ long long icap_conv_wgrad_gather_ws_floats(int B, int Ho, int Wo, int Cout, int 
 int icap_im2col_f32(const float* x, int B, int H, int W, int C, int KH, int KW, int S, int pad_t, int pad_l, int Ho, int Wo, float* col,
                     void* stream) {
     return im2col_f32(x, B, H, W, C, KH, KW, S, pad_t, pad_l, Ho, Wo, col, (hipStream_t)stream);
+}
+
+long long icap_attention_packed_ws_bytes(int seqs, int tokens_q, int tokens_k, int heads, int kv_heads, int dim) {
+    if (seqs <= 0 || tokens_q <= 0 || tokens_k <= 0 || heads <= 0 || kv_heads <= 0) return 0;
+    return attention_ws(attention_splits(seqs, tokens_q, tokens_k, heads, kv_heads), tokens_q, heads, dim);
+}
+
+int icap_attention_packed_fwd(int dtype, const void* q, const void* k, const void* v, void* out, float* lse, const int* cu_q, const int* cu_k,
+                              int seqs, int tokens_q, int tokens_k, int heads, int kv_heads, int dim, long long q_tok, long long q_head,
+                              long long k_tok, long long k_head, long long v_tok, long long v_head, float scale, int causal, void* ws,
+                              long long ws_bytes, void* stream) {
+    AttnArgs a{};
+    a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.cu_q = cu_q; a.cu_k = cu_k;
+    a.seqs = seqs; a.tokens_q = tokens_q; a.tokens_k = tokens_k; a.heads = heads; a.kv_heads = kv_heads; a.dim = dim; a.causal = causal;
+    a.q_tok = q_tok; a.q_head = q_head; a.k_tok = k_tok; a.k_head = k_head; a.v_tok = v_tok; a.v_head = v_head; a.scale = scale;
+    float dummy;
+    if (!lse) a.lse = &dummy;               // the check wants one; the kernels get what was given
+    if (int rc = attention_check("attention_packed_fwd", dtype, a)) return rc;
+    a.lse = lse;
+    if (tokens_q == 0) return ICAP_OK;
+    if (!out || !aligned16(out)) { set_error("attention_packed_fwd: out is null or unaligned"); return ICAP_ERR_ARG; }
+    a.group = heads / kv_heads;
+    a.splits = tokens_k > 0 ? attention_splits(seqs, tokens_q, tokens_k, heads, kv_heads) : 1;
+    if (attention_ws(a.splits, tokens_q, heads, dim) > (ws && aligned16(ws) ? ws_bytes : 0)) {
+        set_error("attention_packed_fwd: the workspace is null, unaligned or too small");
+        return ICAP_ERR_ARG;
+    }
+    a.part = (float*)ws;
+    const hipStream_t st = (hipStream_t)stream;
+    return dtype == DT_F32 ? attention_fwd_f32(a, st) : dtype == DT_BF16 ? attention_fwd_bf16(a, st) : attention_fwd_f16(a, st);
+}
+
+int icap_attention_packed_bwd(int dtype, const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, void* dq,
+                              void* dk, void* dv, const int* cu_q, const int* cu_k, int seqs, int tokens_q, int tokens_k, int heads,
+                              int kv_heads, int dim, long long g_tok, long long g_head, long long q_tok, long long q_head, long long k_tok,
+                              long long k_head, long long v_tok, long long v_head, float scale, int causal, float* ws, void* stream) {
+    AttnArgs a{};
+    a.q = q; a.k = k; a.v = v; a.o = out; a.dout = dout; a.lse = const_cast<float*>(lse); a.dq = dq; a.dk = dk; a.dv = dv; a.cu_q = cu_q; a.cu_k = cu_k;
+    a.seqs = seqs; a.tokens_q = tokens_q; a.tokens_k = tokens_k; a.heads = heads; a.kv_heads = kv_heads; a.dim = dim; a.causal = causal;
+    a.q_tok = q_tok; a.q_head = q_head; a.k_tok = k_tok; a.k_head = k_head; a.v_tok = v_tok; a.v_head = v_head; a.g_tok = g_tok; a.g_head = g_head;
+    a.scale = scale; a.splits = 1; a.delta = ws;
+    if (int rc = attention_check("attention_packed_bwd", dtype, a)) return rc;
+    a.group = heads / kv_heads;
+    if ((tokens_q && (!dout || !out || !dq || !ws)) || (tokens_k && (!dk || !dv))) {
+        set_error("attention_packed_bwd: null tensor");
+        return ICAP_ERR_ARG;
+    }
+    const int e = dtype == DT_F32 ? 4 : 8;
+    if (!aligned16(dout) || !aligned16(out) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || g_tok % e || g_head % e) {
+        set_error("attention_packed_bwd: tensors must be 16-byte aligned, strides multiples of 16 bytes");
+        return ICAP_ERR_ALIGN;
+    }
+    const hipStream_t st = (hipStream_t)stream;
+    return dtype == DT_F32 ? attention_bwd_f32(a, st) : dtype == DT_BF16 ? attention_bwd_bf16(a, st) : attention_bwd_f16(a, st);
+}
+
+long long icap_linear_ce_ws_bytes(int dtype, int rows, int width, int vocab, int backward) {
+    return linear_ce_ws_bytes(dtype, rows, width, vocab, backward);
+}
+
+int icap_linear_ce_fwd(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias, const long long* targets,
+                       int rows, int width, int vocab, long long ignore_index, int mean_over_valid, float* row_loss, float* row_lse, float* out,
+                       void* ws, long long ws_bytes, void* stream) {
+    return linear_ce_fwd(dtype, hidden, ld_h, weight, ld_w, bias, targets, rows, width, vocab, ignore_index, mean_over_valid, row_loss, row_lse, out, ws,
+                         ws_bytes, (hipStream_t)stream);
+}
+
+int icap_linear_ce_bwd(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias, const long long* targets,
+                       int rows, int width, int vocab, long long ignore_index, const float* row_lse, const float* out, const float* grad_out,
+                       void* dhidden, void* dweight, void* dbias, void* ws, long long ws_bytes, void* stream) {
+    return linear_ce_bwd(dtype, hidden, ld_h, weight, ld_w, bias, targets, rows, width, vocab, ignore_index, row_lse, out, grad_out, dhidden, dweight,
+                         dbias, ws, ws_bytes, (hipStream_t)stream);
+}
+
+int icap_adamw_tensors(int count, void* const* params, const void* const* grads, void* const* m, void* const* v, float* const* m_scales,
+                       float* const* v_scales, const long long* sizes, const int* steps, const int* index, int p_dtype, int g_dtype,
+                       int state_bits, double lr, double beta1, double beta2, double eps, double weight_decay, double grad_scale,
+                       unsigned long long seed, const int* step_dev, void* stream) {
+    return adamw_tensors(count, params, grads, m, v, m_scales, v_scales, sizes, steps, index, p_dtype, g_dtype, state_bits, lr, beta1, beta2, eps,
+                         weight_decay, grad_scale, seed, step_dev, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -1011,6 +1011,85 @@ def mha_core(q, k, v, heads):
     return out
 
 
+# ---------------------------------------------------------------------------- operators on fp32, bf16 and fp16 tensors
+DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _ckd(t, name, dtype=None, shape=None):
+    """A tensor of one of the three types (or of `dtype`) on the CURRENT HIP device, whose stream the call is queued on."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise IcapError(f"{name}: expected a tensor on the HIP device, got {getattr(t, 'device', type(t))}; "
+                        "the MI355X path has no CPU fallback")
+    if t.device.index != (_raw_device() if _raw_device is not None else torch.cuda.current_device()):
+        raise IcapError(f"{name}: lives on {t.device}, which is not the current device (torch.cuda.set_device / torch.cuda.device)")
+    if (t.dtype != dtype) if dtype is not None else (t.dtype not in DTYPE_CODES):
+        raise IcapError(f"{name}: expected dtype {dtype if dtype is not None else 'float32, bfloat16 or float16'}, got {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise IcapError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t
+
+
+def _packed_rows(t):
+    """t [tokens, heads, dim] as the attention kernels read it (last axis contiguous, 16-byte aligned rows; a slice of a fused
+    projection is), a contiguous copy otherwise."""
+    per = 16 // t.element_size()
+    if t.stride(2) == 1 and t.stride(0) % per == 0 and t.stride(1) % per == 0 and t.data_ptr() % 16 == 0:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _packed_args(q, k, v, cu_q, cu_k, what):
+    _ckd(q, f"{what}: q")
+    _ckd(k, f"{what}: k", q.dtype)
+    _ckd(v, f"{what}: v", q.dtype)
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[2] != q.shape[2]:
+        raise IcapError(f"{what}: q [tokens_q, heads, dim] and k, v [tokens_k, kv_heads, dim] are wanted, got {tuple(q.shape)}, {tuple(k.shape)}, "
+                        f"{tuple(v.shape)}")
+    if q.shape[1] < 1 or k.shape[1] < 1 or q.shape[1] % k.shape[1]:
+        raise IcapError(f"{what}: {q.shape[1]} heads are not a multiple of {k.shape[1]} key heads")
+    if q.shape[2] < 8 or q.shape[2] % 8 or q.shape[2] > 128:
+        raise IcapError(f"{what}: head dimension {q.shape[2]} must be a multiple of 8, at most 128")
+    cu_k = cu_q if cu_k is None else cu_k
+    for t, name in ((cu_q, "cu_q"), (cu_k, "cu_k")):
+        _ckd(t, f"{what}: {name}", torch.int32)
+        if t.dim() != 1 or t.numel() < 2 or not t.is_contiguous():
+            raise IcapError(f"{what}: {name} must be a contiguous vector of sequences + 1 offsets")
+    if cu_k.numel() != cu_q.numel():
+        raise IcapError(f"{what}: cu_q and cu_k count {cu_q.numel() - 1} and {cu_k.numel() - 1} sequences")
+    return cu_k
+
+
+def attention_packed(q, k, v, cu_q, cu_k=None, causal=True, scale=None, want_lse=False):
+    """Attention over packed sequences (no padding), grouped heads, fp32 / bf16 / fp16, no gradient of its own
+    (training.packed_attention has one).
+
+    q [tokens_q, heads, dim], k, v [tokens_k, kv_heads, dim] (heads a multiple of kv_heads, dim a multiple of 8 up to 128; the last
+    axis contiguous, e.g. slices of one projection), cu_q, cu_k int32 [sequences + 1] on the device: sequence b owns rows
+    cu[b] .. cu[b + 1] (cu_k None: the same).  The offsets start at 0 and do not decrease; they stay on the device, unread by the host.
+    causal: query i of n_q sees keys 0 .. i + n_k - n_q, so a single new token (n_q = 1) sees its whole cache.
+    A row that sees no key, and every row behind the last sequence, gives zeros.  v must be finite, scale (None: dim ** -0.5) positive.
+    Returns out [tokens_q, heads, dim], and with want_lse also log sum exp(scale q k) [tokens_q, heads] in fp32."""
+    cu_k = _packed_args(q, k, v, cu_q, cu_k, "attention_packed")
+    q, k, v = _packed_rows(q), _packed_rows(k), _packed_rows(v)
+    tq, H, D = q.shape
+    tk, K = k.shape[0], k.shape[1]
+    seqs = cu_q.numel() - 1
+    out = torch.empty((tq, H, D), device=q.device, dtype=q.dtype)
+    lse = torch.empty((tq, H), device=q.device, dtype=torch.float32) if want_lse else None
+    lib = N.load()
+    nbytes = lib.icap_attention_packed_ws_bytes(seqs, tq, tk, H, K, D)
+    ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes > 0 else None
+    span = _Span("attention_packed", (tq, tk, seqs, H, K, D, str(q.dtype), bool(causal)))
+    N.check(lib.icap_attention_packed_fwd(DTYPE_CODES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                          lse.data_ptr() if want_lse else None, cu_q.data_ptr(), cu_k.data_ptr(), seqs, tq, tk, H, K, D,
+                                          q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                                          float(scale) if scale is not None else D ** -0.5, int(bool(causal)),
+                                          ws.data_ptr() if ws is not None else None, nbytes, _stream()), "attention_packed")
+    span.done()
+    return (out, lse) if want_lse else out
+
+
 def bahdanau_attention(u, w, a_w, a_b: float, feat, want_alpha=True, alpha_out=None, ctx_out=None):
     """alpha_out [B, B] / ctx_out [B, E]: optional contiguous destinations (a training loop's per-step slices)."""
     B, A = u.shape

@@ -6,11 +6,14 @@ operation runs in ``libicap_hip.so``.
 """
 from __future__ import annotations
 
+from array import array
+from operator import attrgetter
+
 import torch
 
 from . import _native as N
 from . import ops
-from .ops import ACT_NONE, _Span, _ck, _stream
+from .ops import ACT_NONE, DTYPE_CODES, _Span, _ck, _ckd, _packed_args, _packed_rows, _stream
 
 COL_SUM, COL_SQDEV, COL_BN_BWD, COL_LN_BWD, COL_MOMENTS = 0, 1, 2, 3, 4
 
@@ -438,6 +441,198 @@ def embedding_bwd(idx, dy, V):
     dt = torch.zeros(V, E, device=dy.device)
     N.check(N.load().icap_embedding_bwd_f32(idx.data_ptr(), dy.data_ptr(), dy.stride(0), P, E, V, dt.data_ptr(), _stream()), "embedding_bwd")
     return dt
+
+
+# ---------------------------------------------------------------------------- packed attention, vocabulary loss, many tensors
+def attention_packed_bwd(dout, q, k, v, out, lse, cu_q, cu_k=None, causal=True, scale=None):
+    """Gradients of ops.attention_packed: dout in the shape of out, which with lse is what the forward call gave
+    (want_lse=True); the other arguments as there.  Returns (dq, dk, dv), dense; rows behind the last sequence are zeros.
+    The heads that share a key head add up in a fixed order."""
+    cu_k = _packed_args(q, k, v, cu_q, cu_k, "attention_packed_bwd")
+    tq, H, D = q.shape
+    tk, K = k.shape[0], k.shape[1]
+    _ckd(dout, "attention_packed_bwd: dout", q.dtype, q.shape)
+    _ckd(out, "attention_packed_bwd: out", q.dtype, q.shape)
+    _ckd(lse, "attention_packed_bwd: lse", torch.float32, (tq, H))
+    if not out.is_contiguous() or not lse.is_contiguous():
+        raise N.IcapError("attention_packed_bwd: out and lse must be contiguous, as attention_packed returns them")
+    q, k, v, dout = _packed_rows(q), _packed_rows(k), _packed_rows(v), _packed_rows(dout)
+    seqs, dev = cu_q.numel() - 1, q.device
+    dq = torch.empty((tq, H, D), device=dev, dtype=q.dtype)
+    dk, dv = torch.empty((tk, K, D), device=dev, dtype=q.dtype), torch.empty((tk, K, D), device=dev, dtype=q.dtype)
+    ws = torch.empty(max(tq * H, 1), device=dev, dtype=torch.float32)
+    span = _Span("attention_packed_bwd", (tq, tk, seqs, H, K, D, str(q.dtype), bool(causal)))
+    N.check(N.load().icap_attention_packed_bwd(DTYPE_CODES[q.dtype], dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                               lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
+                                               seqs, tq, tk, H, K, D, dout.stride(0), dout.stride(1), q.stride(0), q.stride(1), k.stride(0),
+                                               k.stride(1), v.stride(0), v.stride(1), float(scale) if scale is not None else D ** -0.5,
+                                               int(bool(causal)), ws.data_ptr(), _stream()), "attention_packed_bwd")
+    span.done()
+    return dq, dk, dv
+
+
+def _ce_rows(t, name, dtype=None):
+    """[rows, width] with contiguous rows of one of the three types."""
+    _ckd(t, name, dtype)
+    if t.dim() != 2 or t.size(0) < 1 or t.size(1) < 1 or (t.size(1) > 1 and t.stride(1) != 1) or (t.size(0) > 1 and t.stride(0) < t.size(1)):
+        raise N.IcapError(f"{name}: expected a [rows, width] matrix with contiguous rows, got {tuple(t.shape)} with strides {t.stride()}")
+    return t.stride(0) if t.size(0) > 1 else t.size(1)
+
+
+def linear_ce_fwd(hidden, weight, bias, targets, ignore_index=-100, mean_over_valid=True, want_grad=True):
+    """Cross entropy of hidden @ weight.T + bias over its columns without the [rows, vocab] logits in memory.
+
+    hidden [rows, width], weight [vocab, width], bias [vocab] or None, all fp32, bf16 or fp16 (rows may be strided); targets int64
+    [rows].  A target that is ignore_index or outside the vocabulary is left out.  mean_over_valid: the mean over the rows that count
+    (training.CrossEntropyLoss); otherwise over all rows (training.compute_loss).
+    Returns (loss - a device scalar -, row_loss [rows] fp32, what linear_ce_bwd needs or None)."""
+    ld_h = _ce_rows(hidden, "linear_ce: hidden")
+    ld_w = _ce_rows(weight, "linear_ce: weight", hidden.dtype)
+    R, E = hidden.shape
+    V = weight.shape[0]
+    if weight.shape[1] != E:
+        raise N.IcapError(f"linear_ce: hidden is {E} wide, weight {weight.shape[1]}")
+    if bias is not None and not _ckd(bias, "linear_ce: bias", hidden.dtype, (V,)).is_contiguous():
+        raise N.IcapError("linear_ce: bias must be contiguous")
+    if not _ckd(targets, "linear_ce: targets", torch.int64, (R,)).is_contiguous():
+        raise N.IcapError("linear_ce: targets must be contiguous")
+    lib, dev, code = N.load(), hidden.device, DTYPE_CODES[hidden.dtype]
+    rows = torch.empty((2, R), device=dev, dtype=torch.float32)
+    out = torch.empty(2, device=dev, dtype=torch.float32)
+    nbytes = lib.icap_linear_ce_ws_bytes(code, R, E, V, 0)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    span = _Span("linear_ce_fwd", (R, E, V, str(hidden.dtype)))
+    N.check(lib.icap_linear_ce_fwd(code, hidden.data_ptr(), ld_h, weight.data_ptr(), ld_w, _p(bias), targets.data_ptr(), R, E, V, int(ignore_index),
+                                   int(bool(mean_over_valid)), rows[0].data_ptr(), rows[1].data_ptr(), out.data_ptr(), ws.data_ptr(), nbytes,
+                                   _stream()), "linear_ce_fwd")
+    span.done()
+    return out[0], rows[0], (hidden, weight, bias, targets, int(ignore_index), rows, out) if want_grad else None
+
+
+def linear_ce_bwd(grad_out, saved, need=(True, True, True)):
+    """Gradients of grad_out (fp32 device scalar) times linear_ce_fwd's loss: (dhidden, dweight, dbias), dense, in the tensors'
+    type; need: which of them are wanted (None in the others' places, and for a bias that is None)."""
+    hidden, weight, bias, targets, ignore_index, rows, out = saved
+    g = _ckd(grad_out, "linear_ce_bwd: grad_out", torch.float32)
+    if g.numel() != 1:
+        raise N.IcapError("linear_ce_bwd: grad_out must be one value")
+    (R, E), V, dev, dtype = hidden.shape, weight.shape[0], hidden.device, hidden.dtype
+    _ckd(hidden, "linear_ce_bwd: hidden", dtype)
+    dh = torch.empty((R, E), device=dev, dtype=dtype) if need[0] else None
+    dw = torch.empty((V, E), device=dev, dtype=dtype) if need[1] else None
+    db = torch.empty(V, device=dev, dtype=dtype) if need[2] and bias is not None else None
+    if dh is None and dw is None and db is None:
+        return None, None, None
+    lib, code = N.load(), DTYPE_CODES[dtype]
+    nbytes = lib.icap_linear_ce_ws_bytes(code, R, E, V, 1)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    span = _Span("linear_ce_bwd", (R, E, V, str(dtype)))
+    N.check(lib.icap_linear_ce_bwd(code, hidden.data_ptr(), _ce_rows(hidden, "hidden"), weight.data_ptr(), _ce_rows(weight, "weight"), _p(bias),
+                                   targets.data_ptr(), R, E, V, ignore_index, rows[1].data_ptr(), out.data_ptr(), g.data_ptr(), _p(dh), _p(dw), _p(db),
+                                   ws.data_ptr(), nbytes, _stream()), "linear_ce_bwd")
+    span.done()
+    return dh, dw, db
+
+
+_dtype_of, _shape_of = attrgetter("dtype"), attrgetter("shape")
+
+
+def _check_list(name, tensors, dtypes):
+    """(types, addresses) of tensors that must be contiguous, of these types and on the current device.  Each property is read for
+    a whole list at a time: a Python check a tensor took 9 us a parameter, which for hundreds of them is ten times the kernel."""
+    if not all(issubclass(t, torch.Tensor) for t in set(map(type, tensors))):
+        raise N.IcapError(f"adamw_tensors: {name}: a tensor is wanted")
+    devices = set(map(torch.Tensor.get_device, tensors))
+    if -1 in devices:
+        raise N.IcapError(f"adamw_tensors: {name}: expected tensors on the HIP device; the MI355X path has no CPU fallback")
+    if devices != {torch.cuda.current_device()}:
+        raise N.IcapError(f"adamw_tensors: {name}: lives on another device than the current one (torch.cuda.set_device / torch.cuda.device)")
+    kinds = set(map(_dtype_of, tensors))
+    if not kinds <= set(dtypes):
+        raise N.IcapError(f"adamw_tensors: {name}: expected {' / '.join(map(str, dtypes))}, got {' / '.join(map(str, kinds))}")
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
+        raise N.IcapError(f"adamw_tensors: {name}: tensors must be contiguous")
+    return kinds, list(map(torch.Tensor.data_ptr, tensors))
+
+
+STATE_BLOCK = 256       # values of a tensor that share one scale of an 8-bit optimizer state
+
+
+def adamw_state8(p):
+    """An 8-bit optimizer state of zeros for tensor p: (e4m3 codes in its shape, fp32 scales, one for every 256 values)."""
+    return (torch.zeros(p.shape, device=p.device, dtype=torch.uint8).view(torch.float8_e4m3fn),
+            torch.zeros((p.numel() + STATE_BLOCK - 1) // STATE_BLOCK, device=p.device, dtype=torch.float32))
+
+
+def adamw_tensors(params, grads, exp_avg, exp_avg_sq, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=1e-2, grad_scale=1.0,
+                  seed=0, index=None, step_dev=None):
+    """One AdamW update (training.AdamW's arithmetic, in fp32) of a list of tensors where they lie, in place, some 40 tensors a launch.
+
+    params: fp32, bf16 or fp16, contiguous; grads: their gradients, of the same type or fp32 (None: the tensor is left alone).
+    exp_avg, exp_avg_sq: fp32 tensors (states of 32 bits), or (codes, scales) pairs (states of 8 bits: adamw_state8; the second one
+    holds the SQUARE ROOT of the second moment, rounded at random - with the right mean - from `seed`, the step, the tensor's index
+    and the place, so a step can be repeated).  All states are of one kind.
+    step: from 1, one for all or a list; step_dev: int32 [1] on the device, added to step by the kernel (a step recorded in a HIP
+    graph: step = 0 and the count kept there).  index: the tensors' numbers for the generator (their places in the list).
+    No tensor may appear twice.  A gradient that is not finite spoils its value's states, with 8 bits its block's."""
+    n = len(params)
+    if not (len(grads) == len(exp_avg) == len(exp_avg_sq) == n):
+        raise N.IcapError("adamw_tensors: as many gradients and states as parameters are wanted")
+    steps = list(step) if isinstance(step, (list, tuple)) else [step] * n
+    index = list(range(n)) if index is None else list(index)
+    if len(steps) != n or len(index) != n:
+        raise N.IcapError("adamw_tensors: as many steps and indexes as parameters are wanted")
+    if step_dev is not None and _ckd(step_dev, "adamw_tensors: step_dev", torch.int32).numel() != 1:
+        raise N.IcapError("adamw_tensors: step_dev must be one int32")
+    if any(g is None for g in grads):
+        keep = [i for i in range(n) if grads[i] is not None]
+        params, grads, exp_avg, exp_avg_sq, steps, index = ([x[i] for i in keep] for x in (params, grads, exp_avg, exp_avg_sq, steps, index))
+    if not params:
+        return
+    eight = isinstance(exp_avg[0], (tuple, list))
+    if any((t in (tuple, list)) != eight for t in {*map(type, exp_avg), *map(type, exp_avg_sq)}):
+        raise N.IcapError("adamw_tensors: states of 8 and of 32 bits in one call")
+    f32 = {torch.float32}
+    p_kinds, p_ptr = _check_list("parameter", params, DTYPE_CODES.keys())
+    g_kinds, g_ptr = _check_list("gradient", grads, DTYPE_CODES.keys())
+    sizes = list(map(torch.Tensor.numel, params))
+    if list(map(_shape_of, params)) != list(map(_shape_of, grads)):
+        raise N.IcapError("adamw_tensors: a gradient has another shape than its parameter")
+    if eight:
+        (m, ms), (v, vs) = zip(*exp_avg), zip(*exp_avg_sq)
+        state = [_check_list("state's codes", x, {torch.float8_e4m3fn})[1] for x in (m, v)] + [_check_list("state's scales", x, f32)[1] for x in (ms, vs)]
+        blocks = [(k + STATE_BLOCK - 1) // STATE_BLOCK for k in sizes]
+        right = list(map(torch.Tensor.numel, ms)) == blocks and list(map(torch.Tensor.numel, vs)) == blocks
+    else:
+        m, v = exp_avg, exp_avg_sq
+        state = [_check_list("moment", x, f32)[1] for x in (m, v)]
+        right = True
+    if not right or list(map(torch.Tensor.numel, m)) != sizes or list(map(torch.Tensor.numel, v)) != sizes:
+        raise N.IcapError("adamw_tensors: a state has another size than its parameter")
+    if len(set(p_ptr)) < len(p_ptr) and len({a for a, k in zip(p_ptr, sizes) if k}) < sum(k > 0 for k in sizes):
+        raise N.IcapError("adamw_tensors: a parameter appears twice")
+    columns = [p_ptr, g_ptr, *state, sizes, steps, index]
+    if len(p_kinds) == 1 and len(g_kinds) == 1:
+        groups = {(*p_kinds, *g_kinds): columns}
+    else:
+        groups = {}
+        for row in zip(zip(map(_dtype_of, params), map(_dtype_of, grads)), *columns):
+            for lst, x in zip(groups.setdefault(row[0], [[] for _ in columns]), row[1:]):
+                lst.append(x)
+    if any(g != p and g != torch.float32 for p, g in groups):
+        raise N.IcapError("adamw_tensors: gradients are of their parameter's type or fp32")
+    lib = N.load()
+    for (pd, gd), cols in groups.items():
+        arrays = [array("Q", x) for x in cols[:-3]] + [array("q", cols[-3]), array("i", cols[-2]), array("i", cols[-1])]
+        at = [x.buffer_info()[0] for x in arrays]
+        if not eight:
+            at[4:4] = [None, None]
+        span = _Span("adamw_tensors", (len(cols[0]), sum(cols[-3]), str(pd), 8 if eight else 32))
+        N.check(lib.icap_adamw_tensors(len(cols[0]), *at, DTYPE_CODES[pd], DTYPE_CODES[gd], 8 if eight else 32, float(lr), float(beta1), float(beta2),
+                                       float(eps), float(weight_decay), float(grad_scale), int(seed) & (2 ** 64 - 1), _p(step_dev), _stream()),
+                "adamw_tensors")
+        span.done()
+    ops.bump_weights_generation()       # the kernel writes the parameters by raw pointer: eval-mode weight caches must rebuild
 
 
 # ---------------------------------------------------------------------------- convolutional encoder

@@ -96,6 +96,64 @@ class CrossEntropyLoss(torch.nn.Module):
         return _MaskedCE.apply(outputs, targets, self.ignore_index, True)
 
 
+# ---------------------------------------------------------------------------- attention and loss of a decoder on packed captions
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, causal, scale):
+        out, lse = ops.attention_packed(q, k, v, cu_q, cu_k, causal=causal, scale=scale, want_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
+        ctx.how = (causal, scale)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
+        causal, scale = ctx.how
+        from . import train_ops as T
+        return (*T.attention_packed_bwd(dout, q, k, v, out, lse, cu_q, cu_k, causal=causal, scale=scale), None, None, None, None)
+
+
+def packed_attention(q, k, v, cu_q, cu_k=None, causal=True, scale=None):
+    """ops.attention_packed with its gradient: self-attention of captions (or of any texts) of different lengths without padding,
+    or - causal=False, offsets of their own for the keys - their attention to an image's features."""
+    cu_k = cu_q if cu_k is None else cu_k
+    if not (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v))):
+        return ops.attention_packed(q, k, v, cu_q, cu_k, causal=causal, scale=scale)
+    return _PackedAttention.apply(q, k, v, cu_q, cu_k, bool(causal), scale)
+
+
+class _LinearCE(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, bias, targets, ignore_index, mean_over_valid):
+        from . import train_ops as T
+        value, _, saved = T.linear_ce_fwd(hidden, weight, bias, targets, ignore_index, mean_over_valid)
+        ctx.ignore_index, rows, out = saved[4:]
+        ctx.save_for_backward(hidden, weight, bias, targets, rows, out)
+        return value
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        from . import train_ops as T
+        hidden, weight, bias, targets, rows, out = ctx.saved_tensors
+        g = grad_out.reshape(1).contiguous().float()
+        return (*T.linear_ce_bwd(g, (hidden, weight, bias, targets, ctx.ignore_index, rows, out), need=ctx.needs_input_grad[:3]), None, None, None)
+
+
+def linear_cross_entropy(hidden, weight, bias, targets, ignore_index: int = -100, mean_over_valid: bool = True) -> torch.Tensor:
+    """The loss of an output layer and its criterion in one: cross entropy of hidden @ weight.T + bias, without the logits in
+    memory (train_ops.linear_ce_fwd).  hidden [..., width] fp32, bf16 or fp16, targets [...] int64, weight [vocab, width] and bias
+    [vocab] or None (an nn.Linear's) of the same type.  mean_over_valid: the mean over the rows that are not ignored, as
+    CrossEntropyLoss above; otherwise over all rows, as compute_loss."""
+    if hidden.dim() < 2 or hidden.shape[:-1] != targets.shape:
+        raise N.IcapError(f"linear_cross_entropy: hidden {tuple(hidden.shape)} and targets {tuple(targets.shape)} do not belong together")
+    hidden, targets = hidden.reshape(-1, hidden.size(-1)), targets.reshape(-1).contiguous()
+    if hidden.numel() and hidden.stride(-1) != 1:
+        hidden = hidden.contiguous()
+    return _LinearCE.apply(hidden, weight, bias, targets, int(ignore_index), bool(mean_over_valid))
+
+
 # ---------------------------------------------------------------------------- optimizer
 class FlatParameters:
     """Moves the trainable parameters of a model into ONE flat fp32 tensor.
@@ -230,6 +288,77 @@ class AdamW:
         self.v.copy_(state["exp_avg_sq"])
         self.steps = int(state["step"])
         self.param_steps = [int(s) for s in state["param_steps"]]
+        self.lr, self.betas, self.eps, self.weight_decay = float(state["lr"]), tuple(state["betas"]), float(state["eps"]), float(state["weight_decay"])
+
+
+class AdamWTensors:
+    """AdamW's update over the parameters where they lie - fp32, bf16 or fp16, not moved into a flat buffer, with their own .grad -
+    some 40 tensors a launch (train_ops.adamw_tensors).  state_bits 8: both moments in one byte a value (a quarter of the
+    memory of fp32 states, 4 instead of 16 bytes of traffic a value); 32: fp32 states, results as AdamW's.
+
+    A parameter without a gradient is left alone and its own step count does not advance, as in torch.  The randomness of the
+    8-bit states' rounding follows from `seed`, the step and the parameter's place, so a run can be repeated.
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=8, seed=0):
+        from . import train_ops as T
+        self.params = [p for p in params if p.requires_grad]
+        if not self.params:
+            raise ValueError("no trainable parameters")
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamWTensors: states of 8 or 32 bits, not {state_bits!r}")
+        if len({id(p) for p in self.params}) != len(self.params):
+            raise ValueError("AdamWTensors: a parameter appears twice")
+        for p in self.params:
+            if p.device.type != "cuda" or p.dtype not in ops.DTYPE_CODES:
+                raise N.IcapError("AdamWTensors: fp32, bf16 or fp16 parameters on the HIP device are wanted (no CPU path)")
+        self.lr, self.betas, self.eps, self.weight_decay = float(lr), (float(betas[0]), float(betas[1])), float(eps), float(weight_decay)
+        self.state_bits, self.seed, self.grad_scale = state_bits, int(seed), 1.0
+        new = T.adamw_state8 if state_bits == 8 else (lambda p: torch.zeros(p.shape, device=p.device, dtype=torch.float32))
+        self.m, self.v = [new(p) for p in self.params], [new(p) for p in self.params]
+        self.param_steps = [0] * len(self.params)
+
+    def zero_grad(self, set_to_none: bool = True) -> None:
+        for p in self.params:
+            if set_to_none:
+                p.grad = None
+            elif p.grad is not None:
+                p.grad.zero_()
+
+    def _launch(self, steps, step_dev=None):
+        from . import train_ops as T
+        T.adamw_tensors([p.detach() for p in self.params], [p.grad for p in self.params], self.m, self.v, step=steps, lr=self.lr, beta1=self.betas[0],
+                        beta2=self.betas[1], eps=self.eps, weight_decay=self.weight_decay, grad_scale=self.grad_scale, seed=self.seed,
+                        step_dev=step_dev)
+
+    def step(self) -> None:
+        nxt = [s + (p.grad is not None) for s, p in zip(self.param_steps, self.params)]
+        self._launch(nxt)
+        self.param_steps = nxt
+
+    def record_step(self, step_dev: torch.Tensor) -> None:
+        """The launches of ``step`` with the number of steps already taken since the recording began read from `step_dev` (int32
+        [1] on the device, advanced by the caller inside the graph) - what a step recorded in a HIP graph needs.  Changes no host
+        state: after n replays call ``advance_recorded(n)``."""
+        self._launch([s + 1 for s in self.param_steps], step_dev)
+
+    def advance_recorded(self, replays: int) -> None:
+        ops.bump_weights_generation()
+        self.param_steps = [s + replays * (p.grad is not None) for s, p in zip(self.param_steps, self.params)]
+
+    def state_dict(self):
+        return {"m": self.m, "v": self.v, "param_steps": list(self.param_steps), "state_bits": self.state_bits, "seed": self.seed, "lr": self.lr,
+                "betas": self.betas, "eps": self.eps, "weight_decay": self.weight_decay}
+
+    def load_state_dict(self, state) -> None:
+        def parts(x):
+            return [t for y in x for t in (y if isinstance(y, (tuple, list)) else (y,))]
+        mine, theirs = parts(self.m) + parts(self.v), parts(state["m"]) + parts(state["v"])
+        if state["state_bits"] != self.state_bits or len(state["param_steps"]) != len(self.params) or [t.shape for t in mine] != [t.shape for t in theirs]:
+            raise ValueError("AdamWTensors.load_state_dict: state belongs to a different parameter set or state width")
+        for a, b in zip(mine, theirs):
+            a.copy_(b)
+        self.param_steps, self.seed = [int(s) for s in state["param_steps"]], int(state["seed"])
         self.lr, self.betas, self.eps, self.weight_decay = float(state["lr"]), tuple(state["betas"]), float(state["eps"]), float(state["weight_decay"])
 
 

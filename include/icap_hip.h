@@ -826,6 +826,65 @@ int icap_conv_wgrad_gather_f32(const float* dz, int ldz, const float* x, int B, 
                                int S, int pad_t, int pad_l, int Ho, int Wo, int Cout, float* dw, float* ws, void* stream);
 long long icap_conv_wgrad_gather_ws_floats(int B, int Ho, int Wo, int Cout, int N);
 
+/* ------------------------------------------------------------------ packed sequences, vocabulary loss, many-tensor update
+ * No counterpart in the reference (its decoders never call their self-attention, transformer_word_level.py:72-79; its loss
+ * takes stored logits, data.py:244-252): what a decoder that attends over its own captions needs beside the path above.
+ * These take tensors of three types; sums, softmax statistics and optimizer arithmetic are fp32 whatever the type. */
+#define ICAP_F32 0
+#define ICAP_BF16 1
+#define ICAP_F16 2
+
+/* Attention over packed sequences: sequence b owns rows cu_q[b] .. cu_q[b+1] of q [tokens_q][heads][dim] and rows
+ * cu_k[b] .. cu_k[b+1] of k, v [tokens_k][kv_heads][dim] (int32 [seqs+1] on the device, not decreasing, from 0; offsets beyond
+ * the tensors are cut off).  heads % kv_heads == 0: query head h reads key head h / (heads / kv_heads).  causal: query i of
+ * n_q sees keys 0 .. i + n_k - n_q (places aligned at the sequences' ends, so one new token sees its whole cache); a row that
+ * sees no key gives zeros and a log-sum of -inf.  Rows behind the last sequence give zeros.
+ * out dense [tokens_q][heads][dim]; lse (may be NULL) [tokens_q][heads] = log sum exp(scale q k).  Strides of q, k, v (and dout)
+ * in elements, the last axis contiguous; scale > 0; dim % 8 == 0, dim <= 128; pointers 16-byte aligned and strides multiples of 16 bytes
+ * (error 2 otherwise).  Values of v must be finite (a hidden key's weight is 0, and 0 times infinity is not).
+ * ws: icap_attention_packed_ws_bytes(...) bytes, 16-byte aligned (0: none).
+ * Backward: out, lse as the forward call gave them; dq, dk, dv dense in the shapes of q, k, v; ws: tokens_q * heads floats. */
+long long icap_attention_packed_ws_bytes(int seqs, int tokens_q, int tokens_k, int heads, int kv_heads, int dim);
+int icap_attention_packed_fwd(int dtype, const void* q, const void* k, const void* v, void* out, float* lse, const int* cu_q,
+                              const int* cu_k, int seqs, int tokens_q, int tokens_k, int heads, int kv_heads, int dim,
+                              long long q_tok, long long q_head, long long k_tok, long long k_head, long long v_tok,
+                              long long v_head, float scale, int causal, void* ws, long long ws_bytes, void* stream);
+int icap_attention_packed_bwd(int dtype, const void* dout, const void* q, const void* k, const void* v, const void* out,
+                              const float* lse, void* dq, void* dk, void* dv, const int* cu_q, const int* cu_k, int seqs,
+                              int tokens_q, int tokens_k, int heads, int kv_heads, int dim, long long g_tok, long long g_head,
+                              long long q_tok, long long q_head, long long k_tok, long long k_head, long long v_tok,
+                              long long v_head, float scale, int causal, float* ws, void* stream);
+
+/* Cross entropy of a Linear layer without its logits in memory: x = hidden weight^T + bias, loss_r = log sum_v exp x_rv -
+ * x_r,target (0 for ignored rows: target == ignore_index or outside [0, vocab)); hidden [rows][width] (rows ld_h apart), weight
+ * [vocab][width] (ld_w), bias [vocab] or NULL, all of one type.  out[0] = loss, out[1] = the scale every row was weighted with,
+ * as in icap_ce_loss_fwd_f32 (mean_over_valid likewise); row_loss, row_lse [rows] fp32.
+ * Backward: gradients of grad_out[0] (device scalar) * loss in the tensors' type, dense: dhidden [rows][width], dweight
+ * [vocab][width], dbias [vocab]; each may be NULL.  fp32 products are fp32-accurate; magnitudes of fp32 hidden and weight below 2^74.
+ * ws: icap_linear_ce_ws_bytes(dtype, rows, width, vocab, backward) bytes, 16-byte aligned: bounded by about
+ * 256 MB and copies of hidden and weight, whatever the vocabulary. */
+long long icap_linear_ce_ws_bytes(int dtype, int rows, int width, int vocab, int backward);
+int icap_linear_ce_fwd(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
+                       const long long* targets, int rows, int width, int vocab, long long ignore_index, int mean_over_valid,
+                       float* row_loss, float* row_lse, float* out, void* ws, long long ws_bytes, void* stream);
+int icap_linear_ce_bwd(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
+                       const long long* targets, int rows, int width, int vocab, long long ignore_index, const float* row_lse,
+                       const float* out, const float* grad_out, void* dhidden, void* dweight, void* dbias, void* ws,
+                       long long ws_bytes, void* stream);
+
+/* One AdamW step (icap_adamw_f32's update) over `count` tensors where they lie; the lists are HOST arrays of device pointers.
+ * p_dtype: the parameters' type; g_dtype: the gradients', the same or ICAP_F32.  state_bits 32: m, v fp32 tensors (scales unused,
+ * may be NULL).  state_bits 8: m, v e4m3 codes (one byte a value), m_scales[i], v_scales[i] fp32 [ceil(n / 256)]: the state is
+ * code * scale of the value's block of 256 - the first moment, and the SQUARE ROOT of the second; the first moment's codes are
+ * rounded to nearest, the second's at random with 16 bits from the counter-based generator keyed by (seed, step * 2^20 + index[i],
+ * place / 4).  steps[i]: step of tensor i from 1; with step_dev not NULL the step is *step_dev + steps[i], read by the kernel (a
+ * launch recorded in a HIP graph keeps its arguments).  index[i] < 2^20 names the tensor to the generator.  No alignment
+ * is needed (16-byte aligned tensors are read 16 bytes at a time). */
+int icap_adamw_tensors(int count, void* const* params, const void* const* grads, void* const* m, void* const* v,
+                       float* const* m_scales, float* const* v_scales, const long long* sizes, const int* steps, const int* index,
+                       int p_dtype, int g_dtype, int state_bits, double lr, double beta1, double beta2, double eps,
+                       double weight_decay, double grad_scale, unsigned long long seed, const int* step_dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
