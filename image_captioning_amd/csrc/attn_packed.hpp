@@ -113,7 +113,7 @@ struct Where { int seq, tile, used; };
 
 // Which sequence and which of its tiles workgroup `bid` owns, from the running sum of the sequences' tile counts; every thread
 // looks at one sequence.  seq = -1: behind the last tile; used = the number of tiles there are.  Lengths are bounded by
-// `tokens`, so a wrong list of offsets reads and writes nothing outside the tensors.  sh: 8 ints of LDS.
+// `tokens`, so a wrong list of offsets reads and writes nothing outside the tensors.  sh: 16 ints of LDS.
 template <int NTHR>
 __device__ __forceinline__ Where locate(const int* cu, int seqs, int tokens, int per_token, int rows, int bid, int* sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -129,15 +129,15 @@ __device__ __forceinline__ Where locate(const int* cu, int seqs, int tokens, int
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) { const int t = __shfl_up(inc, d); if (lane >= d) inc += t; }
         if (lane == 63) sh[wave] = inc;
-        if (tid == 0) sh[4] = -1;
+        if (tid == 0) sh[8] = -1;
         __syncthreads();
         int pre = 0, tot = 0;
 #pragma unroll
         for (int w = 0; w < NTHR / 64; ++w) { const int t = sh[w]; if (w < wave) pre += t; tot += t; }
         const int end = base + pre + inc;
-        if (n > 0 && bid < end && bid >= end - n) { sh[4] = s; sh[5] = bid - (end - n); }
+        if (n > 0 && bid < end && bid >= end - n) { sh[8] = s; sh[9] = bid - (end - n); }
         __syncthreads();
-        const int found = sh[4], tile = sh[5];
+        const int found = sh[8], tile = sh[9];
         __syncthreads();
         if (found >= 0) return {__builtin_amdgcn_readfirstlane(found), __builtin_amdgcn_readfirstlane(tile), 0};
         base += tot;
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(NW * 64) void fwd_kernel(const AttnArgs a) {
     constexpr int NTHR = NW * 64, BM = NW * NT * 16, BN = 64, LD = DP + Tile<T>::PAD, CK = DP / 32, CD = DP / 16;
     __shared__ __attribute__((aligned(16))) T sk[BN * LD];
     __shared__ __attribute__((aligned(16))) T sv[BN * LD];
-    __shared__ int sh[8];
+    __shared__ int sh[16];
     const int kvh = blockIdx.x % a.kv_heads, bid = blockIdx.x / a.kv_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane >> 4;
     const Where w = locate<NTHR>(a.cu_q, a.seqs, a.tokens_q, a.group, BM, bid, sh);
     if (w.seq < 0) {
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(const AttnArgs a) {
     constexpr int NTHR = NW * 64, BM = NW * NT * 16, BN = 32, LD = DP + Tile<T>::PAD, CK = DP / 32, CD = DP / 16;
     __shared__ __attribute__((aligned(16))) T sk[BN * LD];
     __shared__ __attribute__((aligned(16))) T sv[BN * LD];
-    __shared__ int sh[8];
+    __shared__ int sh[16];
     const int kvh = blockIdx.x % a.kv_heads, bid = blockIdx.x / a.kv_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane >> 4;
     const Where w = locate<NTHR>(a.cu_q, a.seqs, a.tokens_q, a.group, BM, bid, sh);
     if (w.seq < 0) {
@@ -525,7 +525,7 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(const AttnArgs a) {
     __shared__ __attribute__((aligned(16))) float slse[BR];
     __shared__ __attribute__((aligned(16))) float sdel[BR];
     __shared__ int ssee[BR];
-    __shared__ int sh[8];
+    __shared__ int sh[16];
     const int kvh = blockIdx.x % a.kv_heads, bid = blockIdx.x / a.kv_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane >> 4;
     const Where w = locate<NTHR>(a.cu_k, a.seqs, a.tokens_k, 1, BK, bid, sh);
     if (w.seq < 0) {
@@ -676,44 +676,6 @@ int launch_dkv(const AttnArgs& a, hipStream_t st) {
     const dim3 grid(blocks_for(a, a.tokens_k, NW * NT * 16));
     hipLaunchKernelGGL((dkv_kernel<T, DP, NW, NT>), grid, dim3(NW * 64), 0, st, a);
     return launch_status("attention_packed_bwd");
-}
-
-// rows (or keys) of an average sequence decide the tile: one wave of 16 rows for single tokens, 64 or 128 rows otherwise
-template <typename T, int DP>
-int fwd_dim(const AttnArgs& a, hipStream_t st) {
-    const long long rows = (long long)a.tokens_q * a.group / a.seqs;
-    if (rows <= 16) return launch_fwd<T, DP, 1, 1>(a, st);
-    if (rows <= 96 || sizeof(T) == 4) return launch_fwd<T, DP, 4, 1>(a, st);
-    return launch_fwd<T, DP, 4, 2>(a, st);
-}
-
-template <typename T, int DP>
-int bwd_dim(const AttnArgs& a, hipStream_t st) {
-    const long long rows = (long long)a.tokens_q * a.group / a.seqs, keys = a.tokens_k / a.seqs;
-    int rc;
-    if (rows <= 16) rc = launch_dq<T, DP, 1, 1>(a, st);
-    else if (rows <= 96 || sizeof(T) == 4) rc = launch_dq<T, DP, 4, 1>(a, st);
-    else rc = launch_dq<T, DP, 4, 2>(a, st);
-    if (rc) return rc;
-    if (keys <= 16) return launch_dkv<T, DP, 1, 1>(a, st);
-    if (keys <= 96 || sizeof(T) == 4) return launch_dkv<T, DP, 4, 1>(a, st);
-    return launch_dkv<T, DP, 4, 2>(a, st);
-}
-
-template <typename T>
-int fwd(const AttnArgs& a, hipStream_t st) {
-    if (a.dim <= 32) return fwd_dim<T, 32>(a, st);
-    if (a.dim <= 64) return fwd_dim<T, 64>(a, st);
-    return fwd_dim<T, 128>(a, st);
-}
-
-template <typename T>
-int bwd(const AttnArgs& a, hipStream_t st) {
-    const long long rows = (long long)a.tokens_q * a.heads;
-    if (rows > 0) hipLaunchKernelGGL((delta_kernel<T>), dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, st, a);
-    if (a.dim <= 32) return bwd_dim<T, 32>(a, st);
-    if (a.dim <= 64) return bwd_dim<T, 64>(a, st);
-    return bwd_dim<T, 128>(a, st);
 }
 
 }  // namespace attn

@@ -1,5 +1,6 @@
-// Attention over packed sequences for _Float16 tensors (the kernels: attn_packed.hpp).
-#include "attn_packed.hpp"
+// Attention over packed sequences for fp16 tensors (the kernels: attn_packed.hpp, attn_packed_wide.hpp).
+#include "attn_packed_wide.hpp"
+#include "attn_packed_dispatch.hpp"
 
 namespace icap {
 

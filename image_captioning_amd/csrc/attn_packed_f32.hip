@@ -1,5 +1,6 @@
-// Attention over packed sequences for float tensors (the kernels: attn_packed.hpp).
-#include "attn_packed.hpp"
+// Attention over packed sequences for fp32 tensors (the kernels: attn_packed.hpp).
+#include "attn_packed_wide.hpp"
+#include "attn_packed_dispatch.hpp"
 
 namespace icap {
 

@@ -226,6 +226,12 @@ static int attention_check(const char* what, int dtype, const AttnArgs& a) {
         set_error("%s: q, k, v must be 16-byte aligned, their strides multiples of 16 bytes", what);
         return ICAP_ERR_ALIGN;
     }
+    // offsets within a tile of rows are 32-bit numbers
+    if (a.q_tok < 0 || a.q_head < 0 || a.k_tok < 0 || a.k_head < 0 || a.v_tok < 0 || a.v_head < 0 || a.q_tok > (1 << 24) || a.k_tok > (1 << 24) || a.v_tok > (1 << 24) ||
+        a.q_head * (a.heads / a.kv_heads) > (1 << 30)) {
+        set_error("%s: strides beyond 2^24 elements a token", what);
+        return ICAP_ERR_LIMIT;
+    }
     // rows (tokens x heads) and workgroups are counted in 32 bits
     if ((long long)a.tokens_q * a.heads > (1ll << 30) || (long long)a.tokens_k * a.kv_heads > (1ll << 30) || a.seqs > (1 << 24) ||
         ((long long)a.seqs + 1) * a.kv_heads > (1ll << 30)) {
@@ -1126,6 +1132,7 @@ int icap_attention_packed_bwd(int dtype, const void* dout, const void* q, const 
         set_error("attention_packed_bwd: null tensor");
         return ICAP_ERR_ARG;
     }
+    if (g_tok < 0 || g_head < 0 || g_tok > (1 << 24) || g_head * a.group > (1 << 30)) { set_error("attention_packed_bwd: strides of dout beyond 2^24 elements a token"); return ICAP_ERR_LIMIT; }
     const int e = dtype == DT_F32 ? 4 : 8;
     if (!aligned16(dout) || !aligned16(out) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) || g_tok % e || g_head % e) {
         set_error("attention_packed_bwd: tensors must be 16-byte aligned, strides multiples of 16 bytes");

@@ -1033,7 +1033,8 @@ def _packed_rows(t):
     """t [tokens, heads, dim] as the attention kernels read it (last axis contiguous, 16-byte aligned rows; a slice of a fused
     projection is), a contiguous copy otherwise."""
     per = 16 // t.element_size()
-    if t.stride(2) == 1 and t.stride(0) % per == 0 and t.stride(1) % per == 0 and t.data_ptr() % 16 == 0:
+    if (t.stride(2) == 1 and t.stride(0) % per == 0 and t.stride(1) % per == 0 and t.data_ptr() % 16 == 0 and t.stride(0) <= 1 << 24
+            and t.stride(1) * t.size(1) <= 1 << 30):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()

@@ -599,8 +599,8 @@ def test_training_steps_of_a_decoder_on_packed_captions():
         mine.step()
     for p, r in zip(net.parameters(), ref.parameters()):
         # where a gradient's size is that of its own rounding the update's sign is open: three steps of 1e-3 bound every value
-        assert float((p.double().cpu() - r).abs().max()) <= 2 * 3 * 1e-3 * 1.05
-        assert float((p.double().cpu() - r).norm()) < 2e-3 * float(r.norm() + 1e-2)
+        assert float((p.detach().double().cpu() - r.detach()).abs().max()) <= 2 * 3 * 1e-3 * 1.05
+        assert float((p.detach().double().cpu() - r.detach()).norm()) < 2e-3 * float(r.detach().norm() + 1e-2)
 
 
 def test_captured_step_replays_with_new_inputs():
