@@ -2,13 +2,27 @@
 // gradients, for one element type T.
 //   S = scale q k^T (keys after a query's place hidden when causal, places aligned at the sequences' ENDS), P = softmax(S), O = P V
 //   dV = P^T dO,  dS = P (dO V^T - rowsum(dO O)),  dQ = scale dS K,  dK = scale dS^T Q
-// Query heads that share a key head are rows of one matrix: row r of a sequence is (token r / group, head r % group).  A key
-// is then read once for the whole group, the single-token form fills a 16-row tile with its group, and dK / dV sum over the
-// group inside one workgroup, in a fixed order, without atomics.
-// One pass over the keys with a running maximum and sum.  The products are formed transposed (S^T = K Q^T, O^T = V^T P^T), so
-// that a query is a column (lane % 16) of every accumulator: its maximum, sum and rescaling stay in the lane, and the
-// accumulator of S^T is, register for register, the B operand of the next product (its 4-row groups only permute the
-// contraction, and V^T is read in the same order).  Rows that see no key get zeros (and a log-sum of -inf).
+// Query heads that share a key head are rows of one matrix: row r is (token r / group, head r % group).  A key is read once
+// for the whole group, and dK / dV sum over it inside one workgroup, in a fixed order, without atomics.
+// Tiles are consecutive rows (keys, for dK and dV) of the packed tensors, WHATEVER sequences they belong to: every row knows
+// the range of keys it sees (every key the range of rows that see it), a tile walks over the union of its rows' ranges, and
+// the rest is masked.  Short captions fill tiles together, single tokens of many texts too, and no tile is empty.
+//
+// One pass over the keys with a running maximum and sum.  The products are formed transposed (S^T = K Q^T, O^T = V^T P^T) on
+// 32 x 32 x 16 matrix instructions, so that a query is a column (lane % 32) of every accumulator: its maximum, sum and
+// rescaling stay in the lane, and the eight values a lane half holds of 16 accumulator rows are the B operand of the next product as
+// they come (V^T is read in the same order of the contraction).  Rows that see no key get zeros (and a log-sum of -inf).
+//
+// What bounds it: at dim 128 a wave of 32 rows needs per 64 keys 1024 cycles of its SIMD's matrix core, about as many of
+// its vector unit (32 exponentials of 16 cycles) and a quarter of that of the CU's LDS (32 KB at 128 bytes a cycle).  So two waves a
+// SIMD interleave (four-wave workgroups, two a CU: with one of eight waves all were in the same phase, 404 against 383 us on
+// 12k tokens of bf16 prompts), the scores of the next step are formed beside the exponentials of this one (353 us), and nothing
+// else stays in the loop:
+//   * tiles go global -> LDS without registers, double-buffered, one barrier a step;
+//   * LDS rows are not padded (the direct loads write linearly) but permuted in 16-byte slots by swizzle(), which spreads the 8
+//     rows of a fragment read and the 4 rows of a transposing read over different banks;
+//   * the running maximum is only followed when it grows by more than 2^8 (weights stay below 256, sums in fp32, so nothing
+//     is lost), which leaves the accumulators alone in almost every step.
 #pragma once
 #include "packed.hpp"
 
@@ -17,149 +31,137 @@ namespace attn {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
-template <typename T> struct Tile {
-    static constexpr int PAD = 16 / sizeof(T);      // one 16-byte slot a row: the 16 rows of a fragment read start in different banks
-};
+// acc[32 x 32] += A[32 x 16] B[16 x 32]: a lane brings eight values of A's row and of B's column lane % 32; acc: column lane % 32,
+// register e is row acc_row(e) + 4 (lane / 32).  fp32: slot j of all lanes is one 2-deep product.
+__device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma32(f32x8 a, f32x8 b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ constexpr int acc_row(int e) { return (e & 3) + 8 * (e >> 2); }
 
-// rows of 16-byte pieces: [ROWS][DP] of a packed tensor between global memory and LDS, through registers
+__device__ __forceinline__ f32x16 zeros16() {
+    f32x16 z;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) z[e] = 0.f;
+    return z;
+}
+
+__device__ __forceinline__ int cut(int v, int lo, int hi) { return min(max(v, lo), hi); }
+
+// ------------------------------------------------------------------------------------------------ tiles in LDS
+// permutation of a row's 16-byte slots.  Rows of 256 bytes and more all begin at bank 0, rows of 128 and 64 bytes share a bank line two
+// and four at a time; in 16-bit tiles the lowest bit moves by the third row bit, so that the 32-byte pieces of four
+// consecutive rows, which a transposing read takes together, lie apart.
+template <typename T, int DP>
+__device__ __forceinline__ int swizzle(int row) {
+    if constexpr (sizeof(T) == 4) return DP == 32 ? (row >> 1) & 3 : row & 7;
+    else if constexpr (DP == 128) return ((row & 3) << 1) | ((row >> 2) & 1);
+    else if constexpr (DP == 64) return (((row >> 1) & 1) << 1) | ((row >> 2) & 1);
+    else return (row >> 2) & 1;
+}
+
+// [ROWS][DP] values, global -> LDS
 template <typename T, int ROWS, int DP, int NTHR>
-struct Stage {
-    static constexpr int EPC = 16 / sizeof(T), CH = DP / EPC, N = (ROWS * CH + NTHR - 1) / NTHR, LD = DP + Tile<T>::PAD;
-    u32x4 r[N];
-    // src: row 0, rows `stride` elements apart; valid >= 1 rows exist, the others and columns from dim on become zeros
-    __device__ __forceinline__ void load(const T* src, long long stride, int valid, int dim) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = threadIdx.x + i * NTHR, row = c / CH, col = (c % CH) * EPC;
-            const T* p = src + (long long)min(row, valid - 1) * stride + (col < dim ? col : 0);
-            u32x4 x = *reinterpret_cast<const u32x4*>(p);
-            const unsigned keep = (row < valid && col < dim) ? 0xffffffffu : 0u;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] &= keep;
-            r[i] = x;
-        }
-    }
-    // rows that are (token, head of the group) pairs
-    __device__ __forceinline__ void load_rows(const T* src, long long tok, long long head, int group, int row0, int nrow, int dim) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = threadIdx.x + i * NTHR, row = row0 + c / CH, col = (c % CH) * EPC;
-            const int rr = min(row, nrow - 1), t = rr / group;
-            const T* p = src + (long long)t * tok + (long long)(rr - t * group) * head + (col < dim ? col : 0);
-            u32x4 x = *reinterpret_cast<const u32x4*>(p);
-            const unsigned keep = (row < nrow && col < dim) ? 0xffffffffu : 0u;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] &= keep;
-            r[i] = x;
-        }
-    }
-    __device__ __forceinline__ void store(T* lds) const {
+struct Direct {
+    static constexpr int EPC = 16 / sizeof(T), CH = DP / EPC, PIECES = ROWS * CH, N = PIECES < NTHR ? 1 : PIECES / NTHR;
+    static_assert(PIECES < NTHR ? PIECES % 64 == 0 : PIECES % NTHR == 0, "whole passes, or whole waves of one");
+    int row[N], col[N];
+    __device__ __forceinline__ void init(int dim) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = threadIdx.x + i * NTHR;
-            if (ROWS * CH % NTHR != 0 && c >= ROWS * CH) break;
-            *reinterpret_cast<u32x4*>(lds + (c / CH) * LD + (c % CH) * EPC) = r[i];
+            row[i] = c / CH;
+            const int s = ((c % CH) ^ swizzle<T, DP>(row[i])) * EPC;
+            col[i] = s < dim ? s : 0;           // columns behind dim meet zeros of the other operand
+        }
+    }
+    __device__ __forceinline__ void put(const T* p, int i, T* lds) const {
+        if (PIECES < NTHR && threadIdx.x >= PIECES) return;         // a short tile does not need every wave
+        __builtin_amdgcn_global_load_lds(p, (__attribute__((address_space(3))) void*)(lds + ((threadIdx.x >> 6) * 64 + i * NTHR) * EPC), 16, 0, 0);
+    }
+    // rows first .. of `valid` (>= 1) rows that are `stride` apart; rows outside repeat the nearest one (they are masked)
+    __device__ __forceinline__ void load(const T* src, long long stride, int first, int valid, T* lds) const {
+        const T* p = src + first * stride;
+#pragma unroll
+        for (int i = 0; i < N; ++i) put(p + (cut(row[i], -first, valid - 1 - first) * (int)stride + col[i]), i, lds);
+    }
+    // rows that are (token, head of the group) pairs
+    __device__ __forceinline__ void load_rows(const T* src, int tok, int head, int group, int row0, int end, T* lds) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = min(row0 + row[i], end - 1), t = r / group;
+            put(src + (long long)t * tok + ((r - t * group) * head + col[i]), i, lds);
         }
     }
 };
 
-// fragment of a row-major LDS tile whose rows are the matrix rows: row row0 + lane % 16, columns 32 c + 8 (lane / 16) .. + 7
-template <typename T, int LD>
-__device__ __forceinline__ typename Vec<T>::x8 row_frag(const T* lds, int row0, int c) {
-    const int lane = threadIdx.x & 63;
-    return *reinterpret_cast<const typename Vec<T>::x8*>(lds + (row0 + (lane & 15)) * LD + c * 32 + (lane >> 4) * 8);
+// everything this wave asked for has landed, and every wave is here
+__device__ __forceinline__ void landed() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
-// fragment of the same tile transposed: matrix row = tile column col0 + lane % 16; the contraction runs over the 32 tile rows
-// from row0, in the order of an accumulator's registers: slots 0-3 are rows 4 (lane / 16) + 0..3, slots 4-7 the same + 16.
-// 16-bit types: the transposing LDS read, which hands lane l of 16 column l of the 4 x 16 block its 16 lanes address.
-template <typename T, int LD>
+// fragment whose matrix rows are tile rows: row row0 + lane % 32, columns 16 kk + 8 (lane / 32) .. + 7
+template <typename T, int DP>
+__device__ __forceinline__ typename Vec<T>::x8 row_frag(const T* lds, int row0, int kk) {
+    const int lane = threadIdx.x & 63, r = lane & 31, lh = lane >> 5, f = swizzle<T, DP>(r);
+    const T* p = lds + (row0 + r) * DP;
+    if constexpr (sizeof(T) == 2) return *reinterpret_cast<const typename Vec<T>::x8*>(p + ((kk * 2 + lh) ^ f) * 8);
+    else {
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(p + ((kk * 4 + lh * 2) ^ f) * 4), hi = *reinterpret_cast<const f32x4*>(p + ((kk * 4 + lh * 2 + 1) ^ f) * 4);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+}
+
+// transposed: matrix row = tile column col0 + lane % 32; the contraction runs over 16 tile rows in the order of an accumulator's
+// eight registers: rows {0-3, 8-11} + 4 (lane / 32).  16-bit types: the transposing LDS read, which hands lane l of 16 column l of the
+// 4 x 16 block that its 16 lanes address.
+template <typename T, int DP>
 __device__ __forceinline__ typename Vec<T>::x8 col_frag(const T* lds, int row0, int col0) {
-    const int lane = threadIdx.x & 63, l = lane & 15, grp = lane >> 4;
+    const int lane = threadIdx.x & 63, lh = lane >> 5;
     if constexpr (sizeof(T) == 2) {
-        const T* p = lds + (row0 + grp * 4 + (l >> 2)) * LD + col0 + (l & 3) * 4;
+        const int l = lane & 15, half = (lane >> 4) & 1, r = 4 * lh + (l >> 2), slot = (col0 >> 3) + half * 2 + ((l & 3) >> 1);
+        const T* p = lds + (row0 + r) * DP + (slot ^ swizzle<T, DP>(r)) * 8 + (l & 1) * 4;
         typedef __attribute__((address_space(3))) i16x4* lds_ptr;
         const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p));
-        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 16 * LD));
+        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * DP));
         typedef short i16x8 __attribute__((ext_vector_type(8)));
         const i16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         return __builtin_bit_cast(typename Vec<T>::x8, both);
     } else {
-        const T* p = lds + (row0 + grp * 4) * LD + col0 + l;
+        const int col = col0 + (lane & 31);
         typename Vec<T>::x8 f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { f[j] = p[j * LD]; f[4 + j] = p[(16 + j) * LD]; }
+        for (int j = 0; j < 8; ++j) {
+            const int r = (j & 3) + 8 * (j >> 2) + 4 * lh;
+            f[j] = lds[(row0 + r) * DP + ((col >> 2) ^ swizzle<T, DP>(r)) * 4 + (col & 3)];
+        }
         return f;
     }
 }
 
-// two accumulators (tile rows 0-15 and 16-31 of a 32-row step) as the operand of the product that contracts those rows
+// eight registers of an accumulator (16 of its rows) as an operand: the one rounding of P and dS to a 16-bit type (2^-9 / 2^-12 of
+// each value, as much as the result's own rounding; the sums beside them are taken from the unrounded values)
 template <typename T>
-__device__ __forceinline__ typename Vec<T>::x8 acc_frag(f32x4 a, f32x4 b) {
-    if constexpr (sizeof(T) == 4) return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-    else return __builtin_convertvector(__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7), typename Vec<T>::x8);
+__device__ __forceinline__ typename Vec<T>::x8 acc_frag(const f32x16& a, int half) {
+    f32x8 x;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = a[half * 8 + e];
+    if constexpr (sizeof(T) == 4) return x;
+    else return __builtin_convertvector(x, typename Vec<T>::x8);
 }
 
-// fragment of a global row: columns 32 c + 8 (lane / 16) .. + 7, zeros from dim on and when !ok (p stays readable)
+// fragment of a row in memory: columns 16 kk + 8 (lane / 32) .. + 7, zeros from dim on and when !ok (p stays readable)
 template <typename T>
-__device__ __forceinline__ typename Vec<T>::x8 global_frag(const T* row, int c, int dim, bool ok) {
-    const int col = c * 32 + ((threadIdx.x & 63) >> 4) * 8;
+__device__ __forceinline__ typename Vec<T>::x8 global_frag(const T* row, int kk, int dim, bool ok) {
+    const int col = kk * 16 + ((threadIdx.x & 63) >> 5) * 8;
     typename Vec<T>::x8 f = *reinterpret_cast<const typename Vec<T>::x8*>(row + (col < dim ? col : 0));
     if (!(ok && col < dim)) f = typename Vec<T>::x8{};
     return f;
-}
-
-struct Where { int seq, tile, used; };
-
-// Which sequence and which of its tiles workgroup `bid` owns, from the running sum of the sequences' tile counts; every thread
-// looks at one sequence.  seq = -1: behind the last tile; used = the number of tiles there are.  Lengths are bounded by
-// `tokens`, so a wrong list of offsets reads and writes nothing outside the tensors.  sh: 16 ints of LDS.
-template <int NTHR>
-__device__ __forceinline__ Where locate(const int* cu, int seqs, int tokens, int per_token, int rows, int bid, int* sh) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int base = 0;
-    for (int s0 = 0; s0 < seqs; s0 += NTHR) {
-        const int s = s0 + tid;
-        int n = 0;
-        if (s < seqs) {
-            const int a = min(max(cu[s], 0), tokens), b = min(max(cu[s + 1], a), tokens);
-            n = ((b - a) * per_token + rows - 1) / rows;
-        }
-        int inc = n;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) { const int t = __shfl_up(inc, d); if (lane >= d) inc += t; }
-        if (lane == 63) sh[wave] = inc;
-        if (tid == 0) sh[8] = -1;
-        __syncthreads();
-        int pre = 0, tot = 0;
-#pragma unroll
-        for (int w = 0; w < NTHR / 64; ++w) { const int t = sh[w]; if (w < wave) pre += t; tot += t; }
-        const int end = base + pre + inc;
-        if (n > 0 && bid < end && bid >= end - n) { sh[8] = s; sh[9] = bid - (end - n); }
-        __syncthreads();
-        const int found = sh[8], tile = sh[9];
-        __syncthreads();
-        if (found >= 0) return {__builtin_amdgcn_readfirstlane(found), __builtin_amdgcn_readfirstlane(tile), 0};
-        base += tot;
-    }
-    return {-1, 0, base};
-}
-
-__device__ __forceinline__ void range_of(const int* cu, int s, int tokens, int& begin, int& n) {
-    begin = min(max(cu[s], 0), tokens);
-    n = min(max(cu[s + 1], begin), tokens) - begin;
-}
-
-// rows that belong to no sequence (behind the last one) get zeros, from the workgroups that own no tile
-template <typename T, int NTHR>
-__device__ __forceinline__ void clear_behind(T* dst, float* lse, int first, int tokens, int heads, int dim, int id, int ids) {
-    const long long per = (long long)heads * dim, n = (tokens - first) * per;
-    T* p = dst + first * per;
-    for (long long i = (long long)id * NTHR + threadIdx.x; i < n / 8; i += (long long)ids * NTHR)
-        *reinterpret_cast<typename Vec<T>::x8*>(p + i * 8) = typename Vec<T>::x8{};
-    if (lse)
-        for (long long i = (long long)id * NTHR + threadIdx.x; i < (long long)(tokens - first) * heads; i += (long long)ids * NTHR)
-            lse[(long long)first * heads + i] = -INFINITY;
 }
 
 template <typename T>
@@ -168,191 +170,235 @@ __device__ __forceinline__ void store4(T* p, f32x4 v) {
     else *reinterpret_cast<typename Vec<T>::x4*>(p) = __builtin_convertvector(v, typename Vec<T>::x4);
 }
 
-__device__ __forceinline__ float across_groups_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
-}
-__device__ __forceinline__ float across_groups_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+// one lane's 16 values of a result row (columns col0 + acc_row(e) + 4 (lane / 32)), four at a time
+template <typename T>
+__device__ __forceinline__ void store16(T* p, int col0, int dim, const f32x16& v, float f) {
+    const int lh = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int d = col0 + 8 * g + 4 * lh;
+        if (d < dim) store4<T>(p + d, f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]} * f);
+    }
 }
 
-// Split keys: workgroup z takes a share of the keys (whole steps, at least two of them, so that short sequences are not split)
-template <int BN>
-__device__ __forceinline__ void split_range(int keys, int splits, int z, int& lo, int& hi) {
-    const int steps = (keys + BN - 1) / BN, per = max((steps + splits - 1) / splits, splits > 1 ? 2 : 1) * BN;
-    lo = min(z * per, keys);
-    hi = min(lo + per, keys);
+// ------------------------------------------------------------------------------------------------ who sees whom
+struct Span { int lo, hi; };
+
+// the last sequences that begin at or before places x and y (x <= y), by all 64 lanes of a wave: 64 offsets at a time, two loads for up
+// to 4096 sequences
+__device__ __forceinline__ void find_two(const int* cu, int seqs, int x, int y, int& sx, int& sy) {
+    const int lane = threadIdx.x & 63;
+    int lx = 0, nx = seqs, ly = 0, ny = seqs;
+    while (nx > 1 || ny > 1) {
+        const int ax = (nx + 63) >> 6, ay = (ny + 63) >> 6;
+        const bool ox = lane * ax < nx && cu[lx + lane * ax] <= x, oy = lane * ay < ny && cu[ly + lane * ay] <= y;
+        const int px = max(__popcll(__ballot(ox)) - 1, 0) * ax, py = max(__popcll(__ballot(oy)) - 1, 0) * ay;
+        lx += px;
+        nx = min(ax, nx - px);
+        ly += py;
+        ny = min(ay, ny - py);
+    }
+    sx = __builtin_amdgcn_readfirstlane(lx);
+    sy = __builtin_amdgcn_readfirstlane(ly);
+}
+// the same for a lane of its own, between sequences a and b
+__device__ __forceinline__ int find_between(const int* cu, int x, int a, int b) {
+    while (a < b) {
+        const int mid = (a + b + 1) >> 1;
+        if (cu[mid] <= x) a = mid; else b = mid - 1;
+    }
+    return a;
+}
+
+// The keys that a token sees, and the rows that see a key, from the offsets of sequence s (which may be wrong: they are cut off at the
+// tensors' ends, and a place outside its sequence sees nothing, so nothing outside is read or written)
+struct Edge { int q0, q1, k0, k1; };
+__device__ __forceinline__ Edge edge_of(const AttnArgs& a, int s) {
+    Edge e;
+    e.q0 = cut(a.cu_q[s], 0, a.tokens_q);
+    e.q1 = cut(a.cu_q[s + 1], e.q0, a.tokens_q);
+    e.k0 = cut(a.cu_k[s], 0, a.tokens_k);
+    e.k1 = cut(a.cu_k[s + 1], e.k0, a.tokens_k);
+    return e;
+}
+__device__ __forceinline__ Span keys_of(const AttnArgs& a, const Edge& e, int t) {
+    if (t < e.q0 || t >= e.q1) return {e.k0, e.k0};
+    return {e.k0, a.causal ? cut(e.k1 - (e.q1 - 1 - t), e.k0, e.k1) : e.k1};
+}
+__device__ __forceinline__ Span rows_of(const AttnArgs& a, const Edge& e, int j) {
+    if (j < e.k0 || j >= e.k1) return {e.q0 * a.group, e.q0 * a.group};
+    return {(a.causal ? cut(e.q1 - (e.k1 - j), e.q0, e.q1) : e.q0) * a.group, e.q1 * a.group};
+}
+
+// What the lanes of a wave see together: anything in [some.lo, some.hi), everything in [all.lo, all.hi)
+__device__ __forceinline__ int wave_min_i(int v) {
+    v = min(v, dpp_i<DPP_QUAD_SWAP1>(v));
+    v = min(v, dpp_i<DPP_QUAD_SWAP2>(v));
+    v = min(v, dpp_i<DPP_HALF_MIRROR>(v));
+    v = min(v, dpp_i<DPP_ROW_MIRROR>(v));
+    return min(min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)), min(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+struct Sight { Span mine, some, all; };
+__device__ __forceinline__ Sight sight_of(Span s) {
+    const bool none = s.lo >= s.hi;
+    Sight w;
+    w.mine = s;
+    w.some = {wave_min_i(none ? 0x7fffffff : s.lo), -wave_min_i(none ? 0x7fffffff : -s.hi)};
+    w.all = {-wave_min_i(-s.lo), wave_min_i(s.hi)};
+    return w;
+}
+
+// A tile of `rows` rows (token, head) from row0: the keys that any of them sees, and what this lane's row sees
+template <int ROWS>
+__device__ __forceinline__ Span tile_keys(const AttnArgs& a, int row0, int row, Sight& sight) {
+    const int total = a.tokens_q * a.group, end = cut(a.cu_q[a.seqs], 0, a.tokens_q);
+    const int t0 = row0 / a.group, t1 = min(min(row0 + ROWS, total) - 1, end * a.group - 1) / a.group;
+    if (t0 >= end) { sight = sight_of({0, 0}); return {0, 0}; }          // behind the last sequence
+    int s0, s1;
+    find_two(a.cu_q, a.seqs, t0, t1, s0, s1);
+    const int t = min(row, total - 1) / a.group;
+    const Edge e = edge_of(a, find_between(a.cu_q, min(t, t1), s0, s1));
+    sight = sight_of(row < total ? keys_of(a, e, t) : Span{e.k0, e.k0});
+    const Edge e0 = edge_of(a, s0), e1 = edge_of(a, s1);
+    return {e0.k0, keys_of(a, e1, t1).hi};
+}
+// A tile of keys from key0: the rows that see any of them, and the ones that see this lane's key
+template <int KEYS>
+__device__ __forceinline__ Span tile_rows(const AttnArgs& a, int key0, int key, Sight& sight) {
+    const int end = cut(a.cu_k[a.seqs], 0, a.tokens_k);
+    const int j1 = min(key0 + KEYS, end) - 1;
+    if (key0 >= end) { sight = sight_of({0, 0}); return {0, 0}; }
+    int s0, s1;
+    find_two(a.cu_k, a.seqs, key0, j1, s0, s1);
+    const Edge e = edge_of(a, find_between(a.cu_k, min(key, j1), s0, s1));
+    sight = sight_of(key < end ? rows_of(a, e, key) : Span{0, 0});
+    const Edge e0 = edge_of(a, s0), e1 = edge_of(a, s1);
+    return {rows_of(a, e0, key0).lo, rows_of(a, e1, j1).hi};
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// NW waves of NT x 16 rows each; 64 keys a step, staged through registers while the step before multiplies
-template <typename T, int DP, int NW, int NT>
-__global__ __launch_bounds__(NW * 64) void fwd_kernel(const AttnArgs a) {
-    constexpr int NTHR = NW * 64, BM = NW * NT * 16, BN = 64, LD = DP + Tile<T>::PAD, CK = DP / 32, CD = DP / 16;
-    __shared__ __attribute__((aligned(16))) T sk[BN * LD];
-    __shared__ __attribute__((aligned(16))) T sv[BN * LD];
-    __shared__ int sh[16];
-    const int kvh = blockIdx.x % a.kv_heads, bid = blockIdx.x / a.kv_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane >> 4;
-    const Where w = locate<NTHR>(a.cu_q, a.seqs, a.tokens_q, a.group, BM, bid, sh);
-    if (w.seq < 0) {
-        if (kvh == 0 && blockIdx.y == 0) {
-            int b0, n0;
-            range_of(a.cu_q, a.seqs - 1, a.tokens_q, b0, n0);
-            clear_behind<T, NTHR>((T*)a.out, a.lse, b0 + n0, a.tokens_q, a.heads, a.dim, bid - w.used, gridDim.x / a.kv_heads - w.used);
-        }
-        return;
-    }
-    int q0, nq, k0, nk;
-    range_of(a.cu_q, w.seq, a.tokens_q, q0, nq);
-    range_of(a.cu_k, w.seq, a.tokens_k, k0, nk);
-    const int nrow = nq * a.group, tiles = (nrow + BM - 1) / BM;
-    const int tile = a.causal ? tiles - 1 - w.tile : w.tile;            // the longest tiles of a sequence start first
-    const int row0 = tile * BM + wave * NT * 16, off = nk - nq;
-    const T* qb = (const T*)a.q + (long long)q0 * a.q_tok + (long long)kvh * a.group * a.q_head;
-    const T* kb = (const T*)a.k + (long long)k0 * a.k_tok + (long long)kvh * a.k_head;
-    const T* vb = (const T*)a.v + (long long)k0 * a.v_tok + (long long)kvh * a.v_head;
+template <typename T> constexpr int step_keys() { return sizeof(T) == 4 ? 32 : 64; }       // keys (rows) staged at a time
 
-    int tok[NT], hd[NT], see[NT];           // this lane's row: token, head of the group, number of keys it sees
-    typename Vec<T>::x8 qf[NT][CK];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int r = row0 + t * 16 + (lane & 15), rr = min(r, nrow - 1);
-        tok[t] = rr / a.group;
-        hd[t] = rr - tok[t] * a.group;
-        see[t] = r < nrow ? (a.causal ? min(nk, max(tok[t] + off + 1, 0)) : nk) : 0;
-        const T* p = qb + (long long)tok[t] * a.q_tok + (long long)hd[t] * a.q_head;
-#pragma unroll
-        for (int c = 0; c < CK; ++c) qf[t][c] = global_frag<T>(p, c, a.dim, r < nrow);
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64, DP == 128 && (NW < 4 || sizeof(T) == 4) ? 1 : 2) void fwd_kernel(const AttnArgs a) {
+    constexpr int NTHR = NW * 64, BM = NW * 32, BN = step_keys<T>(), NS = BN / 32, KK = DP / 16, ND = DP / 32;
+    __shared__ __attribute__((aligned(1024))) T sk[2][BN * DP];
+    __shared__ __attribute__((aligned(1024))) T sv[2][BN * DP];
+    const int kvh = blockIdx.x % a.kv_heads, tiles = gridDim.x / a.kv_heads, lane = threadIdx.x & 63, lh = lane >> 5;
+    // causal: the rows of a sequence's end see most keys and start first
+    const int tile = a.causal ? tiles - 1 - (int)(blockIdx.x / a.kv_heads) : blockIdx.x / a.kv_heads;
+    const int row0 = tile * BM, row = row0 + (threadIdx.x >> 6) * 32 + (lane & 31), total = a.tokens_q * a.group;
+    const int tok = min(row, total - 1) / a.group, head = kvh * a.group + min(row, total - 1) - tok * a.group;
+    Sight me;
+    Span keys = tile_keys<BM>(a, row0, row, me);
+    if (a.splits > 1) {             // the part of the keys that this workgroup takes: whole steps, at least two of them
+        const int steps = (keys.hi - keys.lo + BN - 1) / BN, per = max((steps + a.splits - 1) / a.splits, 2) * BN;
+        keys.lo = min(keys.lo + (int)blockIdx.y * per, keys.hi);
+        keys.hi = min(keys.lo + per, keys.hi);
     }
-    // keys that any row of the workgroup sees, any row of this wave sees, and all rows of this wave see (no mask needed there)
-    const int last = min((tile * BM + BM - 1) / a.group, nq - 1);
-    const int keys = a.causal ? min(nk, max(last + off + 1, 0)) : nk;
-    const int wlast = min((row0 + NT * 16 - 1) / a.group, nq - 1);
-    const int wkeys = row0 < nrow ? (a.causal ? min(nk, max(wlast + off + 1, 0)) : nk) : 0;
-    const int wfull = row0 + NT * 16 <= nrow ? (a.causal ? min(nk, max(row0 / a.group + off + 1, 0)) : nk) : 0;
-    int lo, hi;
-    split_range<BN>(keys, a.splits, blockIdx.y, lo, hi);
+    const T* qp = (const T*)a.q + (long long)tok * a.q_tok + (long long)head * a.q_head;
+    // places from here on are counted from the tile's first key
+    const T* kb = (const T*)a.k + (long long)keys.lo * a.k_tok + (long long)kvh * a.k_head;
+    const T* vb = (const T*)a.v + (long long)keys.lo * a.v_tok + (long long)kvh * a.v_head;
+    const int nk = keys.hi - keys.lo, full_lo = me.all.lo - keys.lo, full_hi = me.all.hi - keys.lo;
+    const int see_lo = me.mine.lo - keys.lo - 4 * lh, see_hi = me.mine.hi - keys.lo - 4 * lh;
+    typename Vec<T>::x8 qf[KK];
+#pragma unroll
+    for (int c = 0; c < KK; ++c) qf[c] = global_frag<T>(qp, c, a.dim, row < total);
 
-    f32x4 o[CD][NT];
-    float m[NT], l[NT];
+    f32x16 o[ND];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        m[t] = -INFINITY;
-        l[t] = 0.f;
-#pragma unroll
-        for (int d = 0; d < CD; ++d) o[d][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int d = 0; d < ND; ++d) o[d] = zeros16();
+    float m = -INFINITY, l = 0.f;
     const float c2 = a.scale * LOG2E;
-    Stage<T, BN, DP, NTHR> stk, stv;
-    if (lo < hi) {
-        stk.load(kb + (long long)lo * a.k_tok, a.k_tok, nk - lo, a.dim);
-        stv.load(vb + (long long)lo * a.v_tok, a.v_tok, nk - lo, a.dim);
+    // The scores of the next 32 keys are formed while the exponentials of these run, so K is staged 32 keys ahead of V: a step of
+    // V's keys n0 .. n0 + BN goes with K's n0 + 32 .. n0 + BN + 32
+    Direct<T, BN, DP, NTHR> dir;
+    dir.init(a.dim);
+    auto load = [&](int n0, int buf) __attribute__((always_inline)) {
+        dir.load(kb, a.k_tok, n0 + 32, nk, sk[buf]);
+        dir.load(vb, a.v_tok, n0, nk, sv[buf]);
+    };
+    auto scores = [&](const T* tile, int row) __attribute__((always_inline)) {
+        f32x16 s = zeros16();
+#pragma unroll
+        for (int c = 0; c < KK; ++c) s = mma32(row_frag<T, DP>(tile, row, c), qf[c], s);
+        return s;
+    };
+    // `now`: scores of the 32 keys from n (rows vr of the V tile); returns those of the next 32 (rows kr of the K tile)
+    auto unit = [&](f32x16 now, int n, const T* vt, int vr, const T* kt, int kr) __attribute__((always_inline)) {
+        if (n < full_lo || n + 32 > full_hi) {
+            const int lo = see_lo - n, hi = see_hi - n;         // against constants: no register a place
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (acc_row(e) < lo || acc_row(e) >= hi) now[e] = -INFINITY;
+        }
+        float mx = now[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, now[e]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32)) * c2;
+        if (__any(mx > m + 8.0f)) {
+            const float mn = fmaxf(m, mx);
+            const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d] *= alpha;
+        }
+        const f32x16 next = scores(kt, kr);
+        const float base = m == -INFINITY ? 0.f : m;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(now[j * 8 + e], c2, -base));
+                now[j * 8 + e] = p;
+                sum += p;
+            }
+            const auto pf = acc_frag<T>(now, j);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d] = mma32(col_frag<T, DP>(vt, vr + j * 16, d * 32), pf, o[d]);
+        }
+        l += sum;
+        return next;
+    };
+    if (nk > 0) {
+        dir.load(kb, a.k_tok, 32 - BN, nk, sk[1]);              // its last 32 rows are the first keys
+        load(0, 0);
+        landed();
+        f32x16 s = scores(sk[1], BN - 32);
+        for (int n0 = 0, buf = 0; n0 < nk; n0 += BN, buf ^= 1) {
+            landed();
+            if (n0 + BN < nk) load(n0 + BN, buf ^ 1);
+#pragma unroll
+            for (int u = 0; u < NS; ++u) s = unit(s, n0 + 32 * u, sv[buf], 32 * u, sk[buf], 32 * u);
+        }
     }
-    for (int n0 = lo; n0 < hi; n0 += BN) {
-        stk.store(sk);
-        stv.store(sv);
-        __syncthreads();
-        if (n0 + BN < hi) {
-            stk.load(kb + (long long)(n0 + BN) * a.k_tok, a.k_tok, nk - n0 - BN, a.dim);
-            stv.load(vb + (long long)(n0 + BN) * a.v_tok, a.v_tok, nk - n0 - BN, a.dim);
-        }
-        if (n0 < wkeys) {
-            f32x4 s[4][NT];
+    const float sum = l + __shfl_xor(l, 32);
+    if (row >= total) return;
+    const long long at = (long long)tok * a.heads + head;
+    const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);        // no key: zeros; NaN stays
+    const float lse = sum > 0.f ? fmaf(m, LN2, logf(sum)) : (sum == 0.f ? -INFINITY : sum);
+    if (a.splits > 1) {
+        const long long rows = (long long)a.tokens_q * a.heads;
+        float* part = a.part + (rows * blockIdx.y + at) * a.dim;
 #pragma unroll
-            for (int kt = 0; kt < 4; ++kt) {
+        for (int d = 0; d < ND; ++d) store16<float>(part, d * 32, a.dim, o[d], inv);
+        if (lh == 0) a.part[rows * a.splits * a.dim + rows * blockIdx.y + at] = lse;
+    } else {
 #pragma unroll
-                for (int t = 0; t < NT; ++t) s[kt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < CK; ++c) {
-                    const auto kf = row_frag<T, LD>(sk, kt * 16, c);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) s[kt][t] = mma16(kf, qf[t][c], s[kt][t]);
-                }
-            }
-            if (n0 + BN > wfull) {
-#pragma unroll
-                for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (n0 + kt * 16 + grp * 4 + i >= see[t]) s[kt][t][i] = -INFINITY;
-            }
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                float mx = s[0][t][0];
-#pragma unroll
-                for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[kt][t][i]);
-                mx = across_groups_max(mx);
-                const float mn = fmaxf(m[t], mx * c2);
-                const float base = mn == -INFINITY ? 0.f : mn;
-                const float alpha = __builtin_amdgcn_exp2f(m[t] - base);
-                m[t] = mn;
-                float sum = 0.f;
-#pragma unroll
-                for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p = __builtin_amdgcn_exp2f(fmaf(s[kt][t][i], c2, -base));
-                        s[kt][t][i] = p;
-                        sum += p;
-                    }
-                l[t] = fmaf(l[t], alpha, sum);
-#pragma unroll
-                for (int d = 0; d < CD; ++d) o[d][t] *= alpha;
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                // P is rounded to T for the matrix cores (relative 2^-9 / 2^-12 of each weight, as much as the result's own rounding);
-                // the sum l is taken from the unrounded values
-                typename Vec<T>::x8 pf[NT];
-#pragma unroll
-                for (int t = 0; t < NT; ++t) pf[t] = acc_frag<T>(s[2 * h][t], s[2 * h + 1][t]);
-#pragma unroll
-                for (int d = 0; d < CD; ++d) {
-                    const auto vf = col_frag<T, LD>(sv, h * 32, d * 16);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) o[d][t] = mma16(vf, pf[t], o[d][t]);
-                }
-            }
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int r = row0 + t * 16 + (lane & 15);
-        const float sum = across_groups_sum(l[t]);
-        const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
-        if (r >= nrow) continue;
-        const long long at = (long long)(q0 + tok[t]) * a.heads + kvh * a.group + hd[t];
-        const float lse = sum > 0.f ? fmaf(m[t], LN2, logf(sum)) : (sum == 0.f ? -INFINITY : sum);
-        if (a.splits > 1) {
-            const long long rows = (long long)a.tokens_q * a.heads;
-            float* po = a.part + (rows * blockIdx.y + at) * a.dim;
-#pragma unroll
-            for (int d = 0; d < CD; ++d)
-                if (d * 16 + grp * 4 < a.dim) *reinterpret_cast<f32x4*>(po + d * 16 + grp * 4) = o[d][t] * inv;
-            if (grp == 0) a.part[rows * a.splits * a.dim + rows * blockIdx.y + at] = lse;
-        } else {
-            T* po = (T*)a.out + at * a.dim;
-#pragma unroll
-            for (int d = 0; d < CD; ++d)
-                if (d * 16 + grp * 4 < a.dim) store4<T>(po + d * 16 + grp * 4, o[d][t] * inv);
-            if (grp == 0 && a.lse) a.lse[at] = lse;
-        }
+        for (int d = 0; d < ND; ++d) store16<T>((T*)a.out + at * a.dim, d * 32, a.dim, o[d], inv);
+        if (lh == 0 && a.lse) a.lse[at] = lse;
     }
 }
 
-// joins the shares of split keys: each is a normalised result with its log-sum.  One group of DT threads per row.
+// joins the parts of split keys: each is a normalised result with its log-sum.  dim / 4 threads a row.
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(const AttnArgs a) {
     const int per = a.dim / 4, rpb = 256 / per, i = threadIdx.x / per, d = (threadIdx.x - i * per) * 4;
-    const long long rows = (long long)a.tokens_q * a.heads, used = (long long)min(max(a.cu_q[a.seqs], 0), a.tokens_q) * a.heads;
-    const long long r = (long long)blockIdx.x * rpb + i;
-    if (i >= rpb || r >= used) return;       // rows behind the last sequence were cleared by the first launch
+    const long long rows = (long long)a.tokens_q * a.heads, r = (long long)blockIdx.x * rpb + i;
+    if (i >= rpb || r >= rows) return;
     const float* pl = a.part + rows * a.splits * a.dim;
     float most = -INFINITY;
     for (int z = 0; z < a.splits; ++z) most = fmaxf(most, pl[rows * z + r]);
@@ -361,6 +407,7 @@ __global__ __launch_bounds__(256) void join_kernel(const AttnArgs a) {
     float sum = 0.f;
     for (int z = 0; z < a.splits; ++z) {
         const float w = __builtin_amdgcn_exp2f((pl[rows * z + r] - base) * LOG2E);
+        if (w == 0.f) continue;                 // a part in which this row sees nothing
         sum += w;
         acc += w * *reinterpret_cast<const f32x4*>(a.part + (rows * z + r) * a.dim + d);
     }
@@ -393,289 +440,255 @@ __global__ __launch_bounds__(256) void delta_kernel(const AttnArgs a) {
 }
 
 // dQ: the forward's shape (rows in registers, keys staged), with dO beside Q and dS in P's place
-template <typename T, int DP, int NW, int NT>
-__global__ __launch_bounds__(NW * 64) void dq_kernel(const AttnArgs a) {
-    constexpr int NTHR = NW * 64, BM = NW * NT * 16, BN = 32, LD = DP + Tile<T>::PAD, CK = DP / 32, CD = DP / 16;
-    __shared__ __attribute__((aligned(16))) T sk[BN * LD];
-    __shared__ __attribute__((aligned(16))) T sv[BN * LD];
-    __shared__ int sh[16];
-    const int kvh = blockIdx.x % a.kv_heads, bid = blockIdx.x / a.kv_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane >> 4;
-    const Where w = locate<NTHR>(a.cu_q, a.seqs, a.tokens_q, a.group, BM, bid, sh);
-    if (w.seq < 0) {
-        if (kvh == 0) {
-            int b0, n0;
-            range_of(a.cu_q, a.seqs - 1, a.tokens_q, b0, n0);
-            clear_behind<T, NTHR>((T*)a.dq, nullptr, b0 + n0, a.tokens_q, a.heads, a.dim, bid - w.used, gridDim.x / a.kv_heads - w.used);
-        }
-        return;
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64, DP == 128 && (NW < 4 || sizeof(T) == 4) ? 1 : 2) void dq_kernel(const AttnArgs a) {
+    constexpr int NTHR = NW * 64, BM = NW * 32, BN = step_keys<T>(), NS = BN / 32, KK = DP / 16, ND = DP / 32;
+    __shared__ __attribute__((aligned(1024))) T sk[2][BN * DP];
+    __shared__ __attribute__((aligned(1024))) T sv[2][BN * DP];
+    const int kvh = blockIdx.x % a.kv_heads, tiles = gridDim.x / a.kv_heads, lane = threadIdx.x & 63, lh = lane >> 5;
+    const int tile = a.causal ? tiles - 1 - (int)(blockIdx.x / a.kv_heads) : blockIdx.x / a.kv_heads;
+    const int row0 = tile * BM, row = row0 + (threadIdx.x >> 6) * 32 + (lane & 31), total = a.tokens_q * a.group;
+    const int tok = min(row, total - 1) / a.group, head = kvh * a.group + min(row, total - 1) - tok * a.group;
+    const long long at = (long long)tok * a.heads + head;
+    Sight me;
+    const Span keys = tile_keys<BM>(a, row0, row, me);
+    const T* qp = (const T*)a.q + (long long)tok * a.q_tok + (long long)head * a.q_head;
+    const T* gp = (const T*)a.dout + (long long)tok * a.g_tok + (long long)head * a.g_head;
+    const T* kb = (const T*)a.k + (long long)kvh * a.k_head;
+    const T* vb = (const T*)a.v + (long long)kvh * a.v_head;
+    Direct<T, BN, DP, NTHR> dir;
+    dir.init(a.dim);
+    auto load = [&](int n0, int buf) __attribute__((always_inline)) {
+        dir.load(kb, a.k_tok, n0, keys.hi, sk[buf]);
+        dir.load(vb, a.v_tok, n0, keys.hi, sv[buf]);
+    };
+    if (keys.lo < keys.hi) load(keys.lo, 0);
+    const float lse2 = a.lse[at] * LOG2E, delta = a.delta[at], c2 = a.scale * LOG2E;
+    typename Vec<T>::x8 qf[KK], gf[KK];
+#pragma unroll
+    for (int c = 0; c < KK; ++c) {
+        qf[c] = global_frag<T>(qp, c, a.dim, row < total);
+        gf[c] = global_frag<T>(gp, c, a.dim, row < total);
     }
-    int q0, nq, k0, nk;
-    range_of(a.cu_q, w.seq, a.tokens_q, q0, nq);
-    range_of(a.cu_k, w.seq, a.tokens_k, k0, nk);
-    const int nrow = nq * a.group, tiles = (nrow + BM - 1) / BM;
-    const int tile = a.causal ? tiles - 1 - w.tile : w.tile;
-    const int row0 = tile * BM + wave * NT * 16, off = nk - nq;
-    const T* qb = (const T*)a.q + (long long)q0 * a.q_tok + (long long)kvh * a.group * a.q_head;
-    const T* gb = (const T*)a.dout + (long long)q0 * a.g_tok + (long long)kvh * a.group * a.g_head;
-    const T* kb = (const T*)a.k + (long long)k0 * a.k_tok + (long long)kvh * a.k_head;
-    const T* vb = (const T*)a.v + (long long)k0 * a.v_tok + (long long)kvh * a.v_head;
-    int tok[NT], hd[NT], see[NT];
-    float lse2[NT], delta[NT];
-    typename Vec<T>::x8 qf[NT][CK], gf[NT][CK];
+    f32x16 dq[ND];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int r = row0 + t * 16 + (lane & 15), rr = min(r, nrow - 1);
-        tok[t] = rr / a.group;
-        hd[t] = rr - tok[t] * a.group;
-        see[t] = r < nrow ? (a.causal ? min(nk, max(tok[t] + off + 1, 0)) : nk) : 0;
-        const long long at = (long long)(q0 + tok[t]) * a.heads + kvh * a.group + hd[t];
-        lse2[t] = a.lse[at] * LOG2E;
-        delta[t] = a.delta[at];
-        const T* p = qb + (long long)tok[t] * a.q_tok + (long long)hd[t] * a.q_head;
-        const T* g = gb + (long long)tok[t] * a.g_tok + (long long)hd[t] * a.g_head;
+    for (int d = 0; d < ND; ++d) dq[d] = zeros16();
+    int buf = 0;
+    for (int n0 = keys.lo; n0 < keys.hi; n0 += BN, buf ^= 1) {
+        landed();
+        if (n0 + BN < keys.hi) load(n0 + BN, buf ^ 1);
 #pragma unroll
-        for (int c = 0; c < CK; ++c) {
-            qf[t][c] = global_frag<T>(p, c, a.dim, r < nrow);
-            gf[t][c] = global_frag<T>(g, c, a.dim, r < nrow);
-        }
-    }
-    const int last = min((tile * BM + BM - 1) / a.group, nq - 1);
-    const int keys = a.causal ? min(nk, max(last + off + 1, 0)) : nk;
-    const int wlast = min((row0 + NT * 16 - 1) / a.group, nq - 1);
-    const int wkeys = row0 < nrow ? (a.causal ? min(nk, max(wlast + off + 1, 0)) : nk) : 0;
-    const int wfull = row0 + NT * 16 <= nrow ? (a.causal ? min(nk, max(row0 / a.group + off + 1, 0)) : nk) : 0;
-    f32x4 dq[CD][NT];
+        for (int kt = 0; kt < NS; ++kt) {
+            const int n1 = n0 + kt * 32;
+            if (n1 >= me.some.hi || n1 + 32 <= me.some.lo) continue;
+            f32x16 s = zeros16(), dp = zeros16();
 #pragma unroll
-    for (int d = 0; d < CD; ++d)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) dq[d][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const float c2 = a.scale * LOG2E;
-    Stage<T, BN, DP, NTHR> stk, stv;
-    if (keys > 0) {
-        stk.load(kb, a.k_tok, nk, a.dim);
-        stv.load(vb, a.v_tok, nk, a.dim);
-    }
-    for (int n0 = 0; n0 < keys; n0 += BN) {
-        stk.store(sk);
-        stv.store(sv);
-        __syncthreads();
-        if (n0 + BN < keys) {
-            stk.load(kb + (long long)(n0 + BN) * a.k_tok, a.k_tok, nk - n0 - BN, a.dim);
-            stv.load(vb + (long long)(n0 + BN) * a.v_tok, a.v_tok, nk - n0 - BN, a.dim);
-        }
-        if (n0 < wkeys) {
-            f32x4 s[2][NT], dp[2][NT];
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-                for (int t = 0; t < NT; ++t) s[kt][t] = dp[kt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < CK; ++c) {
-                    const auto kf = row_frag<T, LD>(sk, kt * 16, c);
-                    const auto vf = row_frag<T, LD>(sv, kt * 16, c);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        s[kt][t] = mma16(kf, qf[t][c], s[kt][t]);
-                        dp[kt][t] = mma16(vf, gf[t][c], dp[kt][t]);
-                    }
-                }
-            }
-            const bool mask = n0 + BN > wfull;
-            typename Vec<T>::x8 df[NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float p = __builtin_amdgcn_exp2f(fmaf(s[kt][t][i], c2, -lse2[t]));
-                        float ds = p * (dp[kt][t][i] - delta[t]);
-                        if (mask && n0 + kt * 16 + grp * 4 + i >= see[t]) ds = 0.f;
-                        s[kt][t][i] = ds;
-                    }
-                df[t] = acc_frag<T>(s[0][t], s[1][t]);      // one rounding of dS to T, as of P
+            for (int c = 0; c < KK; ++c) {
+                s = mma32(row_frag<T, DP>(sk[buf], kt * 32, c), qf[c], s);
+                dp = mma32(row_frag<T, DP>(sv[buf], kt * 32, c), gf[c], dp);
             }
 #pragma unroll
-            for (int d = 0; d < CD; ++d) {
-                const auto kf = col_frag<T, LD>(sk, 0, d * 16);
+            for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -lse2)) * (dp[e] - delta);
+            if (n1 < me.all.lo || n1 + 32 > me.all.hi) {
+                const int lo = me.mine.lo - n1 - 4 * lh, hi = me.mine.hi - n1 - 4 * lh;
 #pragma unroll
-                for (int t = 0; t < NT; ++t) dq[d][t] = mma16(kf, df[t], dq[d][t]);
+                for (int e = 0; e < 16; ++e)
+                    if (acc_row(e) < lo || acc_row(e) >= hi) s[e] = 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const auto df = acc_frag<T>(s, j);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) dq[d] = mma32(col_frag<T, DP>(sk[buf], kt * 32 + j * 16, d * 32), df, dq[d]);
             }
         }
-        __syncthreads();
     }
+    if (row >= total) return;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int r = row0 + t * 16 + (lane & 15);
-        if (r >= nrow) continue;
-        T* p = (T*)a.dq + ((long long)(q0 + tok[t]) * a.heads + kvh * a.group + hd[t]) * a.dim;
-#pragma unroll
-        for (int d = 0; d < CD; ++d)
-            if (d * 16 + grp * 4 < a.dim) store4<T>(p + d * 16 + grp * 4, dq[d][t] * a.scale);
-    }
+    for (int d = 0; d < ND; ++d) store16<T>((T*)a.dq + at * a.dim, d * 32, a.dim, dq[d], a.scale);
 }
 
-// dK, dV: keys in registers, rows (Q and dO) staged 32 at a time.  Here S = Q K^T, so a key is a column of every accumulator,
-// and P and dS are again the B operands as they come (dV^T = dO^T P, dK^T = Q^T dS).
-template <typename T, int DP, int NW, int NT>
-__global__ __launch_bounds__(NW * 64) void dkv_kernel(const AttnArgs a) {
-    constexpr int NTHR = NW * 64, BK = NW * NT * 16, BR = 32, LD = DP + Tile<T>::PAD, CK = DP / 32, CD = DP / 16;
-    __shared__ __attribute__((aligned(16))) T sq[BR * LD];
-    __shared__ __attribute__((aligned(16))) T sg[BR * LD];
-    __shared__ __attribute__((aligned(16))) float slse[BR];
-    __shared__ __attribute__((aligned(16))) float sdel[BR];
-    __shared__ int ssee[BR];
-    __shared__ int sh[16];
-    const int kvh = blockIdx.x % a.kv_heads, bid = blockIdx.x / a.kv_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane >> 4;
-    const Where w = locate<NTHR>(a.cu_k, a.seqs, a.tokens_k, 1, BK, bid, sh);
-    if (w.seq < 0) {
-        if (kvh == 0) {
-            int b0, n0;
-            range_of(a.cu_k, a.seqs - 1, a.tokens_k, b0, n0);
-            clear_behind<T, NTHR>((T*)a.dk, nullptr, b0 + n0, a.tokens_k, a.kv_heads, a.dim, bid - w.used, gridDim.x / a.kv_heads - w.used);
-            clear_behind<T, NTHR>((T*)a.dv, nullptr, b0 + n0, a.tokens_k, a.kv_heads, a.dim, bid - w.used, gridDim.x / a.kv_heads - w.used);
-        }
-        return;
-    }
-    int q0, nq, k0, nk;
-    range_of(a.cu_q, w.seq, a.tokens_q, q0, nq);
-    range_of(a.cu_k, w.seq, a.tokens_k, k0, nk);
-    const int nrow = nq * a.group, off = nk - nq;
-    const int key0 = w.tile * BK + wave * NT * 16;
-    const T* qb = (const T*)a.q + (long long)q0 * a.q_tok + (long long)kvh * a.group * a.q_head;
-    const T* gb = (const T*)a.dout + (long long)q0 * a.g_tok + (long long)kvh * a.group * a.g_head;
-    const T* kb = (const T*)a.k + (long long)k0 * a.k_tok + (long long)kvh * a.k_head;
-    const T* vb = (const T*)a.v + (long long)k0 * a.v_tok + (long long)kvh * a.v_head;
-    typename Vec<T>::x8 kf[NT][CK], vf[NT][CK];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int key = key0 + t * 16 + (lane & 15);
-        const long long kk = min(key, nk - 1);
-#pragma unroll
-        for (int c = 0; c < CK; ++c) {
-            kf[t][c] = global_frag<T>(kb + kk * a.k_tok, c, a.dim, key < nk);
-            vf[t][c] = global_frag<T>(vb + kk * a.v_tok, c, a.dim, key < nk);
-        }
-    }
-    f32x4 dk[CD][NT], dv[CD][NT];
-#pragma unroll
-    for (int d = 0; d < CD; ++d)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) dk[d][t] = dv[d][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const float c2 = a.scale * LOG2E;
-    // the first row that sees the workgroup's first key
-    const int first = a.causal ? min(max(w.tile * BK - off, 0), nq) * a.group / BR * BR : 0;
-    Stage<T, BR, DP, NTHR> stq, stg;
-    float rl = 0.f, rd = 0.f;
-    int rs = 0;
-    auto fetch = [&](int r0) __attribute__((always_inline)) {
-        stq.load_rows(qb, a.q_tok, a.q_head, a.group, r0, nrow, a.dim);
-        stg.load_rows(gb, a.g_tok, a.g_head, a.group, r0, nrow, a.dim);
+// dK, dV: keys in registers, rows (Q and dO) staged.  Here S = Q K^T, so a key is a column of every accumulator, and P and dS are again
+// the B operands as they come (dV^T = dO^T P, dK^T = Q^T dS).
+// KW waves of 32 keys each, RG times: the row groups take every RG-th 32 rows and are added up in LDS at the end.  The first keys of
+// a long causal sequence meet all its rows, and that chain of steps - not the sum of the work - is what a launch of few sequences
+// lasts (167 -> 109 us with two groups, 8 bf16 sequences of up to 2048 tokens, dim 64).
+template <typename T, int DP, int KW, int RG>
+__global__ __launch_bounds__(KW * RG * 64, DP == 128 ? 1 : 2) void dkv_kernel(const AttnArgs a) {
+    constexpr int NTHR = KW * RG * 64, BK = KW * 32, BR = 32 * RG, KK = DP / 16, ND = DP / 32;
+    __shared__ __attribute__((aligned(1024))) T tiles[4][BR * DP];
+    static_assert(RG == 1 || sizeof(tiles) >= KW * 64 * ND * 16 * 4, "one of dK, dV of a row group fits the tiles");
+    T (*const sq)[BR * DP] = tiles;
+    T (*const sg)[BR * DP] = tiles + 2;
+    __shared__ __attribute__((aligned(16))) float srow[2][2][BR];       // lse, delta
+    const int kvh = blockIdx.x % a.kv_heads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lh = lane >> 5;
+    const int rg = wave / KW, kw = wave - rg * KW, mine = rg * 32;      // this wave's rows of a step begin at `mine`
+    const int key0 = (int)(blockIdx.x / a.kv_heads) * BK, key = key0 + kw * 32 + (lane & 31);
+    Sight me;
+    const Span rows = tile_rows<BK>(a, key0, key, me);
+    const T* qb = (const T*)a.q + (long long)kvh * a.group * a.q_head;
+    const T* gb = (const T*)a.dout + (long long)kvh * a.group * a.g_head;
+    Direct<T, BR, DP, NTHR> dir;
+    dir.init(a.dim);
+    auto fetch = [&](int r0, int buf) __attribute__((always_inline)) {
+        dir.load_rows(qb, (int)a.q_tok, (int)a.q_head, a.group, r0, rows.hi, sq[buf]);
+        dir.load_rows(gb, (int)a.g_tok, (int)a.g_head, a.group, r0, rows.hi, sg[buf]);
         if (threadIdx.x < BR) {
-            const int r = r0 + threadIdx.x, rr = min(r, nrow - 1), t = rr / a.group;
-            const long long at = (long long)(q0 + t) * a.heads + kvh * a.group + (rr - t * a.group);
-            rl = a.lse[at] * LOG2E;
-            rd = a.delta[at];
-            rs = r < nrow ? (a.causal ? min(nk, max(t + off + 1, 0)) : nk) : 0;
+            const int r = min(r0 + (int)threadIdx.x, rows.hi - 1), t = r / a.group;
+            const long long at = (long long)t * a.heads + kvh * a.group + (r - t * a.group);
+            srow[buf][0][threadIdx.x] = a.lse[at] * LOG2E;
+            srow[buf][1][threadIdx.x] = a.delta[at];
         }
     };
-    if (first < nrow) fetch(first);
-    for (int r0 = first; r0 < nrow; r0 += BR) {
-        stq.store(sq);
-        stg.store(sg);
-        if (threadIdx.x < BR) { slse[threadIdx.x] = rl; sdel[threadIdx.x] = rd; ssee[threadIdx.x] = rs; }
-        __syncthreads();
-        if (r0 + BR < nrow) fetch(r0 + BR);
-        if (key0 < ssee[BR - 1] || r0 + BR > nrow) {        // the last row of the step sees most
-            f32x4 s[2][NT], dp[2][NT];
+    if (rows.lo < rows.hi) fetch(rows.lo, 0);
+    typename Vec<T>::x8 kf[KK], vf[KK];
+    {
+        const long long kk = min(key, a.tokens_k - 1);
+        const T* kp = (const T*)a.k + kk * a.k_tok + (long long)kvh * a.k_head;
+        const T* vp = (const T*)a.v + kk * a.v_tok + (long long)kvh * a.v_head;
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt) {
+        for (int c = 0; c < KK; ++c) {
+            kf[c] = global_frag<T>(kp, c, a.dim, key < a.tokens_k);
+            vf[c] = global_frag<T>(vp, c, a.dim, key < a.tokens_k);
+        }
+    }
+    f32x16 dk[ND], dv[ND];
 #pragma unroll
-                for (int t = 0; t < NT; ++t) s[rt][t] = dp[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zeros16();
+    const float c2 = a.scale * LOG2E;
+    int buf = 0;
+    for (int r0 = rows.lo; r0 < rows.hi; r0 += BR, buf ^= 1) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        landed();
+        if (r0 + BR < rows.hi) fetch(r0 + BR, buf ^ 1);
+        const int r1 = r0 + mine;
+        if (r1 >= me.some.hi || r1 + 32 <= me.some.lo) continue;
+        f32x16 s = zeros16(), dp = zeros16();
 #pragma unroll
-                for (int c = 0; c < CK; ++c) {
-                    const auto qf = row_frag<T, LD>(sq, rt * 16, c);
-                    const auto gf = row_frag<T, LD>(sg, rt * 16, c);
+        for (int c = 0; c < KK; ++c) {
+            s = mma32(row_frag<T, DP>(sq[buf], mine, c), kf[c], s);
+            dp = mma32(row_frag<T, DP>(sg[buf], mine, c), vf[c], dp);
+        }
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        s[rt][t] = mma16(qf, kf[t][c], s[rt][t]);
-                        dp[rt][t] = mma16(gf, vf[t][c], dp[rt][t]);
-                    }
-                }
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 l4 = *reinterpret_cast<const f32x4*>(&srow[buf][0][mine + 8 * g + 4 * lh]), d4 = *reinterpret_cast<const f32x4*>(&srow[buf][1][mine + 8 * g + 4 * lh]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = rt * 16 + grp * 4 + i;
-                    const float lse2 = slse[r], del = sdel[r];
-                    const int see = ssee[r];
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        float p = __builtin_amdgcn_exp2f(fmaf(s[rt][t][i], c2, -lse2));
-                        float ds = p * (dp[rt][t][i] - del);
-                        if (key0 + t * 16 + (lane & 15) >= see) p = ds = 0.f;
-                        s[rt][t][i] = p;
-                        dp[rt][t][i] = ds;
-                    }
-                }
-            }
-            typename Vec<T>::x8 pf[NT], df[NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) { pf[t] = acc_frag<T>(s[0][t], s[1][t]); df[t] = acc_frag<T>(dp[0][t], dp[1][t]); }
-#pragma unroll
-            for (int d = 0; d < CD; ++d) {
-                const auto gt = col_frag<T, LD>(sg, 0, d * 16);
-                const auto qt = col_frag<T, LD>(sq, 0, d * 16);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    dv[d][t] = mma16(gt, pf[t], dv[d][t]);
-                    dk[d][t] = mma16(qt, df[t], dk[d][t]);
-                }
+            for (int i = 0; i < 4; ++i) {
+                const int e = 4 * g + i;
+                s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -l4[i]));
+                dp[e] = s[e] * (dp[e] - d4[i]);
             }
         }
-        __syncthreads();
-    }
+        if (r1 < me.all.lo || r1 + 32 > me.all.hi) {
+            const int lo = me.mine.lo - r1 - 4 * lh, hi = me.mine.hi - r1 - 4 * lh;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int key = key0 + t * 16 + (lane & 15);
-        if (key >= nk) continue;
-        const long long at = ((long long)(k0 + key) * a.kv_heads + kvh) * a.dim;
+            for (int e = 0; e < 16; ++e)
+                if (acc_row(e) < lo || acc_row(e) >= hi) s[e] = dp[e] = 0.f;
+        }
 #pragma unroll
-        for (int d = 0; d < CD; ++d)
-            if (d * 16 + grp * 4 < a.dim) {
-                store4<T>((T*)a.dk + at + d * 16 + grp * 4, dk[d][t] * a.scale);
-                store4<T>((T*)a.dv + at + d * 16 + grp * 4, dv[d][t]);
+        for (int j = 0; j < 2; ++j) {
+            const auto pf = acc_frag<T>(s, j), df = acc_frag<T>(dp, j);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                dv[d] = mma32(col_frag<T, DP>(sg[buf], mine + j * 16, d * 32), pf, dv[d]);
+                dk[d] = mma32(col_frag<T, DP>(sq[buf], mine + j * 16, d * 32), df, dk[d]);
             }
+        }
+    }
+    if constexpr (RG > 1) {
+        float* sum = reinterpret_cast<float*>(tiles) + kw * (64 * ND * 16) + lane;
+        auto add = [&](f32x16 (&x)[ND]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int g = 1; g < RG; ++g) {
+                __syncthreads();
+                if (rg == g) {
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) sum[(d * 16 + e) * 64] = x[d][e];
+                }
+                __syncthreads();
+                if (rg == 0) {
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) x[d][e] += sum[(d * 16 + e) * 64];
+                }
+            }
+        };
+        add(dk);
+        add(dv);
+        if (rg > 0) return;
+    }
+    if (key >= a.tokens_k) return;
+    const long long at = ((long long)key * a.kv_heads + kvh) * a.dim;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+        store16<T>((T*)a.dk + at, d * 32, a.dim, dk[d], a.scale);
+        store16<T>((T*)a.dv + at, d * 32, a.dim, dv[d], 1.0f);
     }
 }
 
 // ------------------------------------------------------------------------------------------------ host
-// workgroups: no more tiles than rows / BM full ones and one partial one a sequence, and one for the rows behind them, each for
-// every key head (the fastest index: neighbours in time work on the same few heads of an XCD, whose L2 then holds their keys)
-inline unsigned blocks_for(const AttnArgs& a, long long rows, int bm) { return (unsigned)((rows / bm + a.seqs + 1) * a.kv_heads); }
+// one workgroup for every tile of `per` rows and every key head (the fastest index: neighbours in time work on the few heads of an XCD,
+// whose L2 then holds their keys)
+inline unsigned blocks_for(const AttnArgs& a, long long rows, int per) { return (unsigned)((rows + per - 1) / per * a.kv_heads); }
 
-template <typename T, int DP, int NW, int NT>
+template <typename T, int DP, int NW>
 int launch_fwd(const AttnArgs& a, hipStream_t st) {
-    const dim3 grid(blocks_for(a, (long long)a.tokens_q * a.group, NW * NT * 16), a.splits);
-    hipLaunchKernelGGL((fwd_kernel<T, DP, NW, NT>), grid, dim3(NW * 64), 0, st, a);
+    hipLaunchKernelGGL((fwd_kernel<T, DP, NW>), dim3(blocks_for(a, (long long)a.tokens_q * a.group, NW * 32), a.splits), dim3(NW * 64), 0, st, a);
     if (a.splits > 1) {
         const int rpb = 256 / (a.dim / 4);
-        const long long rows = (long long)a.tokens_q * a.heads;
-        hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)((rows + rpb - 1) / rpb)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(((long long)a.tokens_q * a.heads + rpb - 1) / rpb)), dim3(256), 0, st, a);
     }
     return launch_status("attention_packed_fwd");
 }
+template <typename T, int DP, int NW>
+void launch_dq(const AttnArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((dq_kernel<T, DP, NW>), dim3(blocks_for(a, (long long)a.tokens_q * a.group, NW * 32)), dim3(NW * 64), 0, st, a);
+}
+template <typename T, int DP, int KW, int RG>
+void launch_dkv(const AttnArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((dkv_kernel<T, DP, KW, RG>), dim3(blocks_for(a, a.tokens_k, KW * 32)), dim3(KW * RG * 64), 0, st, a);
+}
 
-template <typename T, int DP, int NW, int NT>
-int launch_dq(const AttnArgs& a, hipStream_t st) {
-    const dim3 grid(blocks_for(a, (long long)a.tokens_q * a.group, NW * NT * 16));
-    hipLaunchKernelGGL((dq_kernel<T, DP, NW, NT>), grid, dim3(NW * 64), 0, st, a);
+// Waves a workgroup: four where the average sequence fills them (they share each staged tile), two otherwise; split keys go
+// with one wave (attention_splits in capi.hip: few rows, long caches)
+template <typename T, int DP>
+int fwd_dim(const AttnArgs& a, hipStream_t st) {
+    if (a.splits > 1) return launch_fwd<T, DP, 1>(a, st);
+    if ((long long)a.tokens_q * a.group / a.seqs <= 96) return launch_fwd<T, DP, 2>(a, st);
+    return launch_fwd<T, DP, 4>(a, st);
+}
+
+template <typename T, int DP>
+int bwd_dim(const AttnArgs& a, hipStream_t st) {
+    const long long rows = (long long)a.tokens_q * a.group / a.seqs;
+    if (a.tokens_q > 0) {
+        if (rows <= 96) launch_dq<T, DP, 2>(a, st);
+        else launch_dq<T, DP, 4>(a, st);
+    }
+    if (a.tokens_k > 0) {
+        if (rows <= 96) launch_dkv<T, DP, 2, 1>(a, st);
+        else launch_dkv<T, DP, 2, 2>(a, st);
+    }
     return launch_status("attention_packed_bwd");
 }
 
-template <typename T, int DP, int NW, int NT>
-int launch_dkv(const AttnArgs& a, hipStream_t st) {
-    const dim3 grid(blocks_for(a, a.tokens_k, NW * NT * 16));
-    hipLaunchKernelGGL((dkv_kernel<T, DP, NW, NT>), grid, dim3(NW * 64), 0, st, a);
-    return launch_status("attention_packed_bwd");
+template <typename T>
+int fwd(const AttnArgs& a, hipStream_t st) {
+    if (a.dim <= 32) return fwd_dim<T, 32>(a, st);
+    if (a.dim <= 64) return fwd_dim<T, 64>(a, st);
+    return fwd_dim<T, 128>(a, st);
+}
+
+template <typename T>
+int bwd(const AttnArgs& a, hipStream_t st) {
+    const long long rows = (long long)a.tokens_q * a.heads;
+    if (rows > 0) hipLaunchKernelGGL((delta_kernel<T>), dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, st, a);
+    if (a.dim <= 32) return bwd_dim<T, 32>(a, st);
+    if (a.dim <= 64) return bwd_dim<T, 64>(a, st);
+    return bwd_dim<T, 128>(a, st);
 }
 
 }  // namespace attn

@@ -1,6 +1,5 @@
-// Attention over packed sequences for bf16 tensors (the kernels: attn_packed.hpp, attn_packed_wide.hpp).
-#include "attn_packed_wide.hpp"
-#include "attn_packed_dispatch.hpp"
+// Attention over packed sequences for bf16 tensors (the kernels: attn_packed.hpp).
+#include "attn_packed.hpp"
 
 namespace icap {
 

@@ -1,6 +1,5 @@
 // Attention over packed sequences for fp32 tensors (the kernels: attn_packed.hpp).
-#include "attn_packed_wide.hpp"
-#include "attn_packed_dispatch.hpp"
+#include "attn_packed.hpp"
 
 namespace icap {
 

@@ -241,14 +241,13 @@ static int attention_check(const char* what, int dtype, const AttnArgs& a) {
     return ICAP_OK;
 }
 
-// Keys are split when the rows alone give fewer workgroups than the card holds (256 CUs, four one-wave workgroups each):
-// only where one wave covers a sequence's rows (single tokens), so that the partial results stay small.
+// Few rows over long caches (single tokens): tiles of 32 rows alone give fewer workgroups than the card holds (256 CUs, two a CU), so
+// the keys are split over more of them.  Not for prompts, whose rows fill the card, nor where a part would be shorter than two steps.
 static int attention_splits(int seqs, int tokens_q, int tokens_k, int heads, int kv_heads) {
-    const long long rows = (long long)tokens_q * (heads / kv_heads) / seqs;
-    if (rows > 16) return 1;
-    const long long wgs = (long long)seqs * kv_heads, longest = tokens_k;       // the longest sequence may hold them all
-    long long s = (1024 + wgs - 1) / wgs;
-    if (s > longest / 128) s = longest / 128;
+    const long long rows = (long long)tokens_q * (heads / kv_heads), wgs = (rows + 31) / 32 * kv_heads;
+    if (wgs > 256 || tokens_k < 8ll * tokens_q) return 1;
+    long long s = 1024 / wgs;
+    if (s > tokens_k / 128) s = tokens_k / 128;          // one sequence may hold all the keys
     return (int)(s < 1 ? 1 : (s > 32 ? 32 : s));
 }
 

@@ -23,18 +23,6 @@ template <> struct Vec<float> { typedef f32x8 x8; typedef f32x4 x4; };
 template <> struct Vec<__bf16> { typedef bf16x8 x8; typedef bf16x4 x4; };
 template <> struct Vec<_Float16> { typedef f16x8 x8; typedef f16x4 x4; };
 
-// acc[16 x 16] += A[16 x 32] B[32 x 16]: every lane brings eight values of A's row (lane % 16) and eight of B's column
-// (lane % 16); which 32 places of the contraction the eight slots of lane / 16 stand for is the caller's choice, as long as A
-// and B agree.  acc: column lane % 16, rows 4 (lane / 16) .. + 3.  fp32 has no 32-deep instruction: slot j of all lanes is
-// one 4-deep product, so the same fragments serve.
-__device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x4 mma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x4 mma16(f32x8 a, f32x8 b, f32x4 c) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
-    return c;
-}
-
 struct AttnArgs {
     const void *q, *k, *v, *dout, *o;       // element strides below; o dense [tokens_q][heads][dim]
     void *out, *dq, *dk, *dv;               // dense
