@@ -52,15 +52,22 @@ __device__ __forceinline__ f32x16 zeros16() {
 __device__ __forceinline__ int cut(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
 // ------------------------------------------------------------------------------------------------ tiles in LDS
-// permutation of a row's 16-byte slots.  Rows of 256 bytes and more all begin at bank 0, rows of 128 and 64 bytes share a bank line two
-// and four at a time; in 16-bit tiles the lowest bit moves by the third row bit, so that the 32-byte pieces of four
-// consecutive rows, which a transposing read takes together, lie apart.
+// permutation of a row's 16-byte slots.  A 256-byte line of the 64 banks holds one row of 256 bytes (half of one of 512), two of 128 or
+// four of 64.  A fragment read takes one slot of 16 rows at a time, which have to lie in 16 places of the line; a transposing read
+// takes 64 bytes of four consecutive rows, so those differ in the upper bits.  (With 8 places instead of 16, half of the LDS
+// cycles were conflicts.)
 template <typename T, int DP>
 __device__ __forceinline__ int swizzle(int row) {
-    if constexpr (sizeof(T) == 4) return DP == 32 ? (row >> 1) & 3 : row & 7;
-    else if constexpr (DP == 128) return ((row & 3) << 1) | ((row >> 2) & 1);
-    else if constexpr (DP == 64) return (((row >> 1) & 1) << 1) | ((row >> 2) & 1);
-    else return (row >> 2) & 1;
+    if constexpr (sizeof(T) == 4) return DP == 32 ? (row >> 1) & 7 : ((row & 4) << 1) | ((row & 8) >> 1) | (row & 3);
+    else if constexpr (DP == 128) return ((row & 3) << 2) | ((row >> 2) & 3);
+    else if constexpr (DP == 64) return ((row & 2) << 1) | ((row >> 2) & 3);
+    else return (row >> 2) & 3;
+}
+
+// the values of a lane and of lane ^ 32, without the LDS: the swap hands every lane both halves'
+__device__ __forceinline__ f32x2 both_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f32x2{__uint_as_float(r[0]), __uint_as_float(r[1])};
 }
 
 // [ROWS][DP] values, global -> LDS
@@ -125,10 +132,12 @@ __device__ __forceinline__ typename Vec<T>::x8 col_frag(const T* lds, int row0, 
     const int lane = threadIdx.x & 63, lh = lane >> 5;
     if constexpr (sizeof(T) == 2) {
         const int l = lane & 15, half = (lane >> 4) & 1, r = 4 * lh + (l >> 2), slot = (col0 >> 3) + half * 2 + ((l & 3) >> 1);
-        const T* p = lds + (row0 + r) * DP + (slot ^ swizzle<T, DP>(r)) * 8 + (l & 1) * 4;
+        const int f = slot ^ swizzle<T, DP>(r);                 // eight rows further the permutation differs by 2
+        const T* p = lds + (row0 + r) * DP + f * 8 + (l & 1) * 4;
+        const T* q = lds + (row0 + r + 8) * DP + (f ^ 2) * 8 + (l & 1) * 4;
         typedef __attribute__((address_space(3))) i16x4* lds_ptr;
         const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p));
-        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 8 * DP));
+        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(q));
         typedef short i16x8 __attribute__((ext_vector_type(8)));
         const i16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         return __builtin_bit_cast(typename Vec<T>::x8, both);
@@ -336,7 +345,8 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && (NW < 4 || sizeof(T) == 4) ? 
         float mx = now[0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) mx = fmaxf(mx, now[e]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32)) * c2;
+        const f32x2 halves = both_halves(mx);
+        mx = fmaxf(halves[0], halves[1]) * c2;
         if (__any(mx > m + 8.0f)) {
             const float mn = fmaxf(m, mx);
             const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
@@ -393,23 +403,26 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && (NW < 4 || sizeof(T) == 4) ? 
     }
 }
 
-// joins the parts of split keys: each is a normalised result with its log-sum.  dim / 4 threads a row.
+// joins the parts of split keys: each is a normalised result with its log-sum (zeros and -inf where its keys are none of this row's).
+// dim / 4 threads a row, one wave a workgroup.
 template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(const AttnArgs a) {
-    const int per = a.dim / 4, rpb = 256 / per, i = threadIdx.x / per, d = (threadIdx.x - i * per) * 4;
+__global__ __launch_bounds__(64) void join_kernel(const AttnArgs a) {
+    const int per = a.dim / 4, rpb = 64 / per, i = threadIdx.x / per, d = (threadIdx.x - i * per) * 4;
     const long long rows = (long long)a.tokens_q * a.heads, r = (long long)blockIdx.x * rpb + i;
     if (i >= rpb || r >= rows) return;
-    const float* pl = a.part + rows * a.splits * a.dim;
+    const float* pl = a.part + rows * a.splits * a.dim + r;
+    const float* po = a.part + r * a.dim + d;
     float most = -INFINITY;
-    for (int z = 0; z < a.splits; ++z) most = fmaxf(most, pl[rows * z + r]);
+#pragma unroll 8
+    for (int z = 0; z < a.splits; ++z) most = fmaxf(most, pl[rows * z]);
     const float base = most == -INFINITY ? 0.f : most;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     float sum = 0.f;
+#pragma unroll 8
     for (int z = 0; z < a.splits; ++z) {
-        const float w = __builtin_amdgcn_exp2f((pl[rows * z + r] - base) * LOG2E);
-        if (w == 0.f) continue;                 // a part in which this row sees nothing
+        const float w = __builtin_amdgcn_exp2f((pl[rows * z] - base) * LOG2E);
         sum += w;
-        acc += w * *reinterpret_cast<const f32x4*>(a.part + (rows * z + r) * a.dim + d);
+        acc += w * *reinterpret_cast<const f32x4*>(po + rows * a.dim * z);
     }
     const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
     store4<T>((T*)a.out + r * a.dim + d, acc * inv);
@@ -638,8 +651,8 @@ template <typename T, int DP, int NW>
 int launch_fwd(const AttnArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((fwd_kernel<T, DP, NW>), dim3(blocks_for(a, (long long)a.tokens_q * a.group, NW * 32), a.splits), dim3(NW * 64), 0, st, a);
     if (a.splits > 1) {
-        const int rpb = 256 / (a.dim / 4);
-        hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(((long long)a.tokens_q * a.heads + rpb - 1) / rpb)), dim3(256), 0, st, a);
+        const int rpb = 64 / (a.dim / 4);
+        hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(((long long)a.tokens_q * a.heads + rpb - 1) / rpb)), dim3(64), 0, st, a);
     }
     return launch_status("attention_packed_fwd");
 }
