@@ -76,17 +76,17 @@ __device__ __forceinline__ void split(float x, E& hi, E& lo) {
     lo = (E)(x - (float)hi);
 }
 
-template <int BM, int BN> constexpr int smem_bytes() { return 2 * (BM + BN) * ROWB; }
+template <int BM, int BN, int ST> constexpr int smem_bytes() { return ST * (BM + BN) * ROWB; }
 
 // WM x WN waves, each (BM / WM) x 64 of the tile.  Operands go global -> LDS without passing a register (16 bytes a lane, one wave
-// 1 KB); the next K tile is in flight while the current one multiplies; one wait and one barrier a K tile.  The 16-byte slot a lane
+// 1 KB); ST - 1 K tiles are in flight while one multiplies; one wait and one barrier a K tile.  The 16-byte slot a lane
 // fetches is permuted by its row, and the fragment reads apply the same permutation, so that 16 rows meet 16 different slots.
-template <typename E, typename T, int BM, int BN, int WM, int WN, int EP>
+template <typename E, typename T, int BM, int BN, int WM, int WN, int ST, int EP>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
     constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, RM = TM / 32, RN = TN / 32, RPP = NW * 8;
     static_assert(TN == STRIP && TM % 32 == 0 && BM % RPP == 0 && BN % RPP == 0, "wave tiles");
     constexpr int APT = BM / RPP, BPT = BN / RPP, A_BYTES = BM * ROWB, STAGE = (BM + BN) * ROWB, EP_LD = TN + 4;
-    static_assert(NW * 32 * EP_LD * 4 <= 2 * STAGE, "the waves' result images fit the staging buffers");
+    static_assert(NW * 32 * EP_LD * 4 <= ST * STAGE, "the waves' result images fit the staging buffers");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave - wm * WN, lr = lane & 31, lh = lane >> 5;
 
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
     for (int i = 0; i < BPT; ++i) b_off[i] = (long long)min(n0 + i * RPP + srow, p.N - 1) * p.ldb + 8 * lslot;
     const int nk = p.K / BK, total = nk * p.pairs;
     const int per = (total + p.ksplit - 1) / p.ksplit, t_lo = min((int)blockIdx.y * per, total), t_hi = min(t_lo + per, total);
-    int pair = t_lo / nk, kt = t_lo - pair * nk;
+    int pair = t_lo / nk, kt = t_lo - pair * nk, left = t_hi - t_lo;
     auto issue = [&](int buf) __attribute__((always_inline)) {
         unsigned char* base = smem + buf * STAGE + wave * 1024;
         const unsigned short* a = (pair == 2 ? p.a1 : p.a0) + (long long)kt * BK;
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
         for (int i = 0; i < APT; ++i) load16(a + a_off[i], base + i * (NW * 1024));
 #pragma unroll
         for (int i = 0; i < BPT; ++i) load16(b + b_off[i], base + A_BYTES + i * (NW * 1024));
-        if (++kt == nk) { kt = 0; ++pair; }
+        if (--left > 0 && ++kt == nk) { kt = 0; ++pair; }       // behind the last tile it is fetched again, so that the waits can count
     };
     f32x16 acc[RM][RN];
 #pragma unroll
@@ -140,15 +140,20 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
                 for (int j = 0; j < RN; ++j) acc[i][j] = Mma<E>::go(af[i], bf[j], acc[i][j]);
         }
     };
-    if (t_lo < t_hi) issue(0);
-    for (int t = t_lo; t < t_hi; ++t) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();           // K tile t is there for every wave, and everybody has left the buffer filled next
-        asm volatile("" ::: "memory");
-        if (t + 1 < t_hi) issue((t + 1 - t_lo) & 1);
-        compute((t - t_lo) & 1);
+    if (t_lo < t_hi) {
+#pragma unroll
+        for (int i = 0; i < ST - 1; ++i) issue(i);
+        int buf = 0;
+        for (int t = t_lo; t < t_hi; ++t) {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 2) * (APT + BPT)) : "memory");
+            __builtin_amdgcn_s_barrier();       // K tile t is there for every wave, and everybody has left the buffer filled next
+            asm volatile("" ::: "memory");
+            issue(buf == 0 ? ST - 1 : buf - 1);
+            compute(buf);
+            buf = buf + 1 == ST ? 0 : buf + 1;
+        }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 
@@ -331,24 +336,38 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const
 }
 
 // ------------------------------------------------------------------------------------------------ operands
-// largest magnitude of a matrix: one value a workgroup
-__global__ __launch_bounds__(256) void amax_kernel(const float* x, long long ld, int R, int C, float* part) {
+constexpr int AMAX_WGS = 256;
+
+// largest magnitudes of hidden and weight, one value a workgroup: the first AMAX_WGS take one, the others the other
+__global__ __launch_bounds__(256) void amax_kernel(const float* h, long long ld_h, int R, const float* w, long long ld_w, int V, int C, float* part) {
+    const bool second = blockIdx.x >= AMAX_WGS;
+    const float* x = second ? w : h;
+    const long long ld = second ? ld_w : ld_h;
+    const int rows = second ? V : R, lane = threadIdx.x & 63, first = (blockIdx.x & (AMAX_WGS - 1)) * 4 + (threadIdx.x >> 6);
     float m = 0.f;
-    for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < R; r += gridDim.x * 4)
-        for (int c = threadIdx.x & 63; c < C; c += 64) m = fmaxf(m, fabsf(x[r * ld + c]));
+    if (ld % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && C % 4 == 0) {
+        for (int r = first; r < rows; r += AMAX_WGS * 4)
+#pragma unroll 4
+            for (int c = lane * 4; c < C; c += 256) {
+                const f32x4 v = *reinterpret_cast<const f32x4*>(x + r * ld + c);
+                m = fmaxf(fmaxf(m, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
+            }
+    } else {
+        for (int r = first; r < rows; r += AMAX_WGS * 4)
+            for (int c = lane; c < C; c += 64) m = fmaxf(m, fabsf(x[r * ld + c]));
+    }
     __shared__ float red[4];
     m = wave_max(m);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    if (lane == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
     if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
-constexpr int AMAX_WGS = 256;
 
 // scales[0..3] = 2^s_h, 2^-s_h, 2^s_w, 2^-s_w, scales[4] = 2^-(s_h + s_w): powers of two that bring the largest magnitude to [2^13, 2^14]
-__global__ __launch_bounds__(256) void scales_kernel(const float* part_h, const float* part_w, float* scales) {
+__global__ __launch_bounds__(256) void scales_kernel(const float* part, float* scales) {
     __shared__ float red[2][4];
     const int wave = threadIdx.x >> 6;
-    const float h = wave_max(part_h[threadIdx.x]), w = wave_max(part_w[threadIdx.x]);
+    const float h = wave_max(part[threadIdx.x]), w = wave_max(part[AMAX_WGS + threadIdx.x]);
     if ((threadIdx.x & 63) == 0) { red[0][wave] = h; red[1][wave] = w; }
     __syncthreads();
     if (threadIdx.x < 2) {
@@ -362,34 +381,67 @@ __global__ __launch_bounds__(256) void scales_kernel(const float* part_h, const 
     if (threadIdx.x == 0) scales[4] = scales[1] * scales[3];
 }
 
-// src [R][C] (rows ld apart) -> 16-bit planes of it: rows [R][Cp] and / or transposed [C][Rp], zeros up to Cp and Rp (multiples of 64)
+// One matrix [R][C] (rows ld apart) and the 16-bit planes wanted of it: rows [R][Cp] and / or transposed [C][Rp], zeros up to Cp and Rp
+// (multiples of 64)
+struct Turn {
+    const void* src; long long ld; int R, C, Rp, Cp, tiles_c; const float* scale;
+    void *r0, *r1, *c0, *c1;
+    int blocks;
+};
+
+// a workgroup takes 64 x 64 values of one of two matrices: 16-byte loads and stores both ways, turned in LDS
 template <typename T, typename E>
-__global__ __launch_bounds__(256) void planes_kernel(const T* src, long long ld, int R, int C, int Rp, int Cp, const float* scale, E* r0, E* r1,
-                                                     E* c0, E* c1) {
+__global__ __launch_bounds__(256) void planes_kernel(const Turn a, const Turn b) {
+    constexpr int V = 16 / sizeof(T);                   // values of a 16-byte load
     __shared__ E hi[64][66];
-    __shared__ E lo[64][66];
-    const int cx = blockIdx.x * 64, ry = blockIdx.y * 64, tid = threadIdx.x;
-    const float f = scale ? *scale : 1.0f;
-    for (int i = tid; i < 64 * 64; i += 256) {
-        const int r = i >> 6, c = i & 63;
-        float x = 0.f;
-        if (ry + r < R && cx + c < C) x = (float)src[(long long)(ry + r) * ld + cx + c] * f;
-        E h, l;
-        split<E>(x, h, l);
-        hi[r][c] = h;
-        if constexpr (sizeof(T) == 4) lo[r][c] = l;
-        if (r0 && ry + r < R) {
-            r0[(long long)(ry + r) * Cp + cx + c] = h;
-            if constexpr (sizeof(T) == 4) r1[(long long)(ry + r) * Cp + cx + c] = l;
+    __shared__ E lo[sizeof(T) == 4 ? 64 : 1][66];
+    const bool second = (int)blockIdx.x >= a.blocks;
+    const Turn& p = second ? b : a;
+    const int id = second ? blockIdx.x - a.blocks : blockIdx.x, ry = id / p.tiles_c * 64, cx = (id - id / p.tiles_c * p.tiles_c) * 64, tid = threadIdx.x;
+    const T* src = (const T*)p.src;
+    const float f = p.scale ? *p.scale : 1.0f;
+    const bool vec = p.ld % V == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+#pragma unroll
+    for (int i = tid; i < 64 * 64 / V; i += 256) {
+        const int r = i / (64 / V), c = i % (64 / V) * V;
+        T x[V];
+        const T* q = src + (long long)(ry + r) * p.ld + cx + c;
+        if (vec && ry + r < p.R && cx + c + V <= p.C) *reinterpret_cast<u32x4*>(x) = *reinterpret_cast<const u32x4*>(q);
+        else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] = (ry + r < p.R && cx + c + e < p.C) ? q[e] : (T)0.f;
+        }
+        E h[V], l[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            if constexpr (sizeof(T) == 4) split<E>((float)x[e] * f, h[e], l[e]);
+            else h[e] = x[e];
+            hi[r][c + e] = h[e];
+            if constexpr (sizeof(T) == 4) lo[r][c + e] = l[e];
+        }
+        if (p.r0 && ry + r < p.R) {
+            const long long at = (long long)(ry + r) * p.Cp + cx + c;
+            if constexpr (sizeof(T) == 4) {
+                *reinterpret_cast<u32x2*>((E*)p.r0 + at) = *reinterpret_cast<u32x2*>(h);
+                *reinterpret_cast<u32x2*>((E*)p.r1 + at) = *reinterpret_cast<u32x2*>(l);
+            } else *reinterpret_cast<u32x4*>((E*)p.r0 + at) = *reinterpret_cast<u32x4*>(h);
         }
     }
-    if (!c0) return;
+    if (!p.c0) return;
     __syncthreads();
-    for (int i = tid; i < 64 * 64; i += 256) {
-        const int c = i >> 6, r = i & 63;
-        if (cx + c < C) {
-            c0[(long long)(cx + c) * Rp + ry + r] = hi[r][c];
-            if constexpr (sizeof(T) == 4) c1[(long long)(cx + c) * Rp + ry + r] = lo[r][c];
+#pragma unroll
+    for (int i = tid; i < 64 * 8; i += 256) {
+        const int c = i >> 3, r = (i & 7) * 8;
+        if (cx + c >= p.C) continue;
+        const long long at = (long long)(cx + c) * p.Rp + ry + r;
+        E h[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = hi[r + e][c];
+        *reinterpret_cast<u32x4*>((E*)p.c0 + at) = *reinterpret_cast<u32x4*>(h);
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] = lo[r + e][c];
+            *reinterpret_cast<u32x4*>((E*)p.c1 + at) = *reinterpret_cast<u32x4*>(h);
         }
     }
 }
@@ -410,6 +462,7 @@ __global__ __launch_bounds__(256) void bias_kernel(const float* colpart, int blo
     const int v = blockIdx.x * 256 + threadIdx.x;
     if (v >= V) return;
     float s = 0.f;
+#pragma unroll 16
     for (int b = 0; b < blocks; ++b) s += colpart[(long long)b * V + v];
     out[v] = (T)(s * (*f0 * *f1));
 }
@@ -428,30 +481,38 @@ struct Space {
     }
 };
 
-// a tile of 256 x 256 when there are enough of them for the 256 CUs, of 128 x 128 (two workgroups a CU) otherwise
-struct Shape { bool big; int tiles_m, tiles_n; };
-inline Shape shape_of(int M, int N) {
-    const long long big = up(M, 256) / 256 * (up(N, 256) / 256);
-    const bool b = big >= 192;
-    const int t = b ? 256 : 128;
-    return {b, (int)(up(M, t) / t), (int)(up(N, t) / t)};
-}
-inline Shape resized(const Shape& s, int M, int N) { const int t = s.big ? 256 : 128; return {s.big, (int)(up(M, t) / t), (int)(up(N, t) / t)}; }
-// few tiles: the contraction in pieces of at least four K tiles, up to two workgroups a CU
-inline int splits_of(const Shape& s, long long ktiles) {
-    const long long tiles = (long long)s.tiles_m * s.tiles_n, want = s.big ? 256 : 512;
-    long long k = (want + tiles / 2) / tiles;
-    if (k > ktiles / 4) k = ktiles / 4;
-    return (int)(k < 1 ? 1 : (k > 32 ? 32 : k));
+// Tile of a GEMM and the pieces of its contraction.  Measured on whole cards of tiles (us a K tile of 64 of every tile that runs at once) and
+// on a few of them alone: 256 x 256 with eight waves, one workgroup a CU: 1.9 / 1.6; 128 x 128 with four, two a CU: 1.2 / 0.7; 64 x 64
+// with two, two a CU, three K tiles in flight: 0.65 / 0.4 (at 8192 x 2048 x 8192: 1140, 890 and 440 TFLOP/s).  A round of tiles begins
+// and ends with some 4 us.  Pieces of the contraction cost a pass over their fp32 results.  The cheapest of these sums is taken.
+struct Shape { int tile, tiles_m, tiles_n, splits; };
+inline Shape resized(const Shape& s, int M, int N) { return {s.tile, (int)(up(M, s.tile) / s.tile), (int)(up(N, s.tile) / s.tile), s.splits}; }
+inline Shape shape_of(long long M, long long N, long long ktiles, bool may_split) {
+    static const struct { int tile, slots; double full, few; } cfg[3] = {{256, 256, 1.9, 1.6}, {128, 512, 1.2, 0.7}, {64, 512, 0.65, 0.4}};
+    Shape best{};
+    double least = 0.0;
+    for (const auto& c : cfg) {
+        const long long tiles = up(M, c.tile) / c.tile * (up(N, c.tile) / c.tile);
+        for (int k = 1; k <= (may_split ? 32 : 1) && (k == 1 || ktiles / k >= 4); ++k) {
+            const long long wgs = tiles * k, rounds = (wgs + c.slots - 1) / c.slots;
+            const double fill = rounds > 1 ? 1.0 : (double)wgs / c.slots, each = c.few + (c.full - c.few) * fill;
+            const double cost = rounds * (4.0 + (double)((ktiles + k - 1) / k) * each) + (k > 1 ? 4.0 + (double)M * N * 4.0 * (k + 1) / 3e6 : 0.0);
+            if (best.tile == 0 || cost < least) {
+                least = cost;
+                best = {c.tile, (int)(up(M, c.tile) / c.tile), (int)(up(N, c.tile) / c.tile), k};
+            }
+        }
+    }
+    return best;
 }
 
-template <typename E, typename T, int BM, int BN, int WM, int WN, int EP>
+template <typename E, typename T, int BM, int BN, int WM, int WN, int ST, int EP>
 int go(const Gemm& p, hipStream_t st) {
-    static const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_kernel<E, T, BM, BN, WM, WN, EP>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<BM, BN>());
+    static const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_kernel<E, T, BM, BN, WM, WN, ST, EP>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<BM, BN, ST>());
     if (rc != hipSuccess) { set_error("linear_ce: cannot raise the dynamic LDS limit: %s", hipGetErrorString(rc)); return ICAP_ERR_HIP_BASE + (int)rc; }
-    hipLaunchKernelGGL((gemm_kernel<E, T, BM, BN, WM, WN, EP>), dim3((unsigned)(p.tiles_m * p.tiles_n), p.ksplit), dim3(WM * WN * 64),
-                       (smem_bytes<BM, BN>()), st, p);
+    hipLaunchKernelGGL((gemm_kernel<E, T, BM, BN, WM, WN, ST, EP>), dim3((unsigned)(p.tiles_m * p.tiles_n), p.ksplit), dim3(WM * WN * 64),
+                       (smem_bytes<BM, BN, ST>()), st, p);
     return launch_status("linear_ce");
 }
 
@@ -459,7 +520,10 @@ template <typename E, typename T, int EP>
 int gemm(Gemm& p, const Shape& s, hipStream_t st) {
     p.tiles_m = s.tiles_m;
     p.tiles_n = s.tiles_n;
-    return s.big ? go<E, T, 256, 256, 2, 4, EP>(p, st) : go<E, T, 128, 128, 2, 2, EP>(p, st);
+    p.ksplit = s.splits;
+    if (s.tile == 256) return go<E, T, 256, 256, 2, 4, 2, EP>(p, st);
+    if (s.tile == 128) return go<E, T, 128, 128, 2, 2, 2, EP>(p, st);
+    return go<E, T, 64, 64, 2, 1, 4, EP>(p, st);
 }
 
 struct Call {
@@ -506,25 +570,24 @@ Operand<T> room(Space& ws, const void* x, long long ld, int R, int C, bool want_
 }
 
 template <typename T>
-void fill(const Operand<T>& o, const void* x, long long ld, int R, int C, bool is_direct, const float* scale, hipStream_t st) {
-    typedef typename Of<T>::E E;
-    if (is_direct && !o.col0) return;
-    hipLaunchKernelGGL((planes_kernel<T, E>), dim3((unsigned)(up(C, 64) / 64), (unsigned)(up(R, 64) / 64)), dim3(256), 0, st, (const T*)x, ld, R, C,
-                       (int)up(R, 64), (int)up(C, 64), scale, is_direct ? (E*)nullptr : o.row0, o.row1, o.col0, o.col1);
+Turn turn_of(const Operand<T>& o, const void* x, long long ld, int R, int C, bool is_direct, const float* scale) {
+    Turn t{x, ld, R, C, (int)up(R, 64), (int)up(C, 64), (int)(up(C, 64) / 64), scale, is_direct ? nullptr : (void*)o.row0, o.row1, o.col0, o.col1, 0};
+    if (!is_direct || o.col0) t.blocks = (int)(up(R, 64) / 64) * t.tiles_c;
+    return t;
 }
 
 template <typename T>
 struct Plan {
     bool dh_direct, dw_direct;
     Operand<T> h, w;
-    float *scales, *amax;
+    float* amax;
     // forward
     float2* part; float* target_logit; int strips;
     // backward
     int piece; long long ldd, ldt;
     typename Of<T>::E *d0, *d1, *t0, *t1;
     float *colpart, *acc_h, *acc_w;
-    Shape s_logit, s_h, s_w; int k_h, k_w;
+    Shape s_logit, s_h, s_w;
     long long bytes;
 
     Plan(const Call& c, bool backward, char* base) {
@@ -535,9 +598,10 @@ struct Plan {
         if (!base) dh_direct = dw_direct = false;           // the size is asked for without pointers: the larger of the two
         h = room<T>(ws, c.h, c.ld_h, c.R, c.E, backward, dh_direct);
         w = room<T>(ws, c.w, c.ld_w, c.V, c.E, backward, dw_direct);
-        scales = ws.take<float>(8);
-        amax = ws.take<float>(2 * AMAX_WGS);
+        const int pairs = Of<T>::planes == 2 ? 3 : 1;
+        amax = ws.take<float>(Of<T>::planes == 2 && !backward ? 2 * AMAX_WGS : 0);
         if (!backward) {
+            s_logit = shape_of(c.R, c.V, up(c.E, 64) / 64 * pairs, false);
             strips = (int)(up(c.V, STRIP) / STRIP);
             part = ws.take<float2>((long long)c.R * strips);
             target_logit = ws.take<float>(c.R);
@@ -554,36 +618,35 @@ struct Plan {
             t0 = ws.take<E>(piece * ldt);
             d1 = t1 = nullptr;
             if (Of<T>::planes == 2) { d1 = ws.take<E>(c.R * ldd); t1 = ws.take<E>(piece * ldt); }
-            const int pairs = Of<T>::planes == 2 ? 3 : 1;
-            s_logit = shape_of(c.R, piece);
-            s_h = shape_of(c.R, c.E);
-            s_w = shape_of(piece, c.E);
-            k_h = splits_of(s_h, ldd / 64 * pairs);
-            k_w = splits_of(s_w, ldt / 64 * pairs);
+            s_logit = shape_of(c.R, piece, up(c.E, 64) / 64 * pairs, false);
+            s_h = shape_of(c.R, c.E, ldd / 64 * pairs, true);
+            s_w = shape_of(piece, c.E, ldt / 64 * pairs, true);
             colpart = ws.take<float>((long long)s_logit.tiles_m * 2 * c.V);
-            acc_h = ws.take<float>((k_h > 1 || piece < c.V) ? (long long)k_h * c.R * c.E : 0);
-            acc_w = ws.take<float>(k_w > 1 ? (long long)k_w * piece * c.E : 0);
+            acc_h = ws.take<float>((s_h.splits > 1 || piece < c.V) ? (long long)s_h.splits * c.R * c.E : 0);
+            acc_w = ws.take<float>(s_w.splits > 1 ? (long long)s_w.splits * piece * c.E : 0);
         }
         bytes = ws.at;
     }
 };
 
+// scales: five floats, written by the forward call (fp32 tensors) and read by the backward one
 template <typename T>
-void operands(const Call& c, Plan<T>& p, hipStream_t st) {
+void operands(const Call& c, Plan<T>& p, float* scales, bool backward, hipStream_t st) {
     const float *sh = nullptr, *sw = nullptr;
     if constexpr (sizeof(T) == 4) {
-        hipLaunchKernelGGL(amax_kernel, dim3(AMAX_WGS), dim3(256), 0, st, (const float*)c.h, c.ld_h, c.R, c.E, p.amax);
-        hipLaunchKernelGGL(amax_kernel, dim3(AMAX_WGS), dim3(256), 0, st, (const float*)c.w, c.ld_w, c.V, c.E, p.amax + AMAX_WGS);
-        hipLaunchKernelGGL(scales_kernel, dim3(1), dim3(256), 0, st, p.amax, p.amax + AMAX_WGS, p.scales);
-        sh = p.scales;
-        sw = p.scales + 2;
+        if (!backward) {
+            hipLaunchKernelGGL(amax_kernel, dim3(2 * AMAX_WGS), dim3(256), 0, st, (const float*)c.h, c.ld_h, c.R, (const float*)c.w, c.ld_w, c.V, c.E, p.amax);
+            hipLaunchKernelGGL(scales_kernel, dim3(1), dim3(256), 0, st, p.amax, scales);
+        }
+        sh = scales;
+        sw = scales + 2;
     }
-    fill<T>(p.h, c.h, c.ld_h, c.R, c.E, p.dh_direct, sh, st);
-    fill<T>(p.w, c.w, c.ld_w, c.V, c.E, p.dw_direct, sw, st);
+    const Turn a = turn_of<T>(p.h, c.h, c.ld_h, c.R, c.E, p.dh_direct, sh), b = turn_of<T>(p.w, c.w, c.ld_w, c.V, c.E, p.dw_direct, sw);
+    if (a.blocks + b.blocks > 0) hipLaunchKernelGGL((planes_kernel<T, typename Of<T>::E>), dim3(a.blocks + b.blocks), dim3(256), 0, st, a, b);
 }
 
 template <typename T>
-Gemm logits(const Call& c, const Plan<T>& p, int v0, int vn) {
+Gemm logits(const Call& c, const Plan<T>& p, const float* scales, int v0, int vn) {
     Gemm g{};
     g.a0 = (const unsigned short*)p.h.row0;
     g.a1 = (const unsigned short*)p.h.row1;
@@ -593,8 +656,7 @@ Gemm logits(const Call& c, const Plan<T>& p, int v0, int vn) {
     g.ldb = p.w.ld;
     g.M = c.R; g.N = vn; g.K = (int)up(c.E, 64);
     g.pairs = Of<T>::planes == 2 ? 3 : 1;
-    g.ksplit = 1;
-    g.unscale = sizeof(T) == 4 ? p.scales + 4 : nullptr;
+    g.unscale = sizeof(T) == 4 ? scales + 4 : nullptr;
     g.bias = c.bias; g.targets = c.targets; g.ignore = c.ignore; g.V = c.V; g.v0 = v0;
     return g;
 }
@@ -603,10 +665,10 @@ template <typename T>
 int fwd(const Call& c, int mean_over_valid, float* row_loss, float* row_lse, float* out, char* ws, hipStream_t st) {
     typedef typename Of<T>::E E;
     Plan<T> p(c, false, ws);
-    operands<T>(c, p, st);
-    Gemm g = logits<T>(c, p, 0, c.V);
+    operands<T>(c, p, out + 2, false, st);
+    Gemm g = logits<T>(c, p, out + 2, 0, c.V);
     g.part = p.part; g.strips = p.strips; g.target_logit = p.target_logit;
-    if (int rc = gemm<E, T, EP_LSE>(g, shape_of(c.R, c.V), st)) return rc;
+    if (int rc = gemm<E, T, EP_LSE>(g, p.s_logit, st)) return rc;
     hipLaunchKernelGGL(lse_kernel, dim3((c.R + 3) / 4), dim3(256), 0, st, p.part, p.strips, p.target_logit, c.targets, c.R, c.V, c.ignore, row_loss, row_lse);
     hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, c.targets, c.R, c.V, c.ignore, mean_over_valid, out);
     return launch_status("linear_ce_fwd");
@@ -616,11 +678,12 @@ template <typename T>
 int bwd(const Call& c, const float* row_lse, const float* meta, const float* grad_out, void* dh, void* dw, void* db, char* ws, hipStream_t st) {
     typedef typename Of<T>::E E;
     Plan<T> p(c, true, ws);
-    operands<T>(c, p, st);
+    float* scales = const_cast<float*>(meta) + 2;
+    operands<T>(c, p, scales, true, st);
     const float back = __is_same(E, _Float16) ? 1.0f / D_SCALE : 1.0f;
     for (int v0 = 0; v0 < c.V; v0 += p.piece) {
         const int vn = c.V - v0 < p.piece ? c.V - v0 : p.piece;
-        Gemm g = logits<T>(c, p, v0, vn);
+        Gemm g = logits<T>(c, p, scales, v0, vn);
         g.lse = row_lse;
         g.d0 = (unsigned short*)p.d0; g.d1 = (unsigned short*)p.d1; g.t0 = (unsigned short*)p.t0; g.t1 = (unsigned short*)p.t1;
         g.ldd = p.ldd; g.ldt = p.ldt;
@@ -634,15 +697,14 @@ int bwd(const Call& c, const float* row_lse, const float* meta, const float* gra
             q.lda = p.ldd; q.ldb = p.w.ldc;
             q.M = c.R; q.N = c.E; q.K = (int)up(vn, 64);
             q.pairs = g.pairs;
-            q.ksplit = p.k_h;
-            q.f0 = grad_out; q.f1 = meta + 1; q.f2 = sizeof(T) == 4 ? p.scales + 3 : nullptr; q.f = back;
-            const bool whole = p.k_h == 1 && p.piece >= c.V;
+            q.f0 = grad_out; q.f1 = meta + 1; q.f2 = sizeof(T) == 4 ? scales + 3 : nullptr; q.f = back;
+            const bool whole = p.s_h.splits == 1 && p.piece >= c.V;
             if (whole) { q.out = dh; q.ldo = c.E; }
             else { q.acc = p.acc_h; q.accumulate = v0 > 0; }
             if (int rc = gemm<E, T, EP_OUT>(q, p.s_h, st)) return rc;
             if (!whole && v0 + vn == c.V) {
                 const long long n = (long long)c.R * c.E;
-                hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(up(n, 1024) / 1024 > 4096 ? 4096 : up(n, 1024) / 1024)), dim3(256), 0, st, p.acc_h, p.k_h, n,
+                hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(up(n, 1024) / 1024 > 4096 ? 4096 : up(n, 1024) / 1024)), dim3(256), 0, st, p.acc_h, p.s_h.splits, n,
                                    (T*)dh, q);
             }
         }
@@ -653,15 +715,14 @@ int bwd(const Call& c, const float* row_lse, const float* meta, const float* gra
             q.lda = p.ldt; q.ldb = p.h.ldc;
             q.M = vn; q.N = c.E; q.K = (int)up(c.R, 64);
             q.pairs = g.pairs;
-            q.ksplit = p.k_w;
-            q.f0 = grad_out; q.f1 = meta + 1; q.f2 = sizeof(T) == 4 ? p.scales + 1 : nullptr; q.f = back;
+            q.f0 = grad_out; q.f1 = meta + 1; q.f2 = sizeof(T) == 4 ? scales + 1 : nullptr; q.f = back;
             T* dst = (T*)dw + (long long)v0 * c.E;
-            if (p.k_w == 1) { q.out = dst; q.ldo = c.E; }
+            if (p.s_w.splits == 1) { q.out = dst; q.ldo = c.E; }
             else q.acc = p.acc_w;
             if (int rc = gemm<E, T, EP_OUT>(q, resized(p.s_w, vn, c.E), st)) return rc;
-            if (p.k_w > 1) {
+            if (p.s_w.splits > 1) {
                 const long long n = (long long)vn * c.E;
-                hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(up(n, 1024) / 1024 > 4096 ? 4096 : up(n, 1024) / 1024)), dim3(256), 0, st, p.acc_w, p.k_w, n, dst, q);
+                hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(up(n, 1024) / 1024 > 4096 ? 4096 : up(n, 1024) / 1024)), dim3(256), 0, st, p.acc_w, p.s_w.splits, n, dst, q);
             }
         }
     }
@@ -676,8 +737,9 @@ static int check(int dtype, const Call& c, const char* what) {
         set_error("%s: null tensor, empty size or overlapping rows", what);
         return ICAP_ERR_ARG;
     }
-    // blocks of 64 rows are a grid's second index, tiles are counted in 32 bits
-    if (c.R > 65535 * 64 || c.E > (1 << 20) || c.V > 65535 * 64 || up(c.R, 128) / 128 * (up(c.V, 128) / 128) > 0x7fffffffLL) {
+    // tiles and blocks of 64 x 64 values are counted in 32 bits
+    if (c.R > 65535 * 64 || c.E > (1 << 20) || c.V > 65535 * 64 || up(c.R, 64) / 64 * (up(c.V, 64) / 64) > 0x7fffffffLL ||
+        (up(c.R, 64) + up(c.V, 64)) / 64 * (up(c.E, 64) / 64) > 0x7fffffffLL) {
         set_error("%s: rows=%d width=%d vocabulary=%d too large", what, c.R, c.E, c.V);
         return ICAP_ERR_LIMIT;
     }

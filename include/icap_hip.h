@@ -857,8 +857,9 @@ int icap_attention_packed_bwd(int dtype, const void* dout, const void* q, const 
 
 /* Cross entropy of a Linear layer without its logits in memory: x = hidden weight^T + bias, loss_r = log sum_v exp x_rv -
  * x_r,target (0 for ignored rows: target == ignore_index or outside [0, vocab)); hidden [rows][width] (rows ld_h apart), weight
- * [vocab][width] (ld_w), bias [vocab] or NULL, all of one type.  out[0] = loss, out[1] = the scale every row was weighted with,
- * as in icap_ce_loss_fwd_f32 (mean_over_valid likewise); row_loss, row_lse [rows] fp32.
+ * [vocab][width] (ld_w), bias [vocab] or NULL, all of one type.  out [8] fp32: out[0] = loss, out[1] = the scale every row was
+ * weighted with, as in icap_ce_loss_fwd_f32 (mean_over_valid likewise), the others are for the backward call; row_loss, row_lse
+ * [rows] fp32.
  * Backward: gradients of grad_out[0] (device scalar) * loss in the tensors' type, dense: dhidden [rows][width], dweight
  * [vocab][width], dbias [vocab]; each may be NULL.  fp32 products are fp32-accurate; magnitudes of fp32 hidden and weight below 2^74.
  * ws: icap_linear_ce_ws_bytes(dtype, rows, width, vocab, backward) bytes, 16-byte aligned: bounded by about
