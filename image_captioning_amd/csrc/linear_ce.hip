@@ -61,6 +61,16 @@ __device__ __forceinline__ void load16(const void* g, unsigned char* lds_wave_ba
     __builtin_amdgcn_global_load_lds(g, (__attribute__((address_space(3))) void*)(lds_wave_base), 16, 0, 0);
 }
 
+// accumulator row of register e, for lanes 0-31 (lanes 32-63: + 4)
+__device__ __forceinline__ constexpr int acc_row(int e) { return (e & 3) + 8 * (e >> 2); }
+
+// op over a lane and lane ^ 32
+template <typename F>
+__device__ __forceinline__ float other_half(float v, F op) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 __device__ __forceinline__ float final_factor(const Gemm& p) {
     float f = p.f;
     if (p.f0) f *= *p.f0;
@@ -83,10 +93,11 @@ template <int BM, int BN, int ST> constexpr int smem_bytes() { return ST * (BM +
 // fetches is permuted by its row, and the fragment reads apply the same permutation, so that 16 rows meet 16 different slots.
 template <typename E, typename T, int BM, int BN, int WM, int WN, int ST, int EP>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
-    constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, RM = TM / 32, RN = TN / 32, RPP = NW * 8;
+    constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, RM = TM / 32, RN = 2, RPP = NW * 8;
     static_assert(TN == STRIP && TM % 32 == 0 && BM % RPP == 0 && BN % RPP == 0, "wave tiles");
-    constexpr int APT = BM / RPP, BPT = BN / RPP, A_BYTES = BM * ROWB, STAGE = (BM + BN) * ROWB, EP_LD = TN + 4;
-    static_assert(NW * 32 * EP_LD * 4 <= ST * STAGE, "the waves' result images fit the staging buffers");
+    constexpr int APT = BM / RPP, BPT = BN / RPP, A_BYTES = BM * ROWB, STAGE = (BM + BN) * ROWB;
+    constexpr int IMG = 9216, LD4 = TN + 4, LD2 = TN + 8;       // a wave's image of 32 rows: bytes; row lengths of fp32 and 16-bit ones
+    static_assert(NW * IMG <= ST * STAGE && 32 * LD4 * 4 <= IMG && 2 * 32 * LD2 * 2 <= IMG, "the waves' result images fit the staging buffers");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave - wm * WN, lr = lane & 31, lh = lane >> 5;
 
@@ -137,7 +148,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
 #pragma unroll
             for (int i = 0; i < RM; ++i)
 #pragma unroll
-                for (int j = 0; j < RN; ++j) acc[i][j] = Mma<E>::go(af[i], bf[j], acc[i][j]);
+                for (int j = 0; j < RN; ++j) acc[i][j] = Mma<E>::go(bf[j], af[i], acc[i][j]);
         }
     };
     if (t_lo < t_hi) {
@@ -157,132 +168,186 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 
-    // epilogue, every wave on its own, 32 rows at a time: accumulators -> the wave's image in LDS -> eight columns a lane, eight lanes a row
-    float* ew = reinterpret_cast<float*>(smem) + wave * 32 * EP_LD;
+    // Epilogue, every wave on its own, 32 rows at a time.  The products were formed transposed (B's rows as the first operand), so a lane
+    // holds row lane % 32 of C, columns 32 j + acc_row(e) + 4 (lane / 32): a row's statistics stay in two lanes, four
+    // columns are neighbours, and what goes to memory passes the LDS in 8- and 16-byte pieces.
+    unsigned char* img = smem + wave * IMG;
     const float un = p.unscale ? *p.unscale : 1.0f;
-    const float ff = EP == EP_OUT ? (p.acc ? 1.0f : final_factor(p)) : 1.0f;
-    const int c8 = lane & 7, n = n0 + wn * TN + 8 * c8;         // this lane's first column
-    float bias[8], colsum[8];
+    const int nb = n0 + wn * TN;                                // the wave's first column
+    const bool edge = nb + TN > p.N;                            // some columns do not exist
     if constexpr (EP != EP_OUT) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            colsum[e] = 0.f;
-            bias[e] = (p.bias && n + e < p.N) ? (float)((const T*)p.bias)[p.v0 + n + e] : 0.f;
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < RM; ++i) {
+        f32x4 bias[RN][4];
 #pragma unroll
         for (int j = 0; j < RN; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) ew[((e & 3) + 8 * (e >> 2) + 4 * lh) * EP_LD + j * 32 + lr] = acc[i][j][e];
+            for (int g = 0; g < 4; ++g)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int row = q * 8 + (lane >> 3), m = m0 + wm * TM + i * 32 + row;
-            float* im = ew + row * EP_LD + 8 * c8;
-            const f32x4 x0 = *reinterpret_cast<const f32x4*>(im), x1 = *reinterpret_cast<const f32x4*>(im + 4);
-            float v[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
-            if constexpr (EP == EP_LSE) {
-                const long long t = m < p.M ? p.targets[m] - p.v0 : -1;
-                float mx = -INFINITY;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    v[e] = n + e < p.N ? fmaf(v[e], un, bias[e]) : -INFINITY;
-                    mx = fmaxf(mx, v[e]);
-                    if (t == n + e && n + e < p.N) p.target_logit[m] = v[e];
+                for (int e = 0; e < 4; ++e) {
+                    const int n = nb + j * 32 + 8 * g + 4 * lh + e;
+                    bias[j][g][e] = (p.bias && n < p.N) ? (float)((const T*)p.bias)[p.v0 + n] : 0.f;
                 }
-                mx = fmaxf(mx, dpp_f<DPP_QUAD_SWAP1>(mx));
-                mx = fmaxf(mx, dpp_f<DPP_QUAD_SWAP2>(mx));
-                mx = fmaxf(mx, dpp_f<DPP_HALF_MIRROR>(mx));
-                const float base = mx == -INFINITY ? 0.f : mx;
+        f32x4 colsum[RN][4] = {};
+#pragma unroll
+        for (int i = 0; i < RM; ++i) {
+            const int mb = m0 + wm * TM + i * 32, m = mb + lr, mm = min(m, p.M - 1);
+            const long long target = p.targets[mm];
+            const int t = (target >= 0 && target < p.V) ? (int)target - p.v0 - nb : -1;         // the target's column of this strip
+            float x[RN][16];
+#pragma unroll
+            for (int j = 0; j < RN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[j][e] = fmaf(acc[i][j][e], un, bias[j][e >> 2][e & 3]);
+            if (edge) {
+#pragma unroll
+                for (int j = 0; j < RN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (j * 32 + acc_row(e) + 4 * lh >= p.N - nb) x[j][e] = -INFINITY;
+            }
+            if constexpr (EP == EP_LSE) {
+                float mx = x[0][0];
+#pragma unroll
+                for (int j = 0; j < RN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, x[j][e]);
+                mx = other_half(mx, [](float a, float b) { return fmaxf(a, b); });
+                const float base = mx == -INFINITY ? 0.f : mx * LOG2E;
                 float s = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) s += __builtin_amdgcn_exp2f((v[e] - base) * LOG2E);
-                s += dpp_f<DPP_QUAD_SWAP1>(s);
-                s += dpp_f<DPP_QUAD_SWAP2>(s);
-                s += dpp_f<DPP_HALF_MIRROR>(s);
+                for (int j = 0; j < RN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(fmaf(x[j][e], LOG2E, -base));
+                s = other_half(s, [](float a, float b) { return a + b; });
                 const int strip = tile_n * WN + wn;
-                if (c8 == 0 && m < p.M && strip < p.strips) p.part[(long long)m * p.strips + strip] = make_float2(mx, s);
-            } else if constexpr (EP == EP_GRAD) {
-                const int mm = min(m, p.M - 1);
-                const long long tg = p.targets[mm];
-                const bool on = m < p.M && tg >= 0 && tg < p.V && tg != p.ignore;
-                const float lse = p.lse[mm];
-                const long long t = tg - p.v0;
-                typename Vec<E>::x8 hi, lo;
+                if (lh == 0 && m < p.M && strip < p.strips) p.part[(long long)m * p.strips + strip] = make_float2(mx, s);
+                if (__any(t >= 0 && t < TN)) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float d = __builtin_amdgcn_exp2f((fmaf(v[e], un, bias[e]) - lse) * LOG2E);
-                    if (t == n + e) d -= 1.0f;
-                    d = (on && n + e < p.N) ? d : 0.f;
-                    colsum[e] += d;
-                    if constexpr (sizeof(E) == 2 && !__is_same(E, __bf16)) d *= D_SCALE;
-                    v[e] = d;
-                    E h, l;
-                    split<E>(d, h, l);
-                    hi[e] = h;
-                    lo[e] = l;
+                    for (int j = 0; j < RN; ++j)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (t == j * 32 + acc_row(e) + 4 * lh && m < p.M) p.target_logit[m] = x[j][e];
                 }
-                if (m < p.M && n < p.cols_pad) {
-                    *reinterpret_cast<typename Vec<E>::x8*>(p.d0 + (long long)m * p.ldd + n) = hi;
-                    if constexpr (sizeof(T) == 4) *reinterpret_cast<typename Vec<E>::x8*>(p.d1 + (long long)m * p.ldd + n) = lo;
-                }
-                *reinterpret_cast<f32x4*>(im) = f32x4{v[0], v[1], v[2], v[3]};
-                *reinterpret_cast<f32x4*>(im + 4) = f32x4{v[4], v[5], v[6], v[7]};
             } else {
-                if (m < p.M && n < p.N) {
-                    if (p.acc) {
-                        float* o = p.acc + ((long long)blockIdx.y * p.M + m) * p.N + n;
-                        if (p.N % 4 == 0 && n + 8 <= p.N) {
-                            f32x4 y0 = x0, y1 = x1;
-                            if (p.accumulate) { y0 += *reinterpret_cast<const f32x4*>(o); y1 += *reinterpret_cast<const f32x4*>(o + 4); }
-                            *reinterpret_cast<f32x4*>(o) = y0;
-                            *reinterpret_cast<f32x4*>(o + 4) = y1;
-                        } else {
-                            for (int e = 0; e < 8 && n + e < p.N; ++e) o[e] = p.accumulate ? o[e] + v[e] : v[e];
-                        }
-                    } else {
-                        T* o = (T*)p.out + (long long)m * p.ldo + n;
-                        if (p.ldo % 8 == 0 && n + 8 <= p.N) {
-                            typename Vec<T>::x8 y;
+                const bool on = m < p.M && target >= 0 && target < p.V && target != p.ignore;
+                const float lse2 = p.lse[mm] * LOG2E;
+                const bool here = __any(t >= 0 && t < TN);
+                E* hi = reinterpret_cast<E*>(img);
+                E* lo = hi + 32 * LD2;
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) y[e] = (T)(v[e] * ff);
-                            *reinterpret_cast<typename Vec<T>::x8*>(o) = y;
-                        } else {
-                            for (int e = 0; e < 8 && n + e < p.N; ++e) o[e] = (T)(v[e] * ff);
+                for (int j = 0; j < RN; ++j)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        typename Vec<E>::x4 h4, l4;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float d = __builtin_amdgcn_exp2f(fmaf(x[j][4 * g + e], LOG2E, -lse2));
+                            if (here && t == j * 32 + 8 * g + 4 * lh + e) d -= 1.0f;
+                            d = on ? d : 0.f;
+                            colsum[j][g][e] += d;
+                            if constexpr (!__is_same(E, __bf16)) d *= D_SCALE;
+                            E h, l;
+                            split<E>(d, h, l);
+                            h4[e] = h;
+                            l4[e] = l;
                         }
+                        *reinterpret_cast<typename Vec<E>::x4*>(hi + lr * LD2 + j * 32 + 8 * g + 4 * lh) = h4;
+                        if constexpr (sizeof(T) == 4) *reinterpret_cast<typename Vec<E>::x4*>(lo + lr * LD2 + j * 32 + 8 * g + 4 * lh) = l4;
+                    }
+#pragma unroll
+                for (int part = 0; part < (sizeof(T) == 4 ? 2 : 1); ++part) {
+                    const E* im = part ? lo : hi;
+                    unsigned short* d = part ? p.d1 : p.d0;
+                    unsigned short* tr = part ? p.t1 : p.t0;
+                    // rows: eight lanes of 16 bytes each
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int row = q * 8 + (lane >> 3), c = (lane & 7) * 8;
+                        if (mb + row < p.M && nb + c < p.cols_pad)
+                            *reinterpret_cast<u32x4*>(d + (long long)(mb + row) * p.ldd + nb + c) = *reinterpret_cast<const u32x4*>(im + row * LD2 + c);
+                    }
+                    // columns: the transposing LDS read hands a lane four rows of its column at a time
+                    const int col = lane & 48;
+                    u32x4 out[4];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        typedef __attribute__((address_space(3))) i16x4* lds_ptr;
+                        const i16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(im + (4 * r + ((lane & 15) >> 2)) * LD2 + col + (lane & 3) * 4));
+                        const u32x2 w = __builtin_bit_cast(u32x2, v);
+                        out[r >> 1][(r & 1) * 2] = w[0];
+                        out[r >> 1][(r & 1) * 2 + 1] = w[1];
+                    }
+                    if (nb + lane < p.N && mb < p.rows_pad) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) *reinterpret_cast<u32x4*>(tr + (long long)(nb + lane) * p.ldt + mb + 8 * r) = out[r];
                     }
                 }
             }
         }
         if constexpr (EP == EP_GRAD) {
-            // the same 32 rows transposed: a lane takes a column
-            const int nn = n0 + wn * TN + lane, mb = m0 + wm * TM + i * 32;
-            if (nn < p.N && mb < p.rows_pad) {
+            if (p.colpart) {
+                // 32 rows of each column are spread over 32 lanes
 #pragma unroll
-                for (int r8 = 0; r8 < 4; ++r8) {
-                    typename Vec<E>::x8 hi, lo;
+                for (int j = 0; j < RN; ++j)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        E h, l;
-                        split<E>(ew[(r8 * 8 + e) * EP_LD + lane], h, l);
-                        hi[e] = h;
-                        lo[e] = l;
-                    }
-                    *reinterpret_cast<typename Vec<E>::x8*>(p.t0 + (long long)nn * p.ldt + mb + r8 * 8) = hi;
-                    if constexpr (sizeof(T) == 4) *reinterpret_cast<typename Vec<E>::x8*>(p.t1 + (long long)nn * p.ldt + mb + r8 * 8) = lo;
-                }
+                    for (int g = 0; g < 4; ++g)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float v = colsum[j][g][e];
+                            v += dpp_f<DPP_QUAD_SWAP1>(v);
+                            v += dpp_f<DPP_QUAD_SWAP2>(v);
+                            v += dpp_f<DPP_HALF_MIRROR>(v);
+                            v += dpp_f<DPP_ROW_MIRROR>(v);
+                            v += __shfl_xor(v, 16);
+                            const int n = nb + j * 32 + 8 * g + 4 * lh + e;
+                            if (lr == 0 && n < p.N) p.colpart[(long long)(tile_m * WM + wm) * p.ldc + p.v0 + n] = v;
+                        }
             }
         }
-    }
-    if constexpr (EP == EP_GRAD) {
-        if (p.colpart) {
+    } else {
+        const float f = p.acc ? 1.0f : final_factor(p);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                colsum[e] += __shfl_xor(colsum[e], 8);
-                colsum[e] += __shfl_xor(colsum[e], 16);
-                colsum[e] += __shfl_xor(colsum[e], 32);
-                if (lane < 8 && n + e < p.N) p.colpart[(long long)(tile_m * WM + wm) * p.ldc + p.v0 + n + e] = colsum[e];
+        for (int i = 0; i < RM; ++i) {
+            const int mb = m0 + wm * TM + i * 32;
+            if (sizeof(T) == 4 || p.acc) {
+                float* im = reinterpret_cast<float*>(img);
+#pragma unroll
+                for (int j = 0; j < RN; ++j)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        *reinterpret_cast<f32x4*>(im + lr * LD4 + j * 32 + 8 * g + 4 * lh) =
+                            f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]} * f;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const int row = q * 4 + (lane >> 4), c = (lane & 15) * 4, m = mb + row, n = nb + c;
+                    f32x4 v = *reinterpret_cast<const f32x4*>(im + row * LD4 + c);
+                    if (m >= p.M || n >= p.N) continue;
+                    float* o = p.acc ? p.acc + ((long long)blockIdx.y * p.M + m) * p.N + n : (float*)p.out + (long long)m * p.ldo + n;
+                    const bool add = p.acc && p.accumulate;
+                    if (p.N % 4 == 0) {
+                        if (add) v += *reinterpret_cast<const f32x4*>(o);
+                        *reinterpret_cast<f32x4*>(o) = v;
+                    } else {
+                        for (int e = 0; e < 4 && n + e < p.N; ++e) o[e] = add ? o[e] + v[e] : v[e];
+                    }
+                }
+            } else if constexpr (sizeof(T) == 2) {
+                T* im = reinterpret_cast<T*>(img);
+#pragma unroll
+                for (int j = 0; j < RN; ++j)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        *reinterpret_cast<typename Vec<T>::x4*>(im + lr * LD2 + j * 32 + 8 * g + 4 * lh) =
+                            __builtin_convertvector(f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]} * f, typename Vec<T>::x4);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int row = q * 8 + (lane >> 3), c = (lane & 7) * 8, m = mb + row, n = nb + c;
+                    const typename Vec<T>::x8 v = *reinterpret_cast<const typename Vec<T>::x8*>(im + row * LD2 + c);
+                    if (m >= p.M || n >= p.N) continue;
+                    T* o = (T*)p.out + (long long)m * p.ldo + n;
+                    if (p.N % 8 == 0) *reinterpret_cast<typename Vec<T>::x8*>(o) = v;
+                    else
+                        for (int e = 0; e < 8 && n + e < p.N; ++e) o[e] = v[e];
+                }
             }
         }
     }
