@@ -18,23 +18,22 @@
 
 namespace icap {
 
-constexpr int AT_MAX = 40;                  // tensors a launch: 40 x 88 bytes of kernel arguments (the limit is 4096)
+constexpr int AT_MAX = 62;                  // tensors a launch: 62 x 64 bytes of kernel arguments (the limit is 4096)
 constexpr int AT_BLOCK = 256;               // values that share a scale
-constexpr int AT_WAVE_BLOCKS = 4;           // blocks a wave walks over
+constexpr int AT_WAVE_BLOCKS = 4;           // blocks a wave owns
 constexpr int AT_CHUNK = 4 * AT_WAVE_BLOCKS * AT_BLOCK;      // values a workgroup of four waves owns
+constexpr unsigned AT_VEC = 1u << 31;       // in AdamTensor::index: four values can be read at once
 
 struct AdamTensor {
     void* p; const void* g; void* m; void* v; float* ms; float* vs;
     long long n;
-    unsigned first;                         // first workgroup
-    int index, step, vec;                   // place in the caller's list; step (or what is added to *step_dev); 16-byte access
-    float step_size, inv_bc2_sqrt;
+    unsigned first, index;                  // first workgroup; place in the caller's list
 };
 
 struct AdamTable {
     AdamTensor t[AT_MAX];
-    int count;
-    float decay, one_minus_b1, b2, one_minus_b2, eps, grad_scale;
+    int count, step;                        // one step for all (or what is added to *step_dev)
+    float decay, one_minus_b1, b2, one_minus_b2, eps, grad_scale, step_size, inv_bc2_sqrt;
     unsigned long long seed;
     const int* step_dev;
     double lr, beta1, beta2;
@@ -83,6 +82,48 @@ __device__ __forceinline__ float round_at_random(float y, float u, unsigned r16)
     return (u > 0.f && z == 0.f) ? 0.001953125f : z;
 }
 
+// the update of a lane's four values; 8-bit states come and go as codes, with the block's scales
+template <int BITS>
+__device__ __forceinline__ void adamw_four(const AdamTable& a, float step_size, float inv_bc2, unsigned long long key, long long place, f32x4& p, f32x4 g,
+                                           f32x4& m, f32x4& v, unsigned& mc, unsigned& vc, float& ms, float& vs) {
+    if constexpr (BITS == 8) {
+        m = codes_to_f32(mc) * ms;
+        v = codes_to_f32(vc) * vs;
+        v = v * v;
+    }
+    f32x4 u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float gr = g[e] * a.grad_scale;
+        m[e] = m[e] + (gr - m[e]) * a.one_minus_b1;
+        v[e] = v[e] * a.b2 + (gr * gr) * a.one_minus_b2;
+        u[e] = sqrtf(v[e]);
+        const float denom = u[e] * inv_bc2 + a.eps;
+        p[e] = p[e] * a.decay - (m[e] / denom) * step_size;
+    }
+    if constexpr (BITS == 8) {
+        float most_m = 0.f, most_u = 0.f;               // places behind the tensor's end hold zeros
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { most_m = fmaxf(most_m, fabsf(m[e])); most_u = fmaxf(most_u, u[e]); }
+        float im, iu;
+        block_scale(wave_max(most_m), ms, im);
+        block_scale(wave_max(most_u), vs, iu);
+        const unsigned long long draw = mix64(key + 0x9E3779B97F4A7C15ULL * (unsigned long long)(place >> 2));
+        f32x4 ym, yu;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float y = m[e] * im;
+            y = y > 448.0f ? 448.0f : y;                // comparisons, not min / max: a NaN stays one
+            ym[e] = y < -448.0f ? -448.0f : y;
+            float z = u[e] * iu;
+            z = z > 448.0f ? 448.0f : z;
+            yu[e] = round_at_random(z, iu > 0.f ? u[e] : 0.f, (unsigned)(draw >> (16 * e)) & 0xFFFFu);
+        }
+        mc = f32_to_codes(ym);
+        vc = f32_to_codes(yu);
+    }
+}
+
 template <typename P, typename G, int BITS>
 __global__ __launch_bounds__(256) void adamw_tensors_kernel(const AdamTable a) {
     // the tensor this workgroup belongs to: the last one that starts at or before it
@@ -92,11 +133,11 @@ __global__ __launch_bounds__(256) void adamw_tensors_kernel(const AdamTable a) {
         if (a.t[mid].first <= blockIdx.x) lo = mid; else hi = mid;
     }
     const AdamTensor& t = a.t[lo];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long n = t.n, base = (long long)(blockIdx.x - t.first) * AT_CHUNK + wave * (AT_WAVE_BLOCKS * AT_BLOCK);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long n = t.n, base = (long long)(blockIdx.x - t.first) * AT_CHUNK + wave * (AT_WAVE_BLOCKS * AT_BLOCK), blk = base / AT_BLOCK;
     if (base >= n) return;
-    int step = t.step;
-    float step_size = t.step_size, inv_bc2 = t.inv_bc2_sqrt;
+    int step = a.step;
+    float step_size = a.step_size, inv_bc2 = a.inv_bc2_sqrt;
     if (a.step_dev) {                       // the count lives in device memory (a launch in a HIP graph keeps its arguments)
         step += *a.step_dev;
         step_size = (float)(a.lr / (1.0 - pow(a.beta1, (double)step)));
@@ -104,83 +145,66 @@ __global__ __launch_bounds__(256) void adamw_tensors_kernel(const AdamTable a) {
     }
     P* p = (P*)t.p;
     const G* g = (const G*)t.g;
-    const bool vec = t.vec;
+    float *m32 = (float*)t.m, *v32 = (float*)t.v;
+    unsigned char *m8 = (unsigned char*)t.m, *v8 = (unsigned char*)t.v;
     unsigned long long key = 0;
-    if constexpr (BITS == 8) key = mix64(a.seed + 0x9E3779B97F4A7C15ULL * ((unsigned long long)step * (1ull << 20) + t.index));
+    if constexpr (BITS == 8) key = mix64(a.seed + 0x9E3779B97F4A7C15ULL * ((unsigned long long)step * (1ull << 20) + (t.index & ~AT_VEC)));
 
+    if ((t.index & AT_VEC) && base + AT_WAVE_BLOCKS * AT_BLOCK <= n) {
+        // everything is asked for before anything is used: the loads of four blocks are in flight together
+        f32x4 pp[AT_WAVE_BLOCKS], gg[AT_WAVE_BLOCKS], mm[AT_WAVE_BLOCKS], vv[AT_WAVE_BLOCKS];
+        unsigned mc[AT_WAVE_BLOCKS], vc[AT_WAVE_BLOCKS];
+        float ms[AT_WAVE_BLOCKS], vs[AT_WAVE_BLOCKS];
+        const long long i0 = base + lane * 4;
 #pragma unroll
-    for (int b = 0; b < AT_WAVE_BLOCKS; ++b) {
+        for (int b = 0; b < AT_WAVE_BLOCKS; ++b) {
+            const long long i = i0 + b * AT_BLOCK;
+            pp[b] = load4<P>(p + i);
+            gg[b] = load4<G>(g + i);
+            if constexpr (BITS == 32) { mm[b] = load4<float>(m32 + i); vv[b] = load4<float>(v32 + i); }
+            else {
+                mc[b] = *reinterpret_cast<const unsigned*>(m8 + i);
+                vc[b] = *reinterpret_cast<const unsigned*>(v8 + i);
+                ms[b] = t.ms[blk + b];
+                vs[b] = t.vs[blk + b];
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < AT_WAVE_BLOCKS; ++b) {
+            const long long i = i0 + b * AT_BLOCK;
+            adamw_four<BITS>(a, step_size, inv_bc2, key, i, pp[b], gg[b], mm[b], vv[b], mc[b], vc[b], ms[b], vs[b]);
+            put4<P>(p + i, pp[b]);
+            if constexpr (BITS == 32) { put4<float>(m32 + i, mm[b]); put4<float>(v32 + i, vv[b]); }
+            else {
+                *reinterpret_cast<unsigned*>(m8 + i) = mc[b];
+                *reinterpret_cast<unsigned*>(v8 + i) = vc[b];
+                if (lane == 0) { t.ms[blk + b] = ms[b]; t.vs[blk + b] = vs[b]; }
+            }
+        }
+        return;
+    }
+    // a tensor's end, or one that is not aligned: value by value
+    for (int b = 0; b < AT_WAVE_BLOCKS && base + b * AT_BLOCK < n; ++b) {
         const long long i = base + b * AT_BLOCK + lane * 4;
-        if (base + b * AT_BLOCK >= n) break;
         const int have = i + 4 <= n ? 4 : (i < n ? (int)(n - i) : 0);
-        const bool whole = vec && have == 4;
         f32x4 pp = {0.f, 0.f, 0.f, 0.f}, gg = pp, mm = pp, vv = pp;
         unsigned mc = 0, vc = 0;
-        if (whole) {
-            pp = load4<P>(p + i);
-            gg = load4<G>(g + i);
-            if constexpr (BITS == 32) { mm = load4<float>((const float*)t.m + i); vv = load4<float>((const float*)t.v + i); }
-            else { mc = *reinterpret_cast<const unsigned*>((const char*)t.m + i); vc = *reinterpret_cast<const unsigned*>((const char*)t.v + i); }
-        } else {
-            for (int e = 0; e < have; ++e) {
-                pp[e] = (float)p[i + e];
-                gg[e] = (float)g[i + e];
-                if constexpr (BITS == 32) { mm[e] = ((const float*)t.m)[i + e]; vv[e] = ((const float*)t.v)[i + e]; }
-                else { mc |= (unsigned)((const unsigned char*)t.m)[i + e] << (8 * e); vc |= (unsigned)((const unsigned char*)t.v)[i + e] << (8 * e); }
-            }
+        float ms = 0.f, vs = 0.f;
+        for (int e = 0; e < have; ++e) {
+            pp[e] = (float)p[i + e];
+            gg[e] = (float)g[i + e];
+            if constexpr (BITS == 32) { mm[e] = m32[i + e]; vv[e] = v32[i + e]; }
+            else { mc |= (unsigned)m8[i + e] << (8 * e); vc |= (unsigned)v8[i + e] << (8 * e); }
         }
-        if constexpr (BITS == 8) {
-            const long long blk = base / AT_BLOCK + b;
-            mm = codes_to_f32(mc) * t.ms[blk];
-            vv = codes_to_f32(vc) * t.vs[blk];
-            vv = vv * vv;
+        if constexpr (BITS == 8) { ms = t.ms[blk + b]; vs = t.vs[blk + b]; }
+        adamw_four<BITS>(a, step_size, inv_bc2, key, i, pp, gg, mm, vv, mc, vc, ms, vs);
+        for (int e = 0; e < have; ++e) {
+            p[i + e] = (P)pp[e];
+            if constexpr (BITS == 32) { m32[i + e] = mm[e]; v32[i + e] = vv[e]; }
+            else { m8[i + e] = (unsigned char)(mc >> (8 * e)); v8[i + e] = (unsigned char)(vc >> (8 * e)); }
         }
-        f32x4 u;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float gr = gg[e] * a.grad_scale;
-            mm[e] = mm[e] + (gr - mm[e]) * a.one_minus_b1;
-            vv[e] = vv[e] * a.b2 + (gr * gr) * a.one_minus_b2;
-            u[e] = sqrtf(vv[e]);
-            const float denom = u[e] * inv_bc2 + a.eps;
-            pp[e] = pp[e] * a.decay - (mm[e] / denom) * step_size;
-        }
-        if constexpr (BITS == 8) {
-            const long long blk = base / AT_BLOCK + b;
-            float most_m = 0.f, most_u = 0.f;           // places behind the tensor's end hold zeros
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { most_m = fmaxf(most_m, fabsf(mm[e])); most_u = fmaxf(most_u, u[e]); }
-            most_m = wave_max(most_m);
-            most_u = wave_max(most_u);
-            float sm, im, su, iu;
-            block_scale(most_m, sm, im);
-            block_scale(most_u, su, iu);
-            const unsigned long long draw = mix64(key + 0x9E3779B97F4A7C15ULL * (unsigned long long)(i >> 2));
-            f32x4 ym, yu;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float y = mm[e] * im;
-                y = y > 448.0f ? 448.0f : y;            // comparisons, not min / max: a NaN stays one
-                ym[e] = y < -448.0f ? -448.0f : y;
-                float z = u[e] * iu;
-                z = z > 448.0f ? 448.0f : z;
-                yu[e] = round_at_random(z, iu > 0.f ? u[e] : 0.f, (unsigned)(draw >> (16 * e)) & 0xFFFFu);
-            }
-            mc = f32_to_codes(ym);
-            vc = f32_to_codes(yu);
-            if (lane == 0) { t.ms[blk] = sm; t.vs[blk] = su; }
-        }
-        if (whole) {
-            put4<P>(p + i, pp);
-            if constexpr (BITS == 32) { put4<float>((float*)t.m + i, mm); put4<float>((float*)t.v + i, vv); }
-            else { *reinterpret_cast<unsigned*>((char*)t.m + i) = mc; *reinterpret_cast<unsigned*>((char*)t.v + i) = vc; }
-        } else {
-            for (int e = 0; e < have; ++e) {
-                p[i + e] = (P)pp[e];
-                if constexpr (BITS == 32) { ((float*)t.m)[i + e] = mm[e]; ((float*)t.v)[i + e] = vv[e]; }
-                else { ((unsigned char*)t.m)[i + e] = (unsigned char)(mc >> (8 * e)); ((unsigned char*)t.v)[i + e] = (unsigned char)(vc >> (8 * e)); }
-            }
-        }
+        if constexpr (BITS == 8)
+            if (lane == 0) { t.ms[blk + b] = ms; t.vs[blk + b] = vs; }
     }
 }
 
@@ -222,39 +246,48 @@ int adamw_tensors(int count, void* const* p, const void* const* g, void* const* 
     a.seed = seed;
     a.step_dev = step_dev;
     a.lr = lr; a.beta1 = beta1; a.beta2 = beta2;
-    int i = 0;
+    // tensors of one step go together (a parameter that got its first gradient late has a count of its own)
     bool any = false;
-    while (i < count) {
-        a.count = 0;
-        unsigned blocks = 0;
-        for (; i < count && a.count < AT_MAX; ++i) {
-            if (n[i] == 0) continue;
-            const long long need = (n[i] + AT_CHUNK - 1) / AT_CHUNK;
-            if (blocks + need > 0x7fffffffLL) break;
-            AdamTensor& t = a.t[a.count++];
-            t.p = p[i]; t.g = g[i]; t.m = m[i]; t.v = v[i];
-            t.ms = bits == 8 ? ms[i] : nullptr;
-            t.vs = bits == 8 ? vs[i] : nullptr;
-            t.n = n[i];
-            t.first = blocks;
-            t.index = index[i];
-            t.step = steps[i];
-            const size_t sp = 4 * size_of(p_dtype), sg = 4 * size_of(g_dtype), ss = bits == 8 ? 4 : 16;
-            t.vec = (uintptr_t)p[i] % sp == 0 && (uintptr_t)g[i] % sg == 0 && (uintptr_t)m[i] % ss == 0 && (uintptr_t)v[i] % ss == 0;
-            if (!step_dev) {
-                t.step_size = (float)(lr / (1.0 - pow(beta1, (double)steps[i])));
-                t.inv_bc2_sqrt = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)steps[i])));
-            }
-            blocks += (unsigned)need;
+    long long above = -(1ll << 40);
+    for (;;) {
+        long long step = 1ll << 40;
+        for (int i = 0; i < count; ++i)
+            if (n[i] > 0 && steps[i] > above && steps[i] < step) step = steps[i];
+        if (step == 1ll << 40) break;
+        above = step;
+        a.step = (int)step;
+        if (!step_dev) {
+            a.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
+            a.inv_bc2_sqrt = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
         }
-        if (!blocks) continue;
-        any = true;
-        const int key = p_dtype * 3 + g_dtype;
-        if (key == DT_F32 * 3 + DT_F32) adamw_go<float, float>(a, bits, blocks, st);
-        else if (key == DT_BF16 * 3 + DT_BF16) adamw_go<__bf16, __bf16>(a, bits, blocks, st);
-        else if (key == DT_BF16 * 3 + DT_F32) adamw_go<__bf16, float>(a, bits, blocks, st);
-        else if (key == DT_F16 * 3 + DT_F16) adamw_go<_Float16, _Float16>(a, bits, blocks, st);
-        else adamw_go<_Float16, float>(a, bits, blocks, st);
+        int i = 0;
+        while (i < count) {
+            a.count = 0;
+            unsigned blocks = 0;
+            for (; i < count && a.count < AT_MAX; ++i) {
+                if (n[i] == 0 || steps[i] != step) continue;
+                const long long need = (n[i] + AT_CHUNK - 1) / AT_CHUNK;
+                if (blocks + need > 0x7fffffffLL) break;
+                AdamTensor& t = a.t[a.count++];
+                t.p = p[i]; t.g = g[i]; t.m = m[i]; t.v = v[i];
+                t.ms = bits == 8 ? ms[i] : nullptr;
+                t.vs = bits == 8 ? vs[i] : nullptr;
+                t.n = n[i];
+                t.first = blocks;
+                const size_t sp = 4 * size_of(p_dtype), sg = 4 * size_of(g_dtype), ss = bits == 8 ? 4 : 16;
+                const bool vec = (uintptr_t)p[i] % sp == 0 && (uintptr_t)g[i] % sg == 0 && (uintptr_t)m[i] % ss == 0 && (uintptr_t)v[i] % ss == 0;
+                t.index = (unsigned)index[i] | (vec ? AT_VEC : 0u);
+                blocks += (unsigned)need;
+            }
+            if (!blocks) continue;
+            any = true;
+            const int key = p_dtype * 3 + g_dtype;
+            if (key == DT_F32 * 3 + DT_F32) adamw_go<float, float>(a, bits, blocks, st);
+            else if (key == DT_BF16 * 3 + DT_BF16) adamw_go<__bf16, __bf16>(a, bits, blocks, st);
+            else if (key == DT_BF16 * 3 + DT_F32) adamw_go<__bf16, float>(a, bits, blocks, st);
+            else if (key == DT_F16 * 3 + DT_F16) adamw_go<_Float16, _Float16>(a, bits, blocks, st);
+            else adamw_go<_Float16, float>(a, bits, blocks, st);
+        }
     }
     return any ? launch_status("adamw_tensors") : ICAP_OK;
 }

@@ -599,8 +599,9 @@ struct Call {
     long long ignore;
 };
 
-// bytes of D and D^T that a piece of the vocabulary may take: what the last-level cache holds beside its operands
-constexpr long long PIECE_BYTES = 256ll << 20;
+// bytes of D and D^T that a piece of the vocabulary may take: twice the last-level cache (half as many bytes
+// cost 12 % at 6756 words x 4864 rows, which then needed two pieces; twice as many gain 0.5 % at 65536 x 8192)
+constexpr long long PIECE_BYTES = 512ll << 20;
 
 template <typename T> struct Of { typedef T E; static constexpr int planes = 1; };
 template <> struct Of<float> { typedef _Float16 E; static constexpr int planes = 2; };

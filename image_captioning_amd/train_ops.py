@@ -566,7 +566,7 @@ def adamw_state8(p):
 
 def adamw_tensors(params, grads, exp_avg, exp_avg_sq, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=1e-2, grad_scale=1.0,
                   seed=0, index=None, step_dev=None):
-    """One AdamW update (training.AdamW's arithmetic, in fp32) of a list of tensors where they lie, in place, some 40 tensors a launch.
+    """One AdamW update (training.AdamW's arithmetic, in fp32) of a list of tensors where they lie, in place, some 60 tensors a launch.
 
     params: fp32, bf16 or fp16, contiguous; grads: their gradients, of the same type or fp32 (None: the tensor is left alone).
     exp_avg, exp_avg_sq: fp32 tensors (states of 32 bits), or (codes, scales) pairs (states of 8 bits: adamw_state8; the second one

@@ -293,7 +293,7 @@ class AdamW:
 
 class AdamWTensors:
     """AdamW's update over the parameters where they lie - fp32, bf16 or fp16, not moved into a flat buffer, with their own .grad -
-    some 40 tensors a launch (train_ops.adamw_tensors).  state_bits 8: both moments in one byte a value (a quarter of the
+    some 60 tensors a launch (train_ops.adamw_tensors).  state_bits 8: both moments in one byte a value (a quarter of the
     memory of fp32 states, 4 instead of 16 bytes of traffic a value); 32: fp32 states, results as AdamW's.
 
     A parameter without a gradient is left alone and its own step count does not advance, as in torch.  The randomness of the

@@ -863,7 +863,7 @@ int icap_attention_packed_bwd(int dtype, const void* dout, const void* q, const 
  * Backward: gradients of grad_out[0] (device scalar) * loss in the tensors' type, dense: dhidden [rows][width], dweight
  * [vocab][width], dbias [vocab]; each may be NULL.  fp32 products are fp32-accurate; magnitudes of fp32 hidden and weight below 2^74.
  * ws: icap_linear_ce_ws_bytes(dtype, rows, width, vocab, backward) bytes, 16-byte aligned: bounded by about
- * 256 MB and copies of hidden and weight, whatever the vocabulary. */
+ * 512 MB, fp32 partial results and copies of hidden and weight, whatever the vocabulary. */
 long long icap_linear_ce_ws_bytes(int dtype, int rows, int width, int vocab, int backward);
 int icap_linear_ce_fwd(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
                        const long long* targets, int rows, int width, int vocab, long long ignore_index, int mean_over_valid,
