@@ -105,9 +105,9 @@ struct Direct {
     }
 };
 
-// everything this wave asked for has landed, and every wave is here
+// everything this wave asked for (in LDS, too) has landed, and every wave is here
 __device__ __forceinline__ void landed() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
@@ -254,6 +254,7 @@ __device__ __forceinline__ Sight sight_of(Span s) {
     w.mine = s;
     w.some = {wave_min_i(none ? 0x7fffffff : s.lo), -wave_min_i(none ? 0x7fffffff : -s.hi)};
     w.all = {-wave_min_i(-s.lo), wave_min_i(s.hi)};
+    if (w.some.lo == 0x7fffffff) w.some = {0, 0};
     return w;
 }
 
@@ -283,6 +284,48 @@ __device__ __forceinline__ Span tile_rows(const AttnArgs& a, int key0, int key, 
     sight = sight_of(key < end ? rows_of(a, e, key) : Span{0, 0});
     const Edge e0 = edge_of(a, s0), e1 = edge_of(a, s1);
     return {rows_of(a, e0, key0).lo, rows_of(a, e1, j1).hi};
+}
+
+// ------------------------------------------------------------------------------------------------ values that are not finite
+// What a row does not see has the weight zero, but zero times an infinity or a NaN is not zero, and a tile's products meet the keys of
+// all its rows.  So a row (key) whose results are not all finite is formed once more, by its two lanes, from what it sees and nothing
+// else.  Slow, and never reached by finite tensors whose results are finite.
+template <int ND>
+__device__ __forceinline__ bool finite_row(const f32x16 (&x)[ND]) {
+    float z = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z = fmaf(x[d][e], 0.f, z);
+    z += __shfl_xor(z, 32);
+    return z == 0.f;
+}
+// x . y, half of the columns by each of the two lanes that share a row
+template <typename T>
+__device__ __forceinline__ float pair_dot(const T* x, const T* y, int dim) {
+    float s = 0.f;
+    for (int c = ((threadIdx.x & 63) >> 5) * 8; c < dim; c += 16) {
+        const auto a = *reinterpret_cast<const typename Vec<T>::x8*>(x + c), b = *reinterpret_cast<const typename Vec<T>::x8*>(y + c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf((float)a[e], (float)b[e], s);
+    }
+    return s + __shfl_xor(s, 32);
+}
+// a lane's columns of a result row (store16's) += w x
+template <typename T, int ND>
+__device__ __forceinline__ void add_row(f32x16 (&acc)[ND], float w, const T* x, int dim) {
+    const int lh = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = d * 32 + 8 * g + 4 * lh;
+            if (c < dim) {
+                const auto v = *reinterpret_cast<const typename Vec<T>::x4*>(x + c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[d][4 * g + i] = fmaf(w, (float)v[i], acc[d][4 * g + i]);
+            }
+        }
 }
 
 // ------------------------------------------------------------------------------------------------ forward
@@ -385,7 +428,23 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && (NW < 4 || sizeof(T) == 4) ? 
             for (int u = 0; u < NS; ++u) s = unit(s, n0 + 32 * u, sv[buf], 32 * u, sk[buf], 32 * u);
         }
     }
-    const float sum = l + __shfl_xor(l, 32);
+    float sum = l + __shfl_xor(l, 32);
+    if (!finite_row(o)) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] = zeros16();
+        m = -INFINITY;
+        sum = 0.f;
+        for (int j = max(me.mine.lo, keys.lo); j < min(me.mine.hi, keys.hi) && sum == sum; ++j) {       // one NaN in the sum: all is NaN
+            const long long at = j - keys.lo;
+            const float s = pair_dot(qp, kb + at * a.k_tok, a.dim) * c2, most = fmaxf(m, s), base = most == -INFINITY ? 0.f : most;
+            const float alpha = __builtin_amdgcn_exp2f(m - base), p = __builtin_amdgcn_exp2f(s - base);
+            sum = fmaf(sum, alpha, p);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d] *= alpha;
+            add_row(o, p, vb + at * a.v_tok, a.dim);
+            m = most;
+        }
+    }
     if (row >= total) return;
     const long long at = (long long)tok * a.heads + head;
     const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);        // no key: zeros; NaN stays
@@ -452,15 +511,42 @@ __global__ __launch_bounds__(256) void delta_kernel(const AttnArgs a) {
     if (part == 0 && r < rows) a.delta[r] = s;
 }
 
-// dQ: the forward's shape (rows in registers, keys staged), with dO beside Q and dS in P's place
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, DP == 128 && (NW < 4 || sizeof(T) == 4) ? 1 : 2) void dq_kernel(const AttnArgs a) {
-    constexpr int NTHR = NW * 64, BM = NW * 32, BN = step_keys<T>(), NS = BN / 32, KK = DP / 16, ND = DP / 32;
-    __shared__ __attribute__((aligned(1024))) T sk[2][BN * DP];
-    __shared__ __attribute__((aligned(1024))) T sv[2][BN * DP];
+// adds up the accumulators of the G waves that share rows (or keys), in the first of them; at: where a lane's values go in LDS
+template <int ND, int G>
+__device__ __forceinline__ void join_waves(f32x16 (&x)[ND], float* at, int group) {
+#pragma unroll
+    for (int g = 1; g < G; ++g) {
+        __syncthreads();
+        if (group == g) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) at[(d * 16 + e) * 64] = x[d][e];
+        }
+        __syncthreads();
+        if (group == 0) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[d][e] += at[(d * 16 + e) * 64];
+        }
+    }
+}
+
+// dQ: the forward's shape (rows in registers, keys staged), with dO beside Q and dS in P's place.
+// RW waves of 32 rows each, KG times: key groups take every KG-th 32 keys of a step, as the row groups of dK and dV do (one causal
+// sequence of 4096 tokens, 16 heads of 64, forward and backward: 329 -> 299 us; sequences of 200 tokens: 160 -> 163)
+template <typename T, int DP, int RW, int KG>
+__global__ __launch_bounds__(RW * KG * 64, DP == 128 && (RW < 4 || sizeof(T) == 4) ? 1 : 2) void dq_kernel(const AttnArgs a) {
+    constexpr int NTHR = RW * KG * 64, BM = RW * 32, BN = KG > 1 ? 32 * KG : step_keys<T>(), NS = BN / 32 / KG, KK = DP / 16, ND = DP / 32;
+    __shared__ __attribute__((aligned(1024))) T staged[4][BN * DP];
+    static_assert(KG == 1 || sizeof(staged) >= RW * 64 * ND * 16 * 4, "dQ of a key group fits the tiles");
+    T (*const sk)[BN * DP] = staged;
+    T (*const sv)[BN * DP] = staged + 2;
+    const int wave = threadIdx.x >> 6, kg = wave / RW, rw = wave - kg * RW;
     const int kvh = blockIdx.x % a.kv_heads, tiles = gridDim.x / a.kv_heads, lane = threadIdx.x & 63, lh = lane >> 5;
     const int tile = a.causal ? tiles - 1 - (int)(blockIdx.x / a.kv_heads) : blockIdx.x / a.kv_heads;
-    const int row0 = tile * BM, row = row0 + (threadIdx.x >> 6) * 32 + (lane & 31), total = a.tokens_q * a.group;
+    const int row0 = tile * BM, row = row0 + rw * 32 + (lane & 31), total = a.tokens_q * a.group;
     const int tok = min(row, total - 1) / a.group, head = kvh * a.group + min(row, total - 1) - tok * a.group;
     const long long at = (long long)tok * a.heads + head;
     Sight me;
@@ -491,8 +577,8 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && (NW < 4 || sizeof(T) == 4) ? 
         landed();
         if (n0 + BN < keys.hi) load(n0 + BN, buf ^ 1);
 #pragma unroll
-        for (int kt = 0; kt < NS; ++kt) {
-            const int n1 = n0 + kt * 32;
+        for (int ks = 0; ks < NS; ++ks) {
+            const int kt = kg * NS + ks, n1 = n0 + kt * 32;
             if (n1 >= me.some.hi || n1 + 32 <= me.some.lo) continue;
             f32x16 s = zeros16(), dp = zeros16();
 #pragma unroll
@@ -514,6 +600,21 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && (NW < 4 || sizeof(T) == 4) ? 
 #pragma unroll
                 for (int d = 0; d < ND; ++d) dq[d] = mma32(col_frag<T, DP>(sk[buf], kt * 32 + j * 16, d * 32), df, dq[d]);
             }
+        }
+    }
+    if constexpr (KG > 1) {
+        join_waves<ND, KG>(dq, reinterpret_cast<float*>(staged) + rw * (64 * ND * 16) + lane, kg);
+        if (kg > 0) return;
+    }
+    if (!finite_row(dq)) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d) dq[d] = zeros16();
+        float ds = 0.f;
+        for (int j = me.mine.lo; j < me.mine.hi && ds == ds; ++j) {
+            const T* kp = kb + (long long)j * a.k_tok;
+            const float p = __builtin_amdgcn_exp2f(fmaf(pair_dot(qp, kp, a.dim), c2, -lse2));
+            ds = p * (pair_dot(gp, vb + (long long)j * a.v_tok, a.dim) - delta);
+            add_row(dq, ds, kp, a.dim);
         }
     }
     if (row >= total) return;
@@ -571,7 +672,6 @@ __global__ __launch_bounds__(KW * RG * 64, DP == 128 ? 1 : 2) void dkv_kernel(co
     const float c2 = a.scale * LOG2E;
     int buf = 0;
     for (int r0 = rows.lo; r0 < rows.hi; r0 += BR, buf ^= 1) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         landed();
         if (r0 + BR < rows.hi) fetch(r0 + BR, buf ^ 1);
         const int r1 = r0 + mine;
@@ -609,29 +709,27 @@ __global__ __launch_bounds__(KW * RG * 64, DP == 128 ? 1 : 2) void dkv_kernel(co
         }
     }
     if constexpr (RG > 1) {
-        float* sum = reinterpret_cast<float*>(tiles) + kw * (64 * ND * 16) + lane;
-        auto add = [&](f32x16 (&x)[ND]) __attribute__((always_inline)) {
-#pragma unroll
-            for (int g = 1; g < RG; ++g) {
-                __syncthreads();
-                if (rg == g) {
-#pragma unroll
-                    for (int d = 0; d < ND; ++d)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) sum[(d * 16 + e) * 64] = x[d][e];
-                }
-                __syncthreads();
-                if (rg == 0) {
-#pragma unroll
-                    for (int d = 0; d < ND; ++d)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) x[d][e] += sum[(d * 16 + e) * 64];
-                }
-            }
-        };
-        add(dk);
-        add(dv);
+        float* at = reinterpret_cast<float*>(tiles) + kw * (64 * ND * 16) + lane;
+        join_waves<ND, RG>(dk, at, rg);
+        join_waves<ND, RG>(dv, at, rg);
         if (rg > 0) return;
+    }
+    if (!finite_row(dk) || !finite_row(dv)) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zeros16();
+        const long long kk = min(key, a.tokens_k - 1);
+        const T* kp = (const T*)a.k + kk * a.k_tok + (long long)kvh * a.k_head;
+        const T* vp = (const T*)a.v + kk * a.v_tok + (long long)kvh * a.v_head;
+        float p = 0.f;
+        for (int r = me.mine.lo; r < me.mine.hi && p == p; ++r) {
+            const int t = r / a.group, h = r - t * a.group;
+            const T* qp = qb + t * a.q_tok + h * a.q_head;
+            const T* gp = gb + t * a.g_tok + h * a.g_head;
+            const long long at = (long long)t * a.heads + kvh * a.group + h;
+            p = __builtin_amdgcn_exp2f(fmaf(pair_dot(qp, kp, a.dim), c2, -a.lse[at] * LOG2E));
+            add_row(dv, p, gp, a.dim);
+            add_row(dk, p * (pair_dot(gp, vp, a.dim) - a.delta[at]), qp, a.dim);
+        }
     }
     if (key >= a.tokens_k) return;
     const long long at = ((long long)key * a.kv_heads + kvh) * a.dim;
@@ -656,9 +754,9 @@ int launch_fwd(const AttnArgs& a, hipStream_t st) {
     }
     return launch_status("attention_packed_fwd");
 }
-template <typename T, int DP, int NW>
+template <typename T, int DP, int RW, int KG>
 void launch_dq(const AttnArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((dq_kernel<T, DP, NW>), dim3(blocks_for(a, (long long)a.tokens_q * a.group, NW * 32)), dim3(NW * 64), 0, st, a);
+    hipLaunchKernelGGL((dq_kernel<T, DP, RW, KG>), dim3(blocks_for(a, (long long)a.tokens_q * a.group, RW * 32)), dim3(RW * KG * 64), 0, st, a);
 }
 template <typename T, int DP, int KW, int RG>
 void launch_dkv(const AttnArgs& a, hipStream_t st) {
@@ -678,8 +776,8 @@ template <typename T, int DP>
 int bwd_dim(const AttnArgs& a, hipStream_t st) {
     const long long rows = (long long)a.tokens_q * a.group / a.seqs;
     if (a.tokens_q > 0) {
-        if (rows <= 96) launch_dq<T, DP, 2>(a, st);
-        else launch_dq<T, DP, 4>(a, st);
+        if (rows <= 96) launch_dq<T, DP, 2, 1>(a, st);
+        else launch_dq<T, DP, 2, 2>(a, st);
     }
     if (a.tokens_k > 0) {
         if (rows <= 96) launch_dkv<T, DP, 2, 1>(a, st);

@@ -185,6 +185,60 @@ def test_attention_hidden_keys_may_hold_anything():
         assert torch.equal(ops.attention_packed(q, k2, v, cu)[:-1], want[:-1])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("lq,lk,H,K,dim", [([20, 30, 100, 5], [20, 30, 100, 5], 4, 2, 64), ([9, 250, 300], [9, 250, 300], 2, 2, 40), ([1, 1, 1], [900, 1500, 40], 4, 1, 128)])
+def test_attention_sequences_do_not_touch_each_other(dtype, bad, lq, lk, H, K, dim):
+    """Sequence 1 holds NaN or infinities everywhere: the results of the others, which share its tiles, are the formula's."""
+    q, k, v, g = (rnd(sum(n), h, dim, seed=s, dtype=dtype) for n, h, s in ((lq, H, 1), (lk, K, 2), (lk, K, 3), (lq, H, 4)))
+    want = attention_oracle(q, k, v, lq, lk, True, dim ** -0.5, g)
+    rows, keys = slice(lq[0], lq[0] + lq[1]), slice(lk[0], lk[0] + lk[1])
+    for x, at in ((q, rows), (k, keys), (v, keys), (g, rows)):
+        x[at] = bad
+    got = run_attention(q.to(D), k.to(D), v.to(D), lq, lk, True, None, g.to(D))
+    for n, (w, b) in want.items():
+        others = torch.ones(len(w), dtype=torch.bool)
+        others[keys if n in ("dk", "dv") else rows] = False
+        within(got[n].cpu()[others], w[others], b[others], n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("n,dim", [(50, 64), (300, 128)])
+def test_attention_values_behind_a_token_do_not_touch_it(dtype, bad, n, dim):
+    """The last key and value are seen by the last query alone, the first query's row sees the first key alone."""
+    q, k, v, g = (rnd(n, 2, dim, seed=s, dtype=dtype) for s in (5, 6, 7, 8))
+    want = attention_oracle(q, k, v, [n], [n], True, dim ** -0.5, g)
+
+    def changed(x, at):
+        x = x.clone()
+        x[at] = bad
+        return x
+    got = run_attention(q.to(D), changed(k, -1).to(D), changed(v, -1).to(D), [n], [n], True, None, g.to(D))
+    for name in ("out", "lse", "dq"):
+        within(got[name].cpu()[:-1], want[name][0][:-1], want[name][1][:-1], name)
+    got = run_attention(changed(q, 0).to(D), k.to(D), v.to(D), [n], [n], True, None, changed(g, 0).to(D))
+    for name in ("out", "lse", "dq", "dk", "dv"):
+        within(got[name].cpu()[1:], want[name][0][1:], want[name][1][1:], name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_infinite_values_are_the_formulas(dtype):
+    """A visible key of the score -inf has the weight zero; a visible infinite value is the rows' result."""
+    q, k, v = (rnd(40, 1, 24, seed=s, dtype=dtype) for s in (1, 2, 3))
+    q[:, 0, 0] = 1.0
+    k2 = k.clone()
+    k2[7, 0, 0] = -math.inf
+    v2 = v.clone()
+    v2[9, 0, 3] = math.inf
+    got = run_attention(q.to(D), k2.to(D), v2.to(D), [40], [40], False)["out"].cpu()
+    left = torch.arange(40) != 7
+    w, b = attention_oracle(q, k[left], v[left], [40], [39], False, 24 ** -0.5)["out"]
+    cols = torch.arange(24) != 3
+    within(got[:, :, cols], w[:, :, cols], b[:, :, cols], "out")
+    assert (got[:, :, 3] == math.inf).all()
+
+
 def test_attention_offsets_beyond_the_tensors_are_cut_off():
     from image_captioning_amd import ops
     q, k, v = (rnd(40, 2, 32, seed=s).to(D) for s in (1, 2, 3))
