@@ -203,6 +203,7 @@ static inline long long align4(long long n) { return (n + 3) & ~3LL; }
     } while (0)
 
 long long linear_ce_ws_bytes(int, int, int, int, int);
+long long linear_ce_out_floats(int, int, int);
 int linear_ce_fwd(int, const void*, long long, const void*, long long, const void*, const long long*, int, int, int, long long, int, float*, float*,
                   float*, void*, long long, hipStream_t);
 int linear_ce_bwd(int, const void*, long long, const void*, long long, const void*, const long long*, int, int, int, long long, const float*,
@@ -1140,6 +1141,8 @@ int icap_attention_packed_bwd(int dtype, const void* dout, const void* q, const 
     const hipStream_t st = (hipStream_t)stream;
     return dtype == DT_F32 ? attention_bwd_f32(a, st) : dtype == DT_BF16 ? attention_bwd_bf16(a, st) : attention_bwd_f16(a, st);
 }
+
+long long icap_linear_ce_out_floats(int dtype, int rows, int vocab) { return linear_ce_out_floats(dtype, rows, vocab); }
 
 long long icap_linear_ce_ws_bytes(int dtype, int rows, int width, int vocab, int backward) {
     return linear_ce_ws_bytes(dtype, rows, width, vocab, backward);

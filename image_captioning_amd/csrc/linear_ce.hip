@@ -12,7 +12,10 @@
 //   fp16: D 2^14 is rounded to fp16, so that a probability of 1e-8 still has full precision; the factor leaves again exactly.
 //   fp32: every operand is the sum of two fp16 values (22 bits), scaled by a power of two so that its largest magnitude is near
 //   2^14; the products hi hi + hi lo + lo hi drop 2^-22 of each term: as exact as an fp32 dot product, at three fp16
-//   products for one (the fp32 matrix instruction takes sixteen times a 16-bit product).
+//   products for one (the fp32 matrix instruction takes sixteen times a 16-bit product).  For the logits every row of hidden and
+//   every word of the weight has a scale of its own, so that no row touches another; as the contraction of dh and dW runs over words
+//   and rows, those take one scale for all.
+// Rows that are left out are zeros in every operand that sums over rows, whatever they hold (NaN, infinities).
 // Bound: the matrix cores (2 R E V flops a product; one forward, three backward of which the logits are repeated).
 #include "packed.hpp"
 
@@ -30,7 +33,7 @@ struct Gemm {
     const unsigned short *a0, *a1, *b0, *b1;        // planes: high and (fp32 tensors) low parts
     long long lda, ldb;
     int M, N, K, pairs, ksplit, tiles_m, tiles_n;   // K % 64 == 0; pairs 1 or 3
-    const float* unscale;                           // one factor on the accumulators in device memory, or null
+    const float *urow, *ucol;                       // fp32: factors 2^-s of the logits' rows and columns
     // EP_LSE and EP_GRAD
     const void* bias;                               // type of the tensors
     const long long* targets;
@@ -172,7 +175,6 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
     // holds row lane % 32 of C, columns 32 j + acc_row(e) + 4 (lane / 32): a row's statistics stay in two lanes, four
     // columns are neighbours, and what goes to memory passes the LDS in 8- and 16-byte pieces.
     unsigned char* img = smem + wave * IMG;
-    const float un = p.unscale ? *p.unscale : 1.0f;
     const int nb = n0 + wn * TN;                                // the wave's first column
     const bool edge = nb + TN > p.N;                            // some columns do not exist
     if constexpr (EP != EP_OUT) {
@@ -193,10 +195,22 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
             const long long target = p.targets[mm];
             const int t = (target >= 0 && target < p.V) ? (int)target - p.v0 - nb : -1;         // the target's column of this strip
             float x[RN][16];
+            if constexpr (sizeof(T) == 4) {
+                const float ur = p.urow[mm];
 #pragma unroll
-            for (int j = 0; j < RN; ++j)
+                for (int j = 0; j < RN; ++j)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[j][e] = fmaf(acc[i][j][e], un, bias[j][e >> 2][e & 3]);
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x4 f = *reinterpret_cast<const f32x4*>(p.ucol + nb + j * 32 + 8 * g + 4 * lh) * ur;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[j][4 * g + e] = fmaf(acc[i][j][4 * g + e], f[e], bias[j][g][e]);
+                    }
+            } else {
+#pragma unroll
+                for (int j = 0; j < RN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[j][e] = acc[i][j][e] + bias[j][e >> 2][e & 3];
+            }
             if (edge) {
 #pragma unroll
                 for (int j = 0; j < RN; ++j)
@@ -375,11 +389,28 @@ __global__ __launch_bounds__(256) void lse_kernel(const float2* part, int strips
     }
 }
 
-// loss (its sum in 64 bits) and the scale of every row
+// largest of n values >= 0, by 1024 threads
+__device__ __forceinline__ float block_max(const float* x, int n, float* red) {
+    float m = 0.f;
+    for (int i = threadIdx.x; i < n; i += 1024) m = fmaxf(m, x[i]);
+    m = wave_max(m);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, red[i]);
+    return m;
+}
+
+// loss (its sum in 64 bits) and the scale of every row; fp32 (urow, ucol): the scales of whole tensors, from those of their rows
 __global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const long long* targets, int R, int V, long long ignore, int mean_over_valid,
-                                                    float* out) {
+                                                    const float* urow, const float* ucol, float* out) {
     __shared__ double ss[16];
     __shared__ int sc[16];
+    if (urow) {
+        __shared__ float red[16];
+        const float h = block_max(urow, R, red), w = block_max(ucol, V, red);
+        if (threadIdx.x == 0) { out[2] = 1.0f / h; out[3] = h; out[4] = 1.0f / w; out[5] = w; }
+    }
     double s = 0.0;
     int c = 0;
     for (int r = threadIdx.x; r < R; r += 1024) {
@@ -401,58 +432,66 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const
 }
 
 // ------------------------------------------------------------------------------------------------ operands
-constexpr int AMAX_WGS = 256;
-
-// largest magnitudes of hidden and weight, one value a workgroup: the first AMAX_WGS take one, the others the other
-__global__ __launch_bounds__(256) void amax_kernel(const float* h, long long ld_h, int R, const float* w, long long ld_w, int V, int C, float* part) {
-    const bool second = blockIdx.x >= AMAX_WGS;
-    const float* x = second ? w : h;
-    const long long ld = second ? ld_w : ld_h;
-    const int rows = second ? V : R, lane = threadIdx.x & 63, first = (blockIdx.x & (AMAX_WGS - 1)) * 4 + (threadIdx.x >> 6);
-    float m = 0.f;
-    if (ld % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && C % 4 == 0) {
-        for (int r = first; r < rows; r += AMAX_WGS * 4)
-#pragma unroll 4
-            for (int c = lane * 4; c < C; c += 256) {
-                const f32x4 v = *reinterpret_cast<const f32x4*>(x + r * ld + c);
-                m = fmaxf(fmaxf(m, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
-            }
-    } else {
-        for (int r = first; r < rows; r += AMAX_WGS * 4)
-            for (int c = lane; c < C; c += 64) m = fmaxf(m, fabsf(x[r * ld + c]));
-    }
-    __shared__ float red[4];
-    m = wave_max(m);
-    if (lane == 0) red[threadIdx.x >> 6] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-}
-
-// scales[0..3] = 2^s_h, 2^-s_h, 2^s_w, 2^-s_w, scales[4] = 2^-(s_h + s_w): powers of two that bring the largest magnitude to [2^13, 2^14]
-__global__ __launch_bounds__(256) void scales_kernel(const float* part, float* scales) {
-    __shared__ float red[2][4];
-    const int wave = threadIdx.x >> 6;
-    const float h = wave_max(part[threadIdx.x]), w = wave_max(part[AMAX_WGS + threadIdx.x]);
-    if ((threadIdx.x & 63) == 0) { red[0][wave] = h; red[1][wave] = w; }
-    __syncthreads();
-    if (threadIdx.x < 2) {
-        const float m = fmaxf(fmaxf(red[threadIdx.x][0], red[threadIdx.x][1]), fmaxf(red[threadIdx.x][2], red[threadIdx.x][3]));
-        int e = 0;
-        if (m > 0.f && m < INFINITY) e = 14 - min(max(ilogbf(m) + 1, -46), 74);     // 2^+-60: both factors and their product stay fp32 values
-        scales[2 * threadIdx.x] = ldexpf(1.0f, e);
-        scales[2 * threadIdx.x + 1] = ldexpf(1.0f, -e);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) scales[4] = scales[1] * scales[3];
+// 2^-s for values whose largest magnitude is m: 2^s brings it to [2^13, 2^14].  Within 2^+-60, so that factors and their product stay
+// fp32 values; nothing but zeros: the smallest factor, which no other row's exceeds.
+__device__ __forceinline__ float unscale_of(float m) {
+    if (!(m < INFINITY)) return 1.0f;                       // the row's result is not finite, whatever the scale
+    return m > 0.f ? ldexpf(1.0f, min(max(ilogbf(m) + 1, -46), 74) - 14) : ldexpf(1.0f, -60);
 }
 
 // One matrix [R][C] (rows ld apart) and the 16-bit planes wanted of it: rows [R][Cp] and / or transposed [C][Rp], zeros up to Cp and Rp
-// (multiples of 64)
+// (multiples of 64).  fp32: u the rows' factors 2^-s, scale the whole tensor's 2^s.  targets: rows left out are zeros.
 struct Turn {
-    const void* src; long long ld; int R, C, Rp, Cp, tiles_c; const float* scale;
+    const void* src; long long ld; int R, C, Rp, Cp, tiles_c;
+    float* u; const float* scale;
+    const long long* targets; int words; long long ignore;
     void *r0, *r1, *c0, *c1;
     int blocks;
 };
+__device__ __forceinline__ bool left_out(const Turn& p, int r) {
+    if (!p.targets) return false;
+    const long long t = p.targets[r];
+    return t < 0 || t >= p.words || t == p.ignore;
+}
+
+// fp32, forward: the rows of both matrices, each with its own scale; one wave a row
+__global__ __launch_bounds__(256) void rows_kernel(const Turn a, const Turn b) {
+    const int lane = threadIdx.x & 63;
+    int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const bool second = r >= a.R;
+    const Turn& p = second ? b : a;
+    if (second) r -= a.R;
+    if (r >= p.R) return;
+    const float* src = (const float*)p.src + (long long)r * p.ld;
+    const bool out = left_out(p, r), vec = p.ld % 4 == 0 && p.C % 4 == 0 && (reinterpret_cast<uintptr_t>(p.src) & 15) == 0;
+    auto at = [&](int c) __attribute__((always_inline)) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        if (out || c >= p.C) return x;
+        if (vec) return *reinterpret_cast<const f32x4*>(src + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < p.C) x[e] = src[c + e];
+        return x;
+    };
+    float m = 0.f;
+#pragma unroll 4
+    for (int c = lane * 4; c < p.C; c += 256) {
+        const f32x4 v = at(c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(v[e]));
+    }
+    const float u = unscale_of(wave_max(m)), f = 1.0f / u;
+    if (lane == 0) p.u[r] = u;
+#pragma unroll 4
+    for (int c = lane * 4; c < p.Cp; c += 256) {
+        const f32x4 v = at(c) * f;
+        _Float16 h[4], l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split<_Float16>(v[e], h[e], l[e]);
+        *reinterpret_cast<u32x2*>((_Float16*)p.r0 + (long long)r * p.Cp + c) = *reinterpret_cast<u32x2*>(h);
+        *reinterpret_cast<u32x2*>((_Float16*)p.r1 + (long long)r * p.Cp + c) = *reinterpret_cast<u32x2*>(l);
+    }
+}
 
 // a workgroup takes 64 x 64 values of one of two matrices: 16-byte loads and stores both ways, turned in LDS
 template <typename T, typename E>
@@ -471,10 +510,11 @@ __global__ __launch_bounds__(256) void planes_kernel(const Turn a, const Turn b)
         const int r = i / (64 / V), c = i % (64 / V) * V;
         T x[V];
         const T* q = src + (long long)(ry + r) * p.ld + cx + c;
-        if (vec && ry + r < p.R && cx + c + V <= p.C) *reinterpret_cast<u32x4*>(x) = *reinterpret_cast<const u32x4*>(q);
+        const bool in = ry + r < p.R && !left_out(p, ry + r);
+        if (vec && in && cx + c + V <= p.C) *reinterpret_cast<u32x4*>(x) = *reinterpret_cast<const u32x4*>(q);
         else {
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[e] = (ry + r < p.R && cx + c + e < p.C) ? q[e] : (T)0.f;
+            for (int e = 0; e < V; ++e) x[e] = (in && cx + c + e < p.C) ? q[e] : (T)0.f;
         }
         E h[V], l[V];
 #pragma unroll
@@ -487,6 +527,9 @@ __global__ __launch_bounds__(256) void planes_kernel(const Turn a, const Turn b)
         if (p.r0 && ry + r < p.R) {
             const long long at = (long long)(ry + r) * p.Cp + cx + c;
             if constexpr (sizeof(T) == 4) {
+                const float fr = 1.0f / p.u[ry + r];
+#pragma unroll
+                for (int e = 0; e < V; ++e) split<E>((float)x[e] * fr, h[e], l[e]);
                 *reinterpret_cast<u32x2*>((E*)p.r0 + at) = *reinterpret_cast<u32x2*>(h);
                 *reinterpret_cast<u32x2*>((E*)p.r1 + at) = *reinterpret_cast<u32x2*>(l);
             } else *reinterpret_cast<u32x4*>((E*)p.r0 + at) = *reinterpret_cast<u32x4*>(h);
@@ -636,8 +679,8 @@ Operand<T> room(Space& ws, const void* x, long long ld, int R, int C, bool want_
 }
 
 template <typename T>
-Turn turn_of(const Operand<T>& o, const void* x, long long ld, int R, int C, bool is_direct, const float* scale) {
-    Turn t{x, ld, R, C, (int)up(R, 64), (int)up(C, 64), (int)(up(C, 64) / 64), scale, is_direct ? nullptr : (void*)o.row0, o.row1, o.col0, o.col1, 0};
+Turn turn_of(const Operand<T>& o, const void* x, long long ld, int R, int C, bool is_direct, float* u, const float* scale) {
+    Turn t{x, ld, R, C, (int)up(R, 64), (int)up(C, 64), (int)(up(C, 64) / 64), u, scale, nullptr, 0, 0, is_direct ? nullptr : (void*)o.row0, o.row1, o.col0, o.col1, 0};
     if (!is_direct || o.col0) t.blocks = (int)(up(R, 64) / 64) * t.tiles_c;
     return t;
 }
@@ -646,7 +689,6 @@ template <typename T>
 struct Plan {
     bool dh_direct, dw_direct;
     Operand<T> h, w;
-    float* amax;
     // forward
     float2* part; float* target_logit; int strips;
     // backward
@@ -665,7 +707,6 @@ struct Plan {
         h = room<T>(ws, c.h, c.ld_h, c.R, c.E, backward, dh_direct);
         w = room<T>(ws, c.w, c.ld_w, c.V, c.E, backward, dw_direct);
         const int pairs = Of<T>::planes == 2 ? 3 : 1;
-        amax = ws.take<float>(Of<T>::planes == 2 && !backward ? 2 * AMAX_WGS : 0);
         if (!backward) {
             s_logit = shape_of(c.R, c.V, up(c.E, 64) / 64 * pairs, false);
             strips = (int)(up(c.V, STRIP) / STRIP);
@@ -695,24 +736,25 @@ struct Plan {
     }
 };
 
-// scales: five floats, written by the forward call (fp32 tensors) and read by the backward one
+// The forward call's results: loss, scale of a row, and of fp32 tensors (for the backward call) the tensors' scales 2^s_h, 2^-s_h, 2^s_w,
+// 2^-s_w, and from OUT_ROWS on the factors 2^-s of every row of hidden, then of every word (read up to 256 behind the last)
+constexpr int OUT_ROWS = 8;
+inline long long out_floats(int dtype, int R, int V) { return OUT_ROWS + (dtype == DT_F32 ? up(R, 64) + up(V, 64) + 256 : 0); }
+
 template <typename T>
-void operands(const Call& c, Plan<T>& p, float* scales, bool backward, hipStream_t st) {
-    const float *sh = nullptr, *sw = nullptr;
-    if constexpr (sizeof(T) == 4) {
-        if (!backward) {
-            hipLaunchKernelGGL(amax_kernel, dim3(2 * AMAX_WGS), dim3(256), 0, st, (const float*)c.h, c.ld_h, c.R, (const float*)c.w, c.ld_w, c.V, c.E, p.amax);
-            hipLaunchKernelGGL(scales_kernel, dim3(1), dim3(256), 0, st, p.amax, scales);
-        }
-        sh = scales;
-        sw = scales + 2;
-    }
-    const Turn a = turn_of<T>(p.h, c.h, c.ld_h, c.R, c.E, p.dh_direct, sh), b = turn_of<T>(p.w, c.w, c.ld_w, c.V, c.E, p.dw_direct, sw);
-    if (a.blocks + b.blocks > 0) hipLaunchKernelGGL((planes_kernel<T, typename Of<T>::E>), dim3(a.blocks + b.blocks), dim3(256), 0, st, a, b);
+void operands(const Call& c, Plan<T>& p, float* out, bool backward, hipStream_t st) {
+    float *uh = nullptr, *uw = nullptr;
+    if constexpr (sizeof(T) == 4) { uh = out + OUT_ROWS; uw = uh + up(c.R, 64); }
+    Turn a = turn_of<T>(p.h, c.h, c.ld_h, c.R, c.E, p.dh_direct, uh, uh ? out + 2 : nullptr), b = turn_of<T>(p.w, c.w, c.ld_w, c.V, c.E, p.dw_direct, uw, uw ? out + 4 : nullptr);
+    a.targets = c.targets;
+    a.words = c.V;
+    a.ignore = c.ignore;
+    if (sizeof(T) == 4 && !backward) hipLaunchKernelGGL(rows_kernel, dim3((unsigned)(((long long)c.R + c.V + 3) / 4)), dim3(256), 0, st, a, b);
+    else if (a.blocks + b.blocks > 0) hipLaunchKernelGGL((planes_kernel<T, typename Of<T>::E>), dim3(a.blocks + b.blocks), dim3(256), 0, st, a, b);
 }
 
 template <typename T>
-Gemm logits(const Call& c, const Plan<T>& p, const float* scales, int v0, int vn) {
+Gemm logits(const Call& c, const Plan<T>& p, const float* out, int v0, int vn) {
     Gemm g{};
     g.a0 = (const unsigned short*)p.h.row0;
     g.a1 = (const unsigned short*)p.h.row1;
@@ -722,7 +764,7 @@ Gemm logits(const Call& c, const Plan<T>& p, const float* scales, int v0, int vn
     g.ldb = p.w.ld;
     g.M = c.R; g.N = vn; g.K = (int)up(c.E, 64);
     g.pairs = Of<T>::planes == 2 ? 3 : 1;
-    g.unscale = sizeof(T) == 4 ? scales + 4 : nullptr;
+    if (sizeof(T) == 4) { g.urow = out + OUT_ROWS; g.ucol = g.urow + up(c.R, 64) + v0; }
     g.bias = c.bias; g.targets = c.targets; g.ignore = c.ignore; g.V = c.V; g.v0 = v0;
     return g;
 }
@@ -731,12 +773,12 @@ template <typename T>
 int fwd(const Call& c, int mean_over_valid, float* row_loss, float* row_lse, float* out, char* ws, hipStream_t st) {
     typedef typename Of<T>::E E;
     Plan<T> p(c, false, ws);
-    operands<T>(c, p, out + 2, false, st);
-    Gemm g = logits<T>(c, p, out + 2, 0, c.V);
+    operands<T>(c, p, out, false, st);
+    Gemm g = logits<T>(c, p, out, 0, c.V);
     g.part = p.part; g.strips = p.strips; g.target_logit = p.target_logit;
     if (int rc = gemm<E, T, EP_LSE>(g, p.s_logit, st)) return rc;
     hipLaunchKernelGGL(lse_kernel, dim3((c.R + 3) / 4), dim3(256), 0, st, p.part, p.strips, p.target_logit, c.targets, c.R, c.V, c.ignore, row_loss, row_lse);
-    hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, c.targets, c.R, c.V, c.ignore, mean_over_valid, out);
+    hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, c.targets, c.R, c.V, c.ignore, mean_over_valid, g.urow, g.ucol, out);
     return launch_status("linear_ce_fwd");
 }
 
@@ -744,12 +786,11 @@ template <typename T>
 int bwd(const Call& c, const float* row_lse, const float* meta, const float* grad_out, void* dh, void* dw, void* db, char* ws, hipStream_t st) {
     typedef typename Of<T>::E E;
     Plan<T> p(c, true, ws);
-    float* scales = const_cast<float*>(meta) + 2;
-    operands<T>(c, p, scales, true, st);
+    operands<T>(c, p, const_cast<float*>(meta), true, st);         // which only reads it here
     const float back = __is_same(E, _Float16) ? 1.0f / D_SCALE : 1.0f;
     for (int v0 = 0; v0 < c.V; v0 += p.piece) {
         const int vn = c.V - v0 < p.piece ? c.V - v0 : p.piece;
-        Gemm g = logits<T>(c, p, scales, v0, vn);
+        Gemm g = logits<T>(c, p, meta, v0, vn);
         g.lse = row_lse;
         g.d0 = (unsigned short*)p.d0; g.d1 = (unsigned short*)p.d1; g.t0 = (unsigned short*)p.t0; g.t1 = (unsigned short*)p.t1;
         g.ldd = p.ldd; g.ldt = p.ldt;
@@ -763,7 +804,7 @@ int bwd(const Call& c, const float* row_lse, const float* meta, const float* gra
             q.lda = p.ldd; q.ldb = p.w.ldc;
             q.M = c.R; q.N = c.E; q.K = (int)up(vn, 64);
             q.pairs = g.pairs;
-            q.f0 = grad_out; q.f1 = meta + 1; q.f2 = sizeof(T) == 4 ? scales + 3 : nullptr; q.f = back;
+            q.f0 = grad_out; q.f1 = meta + 1; q.f2 = sizeof(T) == 4 ? meta + 5 : nullptr; q.f = back;
             const bool whole = p.s_h.splits == 1 && p.piece >= c.V;
             if (whole) { q.out = dh; q.ldo = c.E; }
             else { q.acc = p.acc_h; q.accumulate = v0 > 0; }
@@ -781,7 +822,7 @@ int bwd(const Call& c, const float* row_lse, const float* meta, const float* gra
             q.lda = p.ldt; q.ldb = p.h.ldc;
             q.M = vn; q.N = c.E; q.K = (int)up(c.R, 64);
             q.pairs = g.pairs;
-            q.f0 = grad_out; q.f1 = meta + 1; q.f2 = sizeof(T) == 4 ? scales + 1 : nullptr; q.f = back;
+            q.f0 = grad_out; q.f1 = meta + 1; q.f2 = sizeof(T) == 4 ? meta + 3 : nullptr; q.f = back;
             T* dst = (T*)dw + (long long)v0 * c.E;
             if (p.s_w.splits == 1) { q.out = dst; q.ldo = c.E; }
             else q.acc = p.acc_w;
@@ -821,13 +862,15 @@ long long linear_ce_ws_bytes(int dtype, int R, int E, int V, int backward) {
     return lce::Plan<_Float16>(c, backward, nullptr).bytes;
 }
 
+long long linear_ce_out_floats(int dtype, int R, int V) { return R <= 0 || V <= 0 ? 0 : lce::out_floats(dtype, R, V); }
+
 int linear_ce_fwd(int dtype, const void* h, long long ld_h, const void* w, long long ld_w, const void* bias, const long long* targets, int R, int E,
                   int V, long long ignore, int mean_over_valid, float* row_loss, float* row_lse, float* out, void* ws, long long ws_bytes,
                   hipStream_t st) {
     const lce::Call c{h, w, bias, ld_h, ld_w, targets, R, E, V, ignore};
     if (int rc = lce::check(dtype, c, "linear_ce_fwd")) return rc;
-    if (!row_loss || !row_lse || !out || !ws || !aligned16(ws) || ws_bytes < linear_ce_ws_bytes(dtype, R, E, V, 0)) {
-        set_error("linear_ce_fwd: null result, or a workspace that is null, unaligned or too small");
+    if (!row_loss || !row_lse || !out || !aligned16(out) || !ws || !aligned16(ws) || ws_bytes < linear_ce_ws_bytes(dtype, R, E, V, 0)) {
+        set_error("linear_ce_fwd: null result, results or a workspace that are unaligned, or a workspace that is null or too small");
         return ICAP_ERR_ARG;
     }
     if (dtype == DT_F32) return lce::fwd<float>(c, mean_over_valid, row_loss, row_lse, out, (char*)ws, st);
@@ -840,7 +883,7 @@ int linear_ce_bwd(int dtype, const void* h, long long ld_h, const void* w, long 
                   long long ws_bytes, hipStream_t st) {
     const lce::Call c{h, w, bias, ld_h, ld_w, targets, R, E, V, ignore};
     if (int rc = lce::check(dtype, c, "linear_ce_bwd")) return rc;
-    if (!row_lse || !meta || !grad_out || !ws || !aligned16(ws) || ws_bytes < linear_ce_ws_bytes(dtype, R, E, V, 1)) {
+    if (!row_lse || !meta || !aligned16(meta) || !grad_out || !ws || !aligned16(ws) || ws_bytes < linear_ce_ws_bytes(dtype, R, E, V, 1)) {
         set_error("linear_ce_bwd: null tensor, or a workspace that is null, unaligned or too small");
         return ICAP_ERR_ARG;
     }

@@ -498,7 +498,7 @@ def linear_ce_fwd(hidden, weight, bias, targets, ignore_index=-100, mean_over_va
         raise N.IcapError("linear_ce: targets must be contiguous")
     lib, dev, code = N.load(), hidden.device, DTYPE_CODES[hidden.dtype]
     rows = torch.empty((2, R), device=dev, dtype=torch.float32)
-    out = torch.empty(8, device=dev, dtype=torch.float32)
+    out = torch.empty(lib.icap_linear_ce_out_floats(code, R, V), device=dev, dtype=torch.float32)
     nbytes = lib.icap_linear_ce_ws_bytes(code, R, E, V, 0)
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
     span = _Span("linear_ce_fwd", (R, E, V, str(hidden.dtype)))

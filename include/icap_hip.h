@@ -856,14 +856,16 @@ int icap_attention_packed_bwd(int dtype, const void* dout, const void* q, const 
                               long long v_head, float scale, int causal, float* ws, void* stream);
 
 /* Cross entropy of a Linear layer without its logits in memory: x = hidden weight^T + bias, loss_r = log sum_v exp x_rv -
- * x_r,target (0 for ignored rows: target == ignore_index or outside [0, vocab)); hidden [rows][width] (rows ld_h apart), weight
- * [vocab][width] (ld_w), bias [vocab] or NULL, all of one type.  out [8] fp32: out[0] = loss, out[1] = the scale every row was
- * weighted with, as in icap_ce_loss_fwd_f32 (mean_over_valid likewise), the others are for the backward call; row_loss, row_lse
- * [rows] fp32.
+ * x_r,target (0 for ignored rows: target == ignore_index or outside [0, vocab), whose hidden rows may hold anything); hidden
+ * [rows][width] (rows ld_h apart), weight [vocab][width] (ld_w), bias [vocab] or NULL, all of one type.  out: fp32, 16-byte aligned,
+ * icap_linear_ce_out_floats(dtype, rows, vocab) values: out[0] = loss, out[1] = the scale every row was weighted with, as in
+ * icap_ce_loss_fwd_f32 (mean_over_valid likewise), the others are for the backward call; row_loss, row_lse [rows] fp32.
  * Backward: gradients of grad_out[0] (device scalar) * loss in the tensors' type, dense: dhidden [rows][width], dweight
- * [vocab][width], dbias [vocab]; each may be NULL.  fp32 products are fp32-accurate; magnitudes of fp32 hidden and weight below 2^74.
+ * [vocab][width], dbias [vocab]; each may be NULL.  fp32 products are fp32-accurate (a gradient to 2^-38 of the largest magnitude of
+ * weight and hidden, too); magnitudes of fp32 hidden and weight below 2^74.
  * ws: icap_linear_ce_ws_bytes(dtype, rows, width, vocab, backward) bytes, 16-byte aligned: bounded by about
  * 512 MB, fp32 partial results and copies of hidden and weight, whatever the vocabulary. */
+long long icap_linear_ce_out_floats(int dtype, int rows, int vocab);
 long long icap_linear_ce_ws_bytes(int dtype, int rows, int width, int vocab, int backward);
 int icap_linear_ce_fwd(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
                        const long long* targets, int rows, int width, int vocab, long long ignore_index, int mean_over_valid,

@@ -343,6 +343,41 @@ def test_linear_ce_sizes(dtype, R, E, V):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, 1e30])
+@pytest.mark.parametrize("E", [64, 40])
+def test_linear_ce_left_out_rows_may_hold_anything(dtype, bad, E):
+    from image_captioning_amd import train_ops as T
+    R, V = 90, 200
+    h, w, b = rnd(R, E, seed=1, dtype=dtype), rnd(V, E, seed=2, scale=0.2, dtype=dtype), rnd(V, seed=3, dtype=dtype)
+    t = torch.randint(0, V, (R,), generator=torch.Generator().manual_seed(4))
+    t[::7], t[3], t[4] = 0, V, -5
+    want = ce_oracle(h, w, b, t, 0, True, 2.0)
+    h[::7], h[3], h[4] = bad, bad, bad
+    h[t == 0] = bad
+    value, row, saved = T.linear_ce_fwd(h.to(D), w.to(D), b.to(D), t.to(D), 0, True)
+    dh, dw, db = T.linear_ce_bwd(torch.tensor([2.0], device=D), saved)
+    for n, x in (("loss", value), ("row_loss", row), ("dh", dh), ("dw", dw), ("db", db)):
+        within(x, *want[n], n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, 1e9])
+def test_linear_ce_rows_do_not_touch_each_other(dtype, bad):
+    """A row that counts and holds NaN, infinities or huge values: the losses of the others, and their rows of dhidden, are the formula's."""
+    from image_captioning_amd import train_ops as T
+    R, E, V = 70, 64, 150
+    h, w = rnd(R, E, seed=1, dtype=dtype), rnd(V, E, seed=2, scale=0.2, dtype=dtype)
+    t = torch.randint(0, V, (R,), generator=torch.Generator().manual_seed(4))
+    want = ce_oracle(h, w, None, t, -100, False, 1.0)
+    h[33] = bad
+    _, row, saved = T.linear_ce_fwd(h.to(D), w.to(D), None, t.to(D), -100, False)
+    dh, _, _ = T.linear_ce_bwd(torch.tensor([1.0], device=D), saved)
+    others = torch.arange(R) != 33
+    for n, x in (("row_loss", row), ("dh", dh)):
+        within(x.cpu()[others], want[n][0][others], want[n][1][others], n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_linear_ce_large_tiles_and_split_contraction(dtype):
     """Enough rows and words for the 256 x 256 tiles, few enough columns that dh and dw split their contraction."""
     compare_ce(dtype, 3300, 64, 4100, g=512.0 if dtype == F16 else 1.0, seed=3)
