@@ -1069,7 +1069,8 @@ def attention_packed(q, k, v, cu_q, cu_k=None, causal=True, scale=None, want_lse
     axis contiguous, e.g. slices of one projection), cu_q, cu_k int32 [sequences + 1] on the device: sequence b owns rows
     cu[b] .. cu[b + 1] (cu_k None: the same).  The offsets start at 0 and do not decrease; they stay on the device, unread by the host.
     causal: query i of n_q sees keys 0 .. i + n_k - n_q, so a single new token (n_q = 1) sees its whole cache.
-    A row that sees no key, and every row behind the last sequence, gives zeros.  v must be finite, scale (None: dim ** -0.5) positive.
+    A row that sees no key, and every row behind the last sequence, gives zeros; NaN or infinities reach the rows that see them alone.
+    scale (None: dim ** -0.5) must be positive.
     Returns out [tokens_q, heads, dim], and with want_lse also log sum exp(scale q k) [tokens_q, heads] in fp32."""
     cu_k = _packed_args(q, k, v, cu_q, cu_k, "attention_packed")
     q, k, v = _packed_rows(q), _packed_rows(k), _packed_rows(v)

@@ -7,6 +7,7 @@ operation runs in ``libicap_hip.so``.
 from __future__ import annotations
 
 from array import array
+from itertools import chain
 from operator import attrgetter
 
 import torch
@@ -483,7 +484,7 @@ def linear_ce_fwd(hidden, weight, bias, targets, ignore_index=-100, mean_over_va
     """Cross entropy of hidden @ weight.T + bias over its columns without the [rows, vocab] logits in memory.
 
     hidden [rows, width], weight [vocab, width], bias [vocab] or None, all fp32, bf16 or fp16 (rows may be strided); targets int64
-    [rows].  A target that is ignore_index or outside the vocabulary is left out.  mean_over_valid: the mean over the rows that count
+    [rows].  A target that is ignore_index or outside the vocabulary leaves its row out, whatever the row holds.  mean_over_valid: the mean over the rows that count
     (training.CrossEntropyLoss); otherwise over all rows (training.compute_loss).
     Returns (loss - a device scalar -, row_loss [rows] fp32, what linear_ce_bwd needs or None)."""
     ld_h = _ce_rows(hidden, "linear_ce: hidden")
@@ -574,7 +575,7 @@ def adamw_tensors(params, grads, exp_avg, exp_avg_sq, step, lr, beta1=0.9, beta2
     and the place, so a step can be repeated).  All states are of one kind.
     step: from 1, one for all or a list; step_dev: int32 [1] on the device, added to step by the kernel (a step recorded in a HIP
     graph: step = 0 and the count kept there).  index: the tensors' numbers for the generator (their places in the list).
-    No tensor may appear twice.  A gradient that is not finite spoils its value's states, with 8 bits its block's."""
+    No parameter or state may appear twice.  A gradient that is not finite spoils its value's states, with 8 bits its block's."""
     n = len(params)
     if not (len(grads) == len(exp_avg) == len(exp_avg_sq) == n):
         raise N.IcapError("adamw_tensors: as many gradients and states as parameters are wanted")
@@ -609,8 +610,11 @@ def adamw_tensors(params, grads, exp_avg, exp_avg_sq, step, lr, beta1=0.9, beta2
         right = True
     if not right or list(map(torch.Tensor.numel, m)) != sizes or list(map(torch.Tensor.numel, v)) != sizes:
         raise N.IcapError("adamw_tensors: a state has another size than its parameter")
-    if len(set(p_ptr)) < len(p_ptr) and len({a for a, k in zip(p_ptr, sizes) if k}) < sum(k > 0 for k in sizes):
-        raise N.IcapError("adamw_tensors: a parameter appears twice")
+    written = [p_ptr, *state]
+    if len(set(chain(*written))) < len(written) * len(params):          # empty tensors share an address
+        used = [a for x in written for a, k in zip(x, sizes) if k]
+        if len(set(used)) < len(used):
+            raise N.IcapError("adamw_tensors: a parameter or a state appears twice")
     columns = [p_ptr, g_ptr, *state, sizes, steps, index]
     if len(p_kinds) == 1 and len(g_kinds) == 1:
         groups = {(*p_kinds, *g_kinds): columns}

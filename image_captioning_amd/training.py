@@ -327,7 +327,7 @@ class AdamWTensors:
 
     def _launch(self, steps, step_dev=None):
         from . import train_ops as T
-        T.adamw_tensors([p.detach() for p in self.params], [p.grad for p in self.params], self.m, self.v, step=steps, lr=self.lr, beta1=self.betas[0],
+        T.adamw_tensors(self.params, [p.grad for p in self.params], self.m, self.v, step=steps, lr=self.lr, beta1=self.betas[0],
                         beta2=self.betas[1], eps=self.eps, weight_decay=self.weight_decay, grad_scale=self.grad_scale, seed=self.seed,
                         step_dev=step_dev)
 

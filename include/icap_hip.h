@@ -841,7 +841,7 @@ long long icap_conv_wgrad_gather_ws_floats(int B, int Ho, int Wo, int Cout, int 
  * sees no key gives zeros and a log-sum of -inf.  Rows behind the last sequence give zeros.
  * out dense [tokens_q][heads][dim]; lse (may be NULL) [tokens_q][heads] = log sum exp(scale q k).  Strides of q, k, v (and dout)
  * in elements, the last axis contiguous; scale > 0; dim % 8 == 0, dim <= 128; pointers 16-byte aligned and strides multiples of 16 bytes
- * (error 2 otherwise).  Values of v must be finite (a hidden key's weight is 0, and 0 times infinity is not).
+ * (error 2 otherwise).  Rows do not touch what they do not see: NaN or infinities of another sequence, or of later keys, stay there.
  * ws: icap_attention_packed_ws_bytes(...) bytes, 16-byte aligned (0: none).
  * Backward: out, lse as the forward call gave them; dq, dk, dv dense in the shapes of q, k, v; ws: tokens_q * heads floats. */
 long long icap_attention_packed_ws_bytes(int seqs, int tokens_q, int tokens_k, int heads, int kv_heads, int dim);

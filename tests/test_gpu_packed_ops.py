@@ -608,6 +608,12 @@ def test_adamw_tensors_refusals_on_the_device():
             T.adamw_tensors(**bad, step=1, lr=1e-3)
     with pytest.raises(N.IcapError):
         T.adamw_tensors([p], [g], [m], [v], step=0, lr=1e-3)
+    p2, m2, v2, t8 = torch.zeros_like(p), torch.zeros_like(p), torch.zeros_like(p), T.adamw_state8(p)
+    for states in (([m, m], [v, v2]), ([m, m2], [v, m]), ([m, p], [v, v2]), ([s8, T.adamw_state8(p)], [t8, s8])):
+        with pytest.raises(N.IcapError, match="twice"):
+            T.adamw_tensors([p, p2], [g, g], *states, step=1, lr=1e-3)
+    e, e2 = torch.zeros(0, device=D), torch.zeros(0, device=D)
+    T.adamw_tensors([p, e, e2], [g, e, e2], [m, e, e2], [v, e, e2], step=1, lr=1e-3)          # empty tensors share an address
     assert not p.any()
 
 
