@@ -153,8 +153,8 @@ __device__ __forceinline__ typename Vec<T>::x8 col_frag(const T* lds, int row0, 
     }
 }
 
-// eight registers of an accumulator (16 of its rows) as an operand: the one rounding of P and dS to a 16-bit type (2^-9 / 2^-12 of
-// each value, as much as the result's own rounding; the sums beside them are taken from the unrounded values)
+// eight registers of an accumulator (16 of its rows) as an operand: the one rounding of P to a 16-bit type (2^-9 / 2^-12 of
+// each value, as much as the result's own rounding; the sum of P itself is taken from the unrounded values)
 template <typename T>
 __device__ __forceinline__ typename Vec<T>::x8 acc_frag(const f32x16& a, int half) {
     f32x8 x;
@@ -162,6 +162,26 @@ __device__ __forceinline__ typename Vec<T>::x8 acc_frag(const f32x16& a, int hal
     for (int e = 0; e < 8; ++e) x[e] = a[half * 8 + e];
     if constexpr (sizeof(T) == 4) return x;
     else return __builtin_convertvector(x, typename Vec<T>::x8);
+}
+
+// dS in two parts, high and low (16-bit types; 16 bits and more of each value): its terms differ in sign, so that one rounded part made
+// dQ and dK 1.53 times as far off as rounding the exact results does; two: 1.17 times, the rest from O's own rounding in delta.  The
+// second product costs 8 % of a training pass (222 -> 241 us, 8 bf16 sequences of up to 2048 tokens, dim 64) to 19 % (dim 128).
+template <typename T>
+__device__ __forceinline__ void acc_parts(const f32x16& a, int half, typename Vec<T>::x8& hi, typename Vec<T>::x8& lo) {
+    f32x8 x, y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        x[e] = a[half * 8 + e];
+        if constexpr (__is_same(T, __bf16)) y[e] = __uint_as_float(__float_as_uint(x[e]) & 0xffff0000u);
+    }
+    if constexpr (__is_same(T, __bf16)) {
+        hi = __builtin_convertvector(y, typename Vec<T>::x8);
+    } else {
+        hi = __builtin_convertvector(x, typename Vec<T>::x8);
+        y = __builtin_convertvector(hi, f32x8);
+    }
+    lo = __builtin_convertvector(x - y, typename Vec<T>::x8);
 }
 
 // fragment of a row in memory: columns 16 kk + 8 (lane / 32) .. + 7, zeros from dim on and when !ok (p stays readable)
@@ -596,9 +616,19 @@ __global__ __launch_bounds__(RW * KG * 64, DP == 128 && (RW < 4 || sizeof(T) == 
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const auto df = acc_frag<T>(s, j);
+                if constexpr (sizeof(T) == 4) {
+                    const auto df = acc_frag<T>(s, j);
 #pragma unroll
-                for (int d = 0; d < ND; ++d) dq[d] = mma32(col_frag<T, DP>(sk[buf], kt * 32 + j * 16, d * 32), df, dq[d]);
+                    for (int d = 0; d < ND; ++d) dq[d] = mma32(col_frag<T, DP>(sk[buf], kt * 32 + j * 16, d * 32), df, dq[d]);
+                } else {
+                    typename Vec<T>::x8 hi, lo;
+                    acc_parts<T>(s, j, hi, lo);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        const auto kf = col_frag<T, DP>(sk[buf], kt * 32 + j * 16, d * 32);
+                        dq[d] = mma32(kf, lo, mma32(kf, hi, dq[d]));
+                    }
+                }
             }
         }
     }
@@ -700,11 +730,16 @@ __global__ __launch_bounds__(KW * RG * 64, DP == 128 ? 1 : 2) void dkv_kernel(co
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const auto pf = acc_frag<T>(s, j), df = acc_frag<T>(dp, j);
+            const auto pf = acc_frag<T>(s, j);
+            typename Vec<T>::x8 hi, lo;
+            if constexpr (sizeof(T) == 4) hi = acc_frag<T>(dp, j);
+            else acc_parts<T>(dp, j, hi, lo);
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 dv[d] = mma32(col_frag<T, DP>(sg[buf], mine + j * 16, d * 32), pf, dv[d]);
-                dk[d] = mma32(col_frag<T, DP>(sq[buf], mine + j * 16, d * 32), df, dk[d]);
+                const auto qt = col_frag<T, DP>(sq[buf], mine + j * 16, d * 32);
+                dk[d] = mma32(qt, hi, dk[d]);
+                if constexpr (sizeof(T) == 2) dk[d] = mma32(qt, lo, dk[d]);
             }
         }
     }
