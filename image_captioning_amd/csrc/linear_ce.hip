@@ -3,11 +3,12 @@
 //   D = softmax(x) - onehot(target) (zero rows where ignored),  dh = g D W,  dW = g D^T h,  db = g sum_r D,  g = grad_out scale
 // Forward: one GEMM whose epilogue keeps, of every 64-column strip of a row, only its maximum and its sum of exponentials
 // (8 bytes for 64 logits) and the target's logit; a second launch joins the strips.
-// Backward: the vocabulary in pieces.  The logits of a piece are formed again, turned into D in the epilogue (16 bits, row-major
-// and transposed), and multiplied while the cache still holds them; dh collects the pieces in fp32.  The bias gradient is summed
-// from the unrounded D.  Every sum has a fixed order.
-// All products are one GEMM kernel: C[m][n] = sum_k A[m][k] B[n][k] on the 16-bit matrix cores, fp32 accumulation, operands with
-// contiguous k (dh and dW take W, h and D transposed: W and h are turned once a call, D is written both ways).
+// Backward: the vocabulary in pieces.  The logits of a piece are formed again, turned into D in the epilogue (16 bits), and multiplied
+// while the cache still holds them; dh collects the pieces in fp32.  The bias gradient is summed from the unrounded D.  Every
+// sum has a fixed order.
+// All products are one GEMM kernel: C[m][n] = sum_k A[m][k] B[n][k] on the 16-bit matrix cores, fp32 accumulation.  An operand's k is
+// contiguous (x), or its rows are k (W in dh, D and h in dW): those tiles pass the LDS's transposing read on their way to the matrix cores, and
+// nothing is transposed in memory.
 //   bf16: D is rounded to bf16 (2^-9 of each value, as much as the result's own rounding).
 //   fp16: D 2^14 is rounded to fp16, so that a probability of 1e-8 still has full precision; the factor leaves again exactly.
 //   fp32: every operand is the sum of two fp16 values (22 bits), scaled by a power of two so that its largest magnitude is near
@@ -33,6 +34,7 @@ struct Gemm {
     const unsigned short *a0, *a1, *b0, *b1;        // planes: high and (fp32 tensors) low parts
     long long lda, ldb;
     int M, N, K, pairs, ksplit, tiles_m, tiles_n;   // K % 64 == 0; pairs 1 or 3
+    int a_cols, b_cols;                             // operands whose rows are k (K of them): columns there are (% 8 == 0)
     const float *urow, *ucol;                       // fp32: factors 2^-s of the logits' rows and columns
     // EP_LSE and EP_GRAD
     const void* bias;                               // type of the tensors
@@ -41,8 +43,8 @@ struct Gemm {
     int V, v0;                                      // column 0 of this product is word v0; words end at V
     float2* part; int strips; float* target_logit;  // EP_LSE
     const float* lse;                               // EP_GRAD
-    unsigned short *d0, *d1, *t0, *t1;              // D [M][ldd] and D^T [N][ldt], planes
-    long long ldd, ldt;
+    unsigned short *d0, *d1;                        // D [rows_pad][ldd], planes
+    long long ldd;
     int rows_pad, cols_pad;                         // D is written (zeros) up to these multiples of 64
     float* colpart; long long ldc;                  // [row blocks][ldc]
     // EP_OUT
@@ -94,7 +96,11 @@ template <int BM, int BN, int ST> constexpr int smem_bytes() { return ST * (BM +
 // WM x WN waves, each (BM / WM) x 64 of the tile.  Operands go global -> LDS without passing a register (16 bytes a lane, one wave
 // 1 KB); ST - 1 K tiles are in flight while one multiplies; one wait and one barrier a K tile.  The 16-byte slot a lane
 // fetches is permuted by its row, and the fragment reads apply the same permutation, so that 16 rows meet 16 different slots.
-template <typename E, typename T, int BM, int BN, int WM, int WN, int ST, int EP>
+// AT, BT: the operand's rows are k.  Its tile is [64][BM]; a transposing read takes 64 bytes of four rows, which the permutation puts into
+// different quarters of the LDS's 256-byte line.
+template <int COLS> __device__ __forceinline__ int quarter(int k) { return COLS >= 128 ? (k & 3) << 2 : (k & 2) << 1; }
+
+template <typename E, typename T, int BM, int BN, int WM, int WN, int ST, int EP, bool AT, bool BT>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
     constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, RM = TM / 32, RN = 2, RPP = NW * 8;
     static_assert(TN == STRIP && TM % 32 == 0 && BM % RPP == 0 && BN % RPP == 0, "wave tiles");
@@ -104,25 +110,34 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave - wm * WN, lr = lane & 31, lh = lane >> 5;
 
-    // each XCD (workgroups go round them) walks a contiguous range of tiles, in which neighbours share their B panel
+    // each XCD (workgroups go round them) walks a contiguous range of tiles, four rows of tiles at a time: the 32 tiles of 256 x 256 that it
+    // works on share 4 + 8 panels (with one column of all rows, 1 + 32, the last-level cache bound the long products: 4864 rows x 6756 words
+    // of fp32 610 -> 587 us, 8192 x 65536 of bf16 8600 -> 8280)
+    constexpr int GROUP = 4;
     const int nwg = gridDim.x, xcd = blockIdx.x & 7, slot = blockIdx.x >> 3, tq = nwg >> 3, tr = nwg & 7;
     const int tlin = xcd * tq + (xcd < tr ? xcd : tr) + slot;
-    const int tile_n = tlin / p.tiles_m, tile_m = tlin - tile_n * p.tiles_m;
+    const int group = tlin / (GROUP * p.tiles_n), in = tlin - group * (GROUP * p.tiles_n), gm = min(p.tiles_m - group * GROUP, GROUP);
+    const int tile_n = in / gm, tile_m = group * GROUP + in - tile_n * gm;
     const int m0 = tile_m * BM, n0 = tile_n * BN;
 
     const int srow = wave * 8 + (lane >> 3), lslot = (lane & 7) ^ ((wave * 4 + (lane >> 4)) & 7);
+    // rows of k: a wave fetches 512 / BM of them at a time
+    constexpr int ALR = BM / 8, BLR = BN / 8, AK = 64 / ALR, BKR = 64 / BLR;
+    const int ak = wave * AK + lane / ALR, bk = wave * BKR + lane / BLR;        // + i NW AK: four rows' quarters are the same for every i
+    static_assert(NW * AK % 4 == 0 && NW * BKR % 4 == 0, "permutation of the rows of k");
+    const int acol = min(m0 + ((lane % ALR) ^ quarter<BM>(ak)) * 8, p.a_cols - 8), bcol = min(n0 + ((lane % BLR) ^ quarter<BN>(bk)) * 8, p.b_cols - 8);
     long long a_off[APT], b_off[BPT];
 #pragma unroll
-    for (int i = 0; i < APT; ++i) a_off[i] = (long long)min(m0 + i * RPP + srow, p.M - 1) * p.lda + 8 * lslot;
+    for (int i = 0; i < APT; ++i) a_off[i] = AT ? (long long)(ak + i * NW * AK) * p.lda + acol : (long long)min(m0 + i * RPP + srow, p.M - 1) * p.lda + 8 * lslot;
 #pragma unroll
-    for (int i = 0; i < BPT; ++i) b_off[i] = (long long)min(n0 + i * RPP + srow, p.N - 1) * p.ldb + 8 * lslot;
+    for (int i = 0; i < BPT; ++i) b_off[i] = BT ? (long long)(bk + i * NW * BKR) * p.ldb + bcol : (long long)min(n0 + i * RPP + srow, p.N - 1) * p.ldb + 8 * lslot;
     const int nk = p.K / BK, total = nk * p.pairs;
     const int per = (total + p.ksplit - 1) / p.ksplit, t_lo = min((int)blockIdx.y * per, total), t_hi = min(t_lo + per, total);
     int pair = t_lo / nk, kt = t_lo - pair * nk, left = t_hi - t_lo;
     auto issue = [&](int buf) __attribute__((always_inline)) {
         unsigned char* base = smem + buf * STAGE + wave * 1024;
-        const unsigned short* a = (pair == 2 ? p.a1 : p.a0) + (long long)kt * BK;
-        const unsigned short* b = (pair == 1 ? p.b1 : p.b0) + (long long)kt * BK;
+        const unsigned short* a = (pair == 2 ? p.a1 : p.a0) + (AT ? kt * BK * p.lda : (long long)kt * BK);
+        const unsigned short* b = (pair == 1 ? p.b1 : p.b0) + (BT ? kt * BK * p.ldb : (long long)kt * BK);
 #pragma unroll
         for (int i = 0; i < APT; ++i) load16(a + a_off[i], base + i * (NW * 1024));
 #pragma unroll
@@ -137,17 +152,39 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     const int sw = (lr >> 1) & 7;
+    // transposing reads: this lane's byte of a tile for the 32 columns from c, k 0 - 3 (+ 8 for lanes 32-63)
+    const int tk = 8 * lh + ((lane & 15) >> 2), tslot = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    int at[RM], bt[RN];
+#pragma unroll
+    for (int i = 0; i < RM; ++i) at[i] = tk * BM * 2 + ((((wm * TM + i * 32) >> 3) + tslot) ^ quarter<BM>(tk)) * 16 + (lane & 1) * 8;
+#pragma unroll
+    for (int j = 0; j < RN; ++j) bt[j] = tk * BN * 2 + ((((wn * TN + j * 32) >> 3) + tslot) ^ quarter<BN>(tk)) * 16 + (lane & 1) * 8;
+    auto turned = [&](const unsigned char* x, int row) __attribute__((always_inline)) {         // k 0 - 3 and 4 - 7 of one column
+        typedef __attribute__((address_space(3))) i16x4* lds_ptr;
+        typedef short i16x8 __attribute__((ext_vector_type(8)));
+        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)x), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(x + 4 * row));
+        const i16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        return __builtin_bit_cast(typename Vec<E>::x8, both);
+    };
     auto compute = [&](int buf) __attribute__((always_inline)) {
-        const unsigned char* sa = smem + buf * STAGE + (wm * TM + lr) * ROWB;
-        const unsigned char* sb = smem + buf * STAGE + A_BYTES + (wn * TN + lr) * ROWB;
+        const unsigned char* ta = smem + buf * STAGE;
+        const unsigned char* tb = ta + A_BYTES;
+        const unsigned char* sa = ta + (wm * TM + lr) * ROWB;
+        const unsigned char* sb = tb + (wn * TN + lr) * ROWB;
 #pragma unroll
         for (int s = 0; s < BK / 16; ++s) {
             const int off = ((2 * s + lh) ^ sw) * 16;
             typename Vec<E>::x8 af[RM], bf[RN];
 #pragma unroll
-            for (int i = 0; i < RM; ++i) af[i] = *reinterpret_cast<const typename Vec<E>::x8*>(sa + i * 32 * ROWB + off);
+            for (int i = 0; i < RM; ++i) {
+                if constexpr (AT) af[i] = turned(ta + at[i] + s * 16 * BM * 2, BM * 2);
+                else af[i] = *reinterpret_cast<const typename Vec<E>::x8*>(sa + i * 32 * ROWB + off);
+            }
 #pragma unroll
-            for (int j = 0; j < RN; ++j) bf[j] = *reinterpret_cast<const typename Vec<E>::x8*>(sb + j * 32 * ROWB + off);
+            for (int j = 0; j < RN; ++j) {
+                if constexpr (BT) bf[j] = turned(tb + bt[j] + s * 16 * BN * 2, BN * 2);
+                else bf[j] = *reinterpret_cast<const typename Vec<E>::x8*>(sb + j * 32 * ROWB + off);
+            }
 #pragma unroll
             for (int i = 0; i < RM; ++i)
 #pragma unroll
@@ -271,28 +308,12 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
                 for (int part = 0; part < (sizeof(T) == 4 ? 2 : 1); ++part) {
                     const E* im = part ? lo : hi;
                     unsigned short* d = part ? p.d1 : p.d0;
-                    unsigned short* tr = part ? p.t1 : p.t0;
                     // rows: eight lanes of 16 bytes each
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const int row = q * 8 + (lane >> 3), c = (lane & 7) * 8;
-                        if (mb + row < p.M && nb + c < p.cols_pad)
+                        if (mb + row < p.rows_pad && nb + c < p.cols_pad)
                             *reinterpret_cast<u32x4*>(d + (long long)(mb + row) * p.ldd + nb + c) = *reinterpret_cast<const u32x4*>(im + row * LD2 + c);
-                    }
-                    // columns: the transposing LDS read hands a lane four rows of its column at a time
-                    const int col = lane & 48;
-                    u32x4 out[4];
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) {
-                        typedef __attribute__((address_space(3))) i16x4* lds_ptr;
-                        const i16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(im + (4 * r + ((lane & 15) >> 2)) * LD2 + col + (lane & 3) * 4));
-                        const u32x2 w = __builtin_bit_cast(u32x2, v);
-                        out[r >> 1][(r & 1) * 2] = w[0];
-                        out[r >> 1][(r & 1) * 2 + 1] = w[1];
-                    }
-                    if (nb + lane < p.N && mb < p.rows_pad) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) *reinterpret_cast<u32x4*>(tr + (long long)(nb + lane) * p.ldt + mb + 8 * r) = out[r];
                     }
                 }
             }
@@ -439,117 +460,70 @@ __device__ __forceinline__ float unscale_of(float m) {
     return m > 0.f ? ldexpf(1.0f, min(max(ilogbf(m) + 1, -46), 74) - 14) : ldexpf(1.0f, -60);
 }
 
-// One matrix [R][C] (rows ld apart) and the 16-bit planes wanted of it: rows [R][Cp] and / or transposed [C][Rp], zeros up to Cp and Rp
-// (multiples of 64).  fp32: u the rows' factors 2^-s, scale the whole tensor's 2^s.  targets: rows left out are zeros.
-struct Turn {
-    const void* src; long long ld; int R, C, Rp, Cp, tiles_c;
+// One matrix [R][C] (rows ld apart) and the 16-bit planes wanted of it, [.][Cp] with zeros from C on: r0, r1 for x (fp32: u the rows' factors
+// 2^-s, found by the forward call), c0, c1 for the products that sum over rows (fp32: scale the whole tensor's 2^s), with zeros in rows R to
+// Rp.  targets: rows left out are zeros.
+struct Planes {
+    const void* src; long long ld; int R, C, Rp, Cp;
     float* u; const float* scale;
     const long long* targets; int words; long long ignore;
     void *r0, *r1, *c0, *c1;
-    int blocks;
 };
-__device__ __forceinline__ bool left_out(const Turn& p, int r) {
-    if (!p.targets) return false;
-    const long long t = p.targets[r];
-    return t < 0 || t >= p.words || t == p.ignore;
-}
 
-// fp32, forward: the rows of both matrices, each with its own scale; one wave a row
-__global__ __launch_bounds__(256) void rows_kernel(const Turn a, const Turn b) {
+// the rows of both matrices, one wave a row; FIND: the rows' factors are found first
+template <typename T, typename E, bool FIND>
+__global__ __launch_bounds__(256) void planes_kernel(const Planes a, const Planes b) {
+    constexpr int V = 16 / sizeof(T);                   // values of a 16-byte load
     const int lane = threadIdx.x & 63;
     int r = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const bool second = r >= a.R;
-    const Turn& p = second ? b : a;
-    if (second) r -= a.R;
-    if (r >= p.R) return;
-    const float* src = (const float*)p.src + (long long)r * p.ld;
-    const bool out = left_out(p, r), vec = p.ld % 4 == 0 && p.C % 4 == 0 && (reinterpret_cast<uintptr_t>(p.src) & 15) == 0;
-    auto at = [&](int c) __attribute__((always_inline)) {
-        f32x4 x = {0.f, 0.f, 0.f, 0.f};
-        if (out || c >= p.C) return x;
-        if (vec) return *reinterpret_cast<const f32x4*>(src + c);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c + e < p.C) x[e] = src[c + e];
-        return x;
-    };
-    float m = 0.f;
-#pragma unroll 4
-    for (int c = lane * 4; c < p.C; c += 256) {
-        const f32x4 v = at(c);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(v[e]));
+    const bool second = r >= a.Rp;
+    const Planes& p = second ? b : a;
+    if (second) r -= a.Rp;
+    if (r >= p.Rp) return;
+    const T* src = (const T*)p.src + (long long)r * p.ld;
+    bool in = r < p.R;
+    if (in && p.targets) {
+        const long long t = p.targets[r];
+        in = t >= 0 && t < p.words && t != p.ignore;
     }
-    const float u = unscale_of(wave_max(m)), f = 1.0f / u;
-    if (lane == 0) p.u[r] = u;
-#pragma unroll 4
-    for (int c = lane * 4; c < p.Cp; c += 256) {
-        const f32x4 v = at(c) * f;
-        _Float16 h[4], l[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) split<_Float16>(v[e], h[e], l[e]);
-        *reinterpret_cast<u32x2*>((_Float16*)p.r0 + (long long)r * p.Cp + c) = *reinterpret_cast<u32x2*>(h);
-        *reinterpret_cast<u32x2*>((_Float16*)p.r1 + (long long)r * p.Cp + c) = *reinterpret_cast<u32x2*>(l);
-    }
-}
-
-// a workgroup takes 64 x 64 values of one of two matrices: 16-byte loads and stores both ways, turned in LDS
-template <typename T, typename E>
-__global__ __launch_bounds__(256) void planes_kernel(const Turn a, const Turn b) {
-    constexpr int V = 16 / sizeof(T);                   // values of a 16-byte load
-    __shared__ E hi[64][66];
-    __shared__ E lo[sizeof(T) == 4 ? 64 : 1][66];
-    const bool second = (int)blockIdx.x >= a.blocks;
-    const Turn& p = second ? b : a;
-    const int id = second ? blockIdx.x - a.blocks : blockIdx.x, ry = id / p.tiles_c * 64, cx = (id - id / p.tiles_c * p.tiles_c) * 64, tid = threadIdx.x;
-    const T* src = (const T*)p.src;
-    const float f = p.scale ? *p.scale : 1.0f;
-    const bool vec = p.ld % V == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
-#pragma unroll
-    for (int i = tid; i < 64 * 64 / V; i += 256) {
-        const int r = i / (64 / V), c = i % (64 / V) * V;
-        T x[V];
-        const T* q = src + (long long)(ry + r) * p.ld + cx + c;
-        const bool in = ry + r < p.R && !left_out(p, ry + r);
-        if (vec && in && cx + c + V <= p.C) *reinterpret_cast<u32x4*>(x) = *reinterpret_cast<const u32x4*>(q);
+    const bool vec = p.ld % V == 0 && p.C % V == 0 && (reinterpret_cast<uintptr_t>(p.src) & 15) == 0;
+    auto at = [&](int c, T (&x)[V]) __attribute__((always_inline)) {
+        if (vec && in && c < p.C) *reinterpret_cast<u32x4*>(x) = *reinterpret_cast<const u32x4*>(src + c);
         else {
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[e] = (in && cx + c + e < p.C) ? q[e] : (T)0.f;
+            for (int e = 0; e < V; ++e) x[e] = (in && c + e < p.C) ? src[c + e] : (T)0.f;
         }
-        E h[V], l[V];
+    };
+    float u = 1.0f;
+    if constexpr (FIND) {
+        float m = 0.f;
+#pragma unroll 4
+        for (int c = lane * V; c < p.C; c += 64 * V) {
+            T x[V];
+            at(c, x);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            if constexpr (sizeof(T) == 4) split<E>((float)x[e] * f, h[e], l[e]);
-            else h[e] = x[e];
-            hi[r][c + e] = h[e];
-            if constexpr (sizeof(T) == 4) lo[r][c + e] = l[e];
+            for (int e = 0; e < V; ++e) m = fmaxf(m, fabsf(x[e]));
         }
-        if (p.r0 && ry + r < p.R) {
-            const long long at = (long long)(ry + r) * p.Cp + cx + c;
-            if constexpr (sizeof(T) == 4) {
-                const float fr = 1.0f / p.u[ry + r];
+        u = unscale_of(wave_max(m));
+        if (lane == 0 && r < p.R) p.u[r] = u;
+    } else if (sizeof(T) == 4 && r < p.R) u = p.u[r];
+    const float f[2] = {1.0f / u, p.scale ? *p.scale : 1.0f};
+#pragma unroll 4
+    for (int c = lane * V; c < p.Cp; c += 64 * V) {
+        const long long to = (long long)r * p.Cp + c;
+        T x[V];
+        at(c, x);
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x4*>((E*)p.r0 + to) = *reinterpret_cast<u32x4*>(x);
+        else {
+            E h[V], l[V];
 #pragma unroll
-                for (int e = 0; e < V; ++e) split<E>((float)x[e] * fr, h[e], l[e]);
-                *reinterpret_cast<u32x2*>((E*)p.r0 + at) = *reinterpret_cast<u32x2*>(h);
-                *reinterpret_cast<u32x2*>((E*)p.r1 + at) = *reinterpret_cast<u32x2*>(l);
-            } else *reinterpret_cast<u32x4*>((E*)p.r0 + at) = *reinterpret_cast<u32x4*>(h);
-        }
-    }
-    if (!p.c0) return;
-    __syncthreads();
+            for (int k = 0; k < (FIND ? 1 : 2); ++k) {
+                if (k == 0 && r >= p.R) continue;
 #pragma unroll
-    for (int i = tid; i < 64 * 8; i += 256) {
-        const int c = i >> 3, r = (i & 7) * 8;
-        if (cx + c >= p.C) continue;
-        const long long at = (long long)(cx + c) * p.Rp + ry + r;
-        E h[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = hi[r + e][c];
-        *reinterpret_cast<u32x4*>((E*)p.c0 + at) = *reinterpret_cast<u32x4*>(h);
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[e] = lo[r + e][c];
-            *reinterpret_cast<u32x4*>((E*)p.c1 + at) = *reinterpret_cast<u32x4*>(h);
+                for (int e = 0; e < V; ++e) split<E>(x[e] * f[k], h[e], l[e]);
+                *reinterpret_cast<u32x2*>((E*)(k ? p.c0 : p.r0) + to) = *reinterpret_cast<u32x2*>(h);
+                *reinterpret_cast<u32x2*>((E*)(k ? p.c1 : p.r1) + to) = *reinterpret_cast<u32x2*>(l);
+            }
         }
     }
 }
@@ -614,24 +588,24 @@ inline Shape shape_of(long long M, long long N, long long ktiles, bool may_split
     return best;
 }
 
-template <typename E, typename T, int BM, int BN, int WM, int WN, int ST, int EP>
+template <typename E, typename T, int BM, int BN, int WM, int WN, int ST, int EP, bool AT, bool BT>
 int go(const Gemm& p, hipStream_t st) {
-    static const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_kernel<E, T, BM, BN, WM, WN, ST, EP>),
+    static const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_kernel<E, T, BM, BN, WM, WN, ST, EP, AT, BT>),
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<BM, BN, ST>());
     if (rc != hipSuccess) { set_error("linear_ce: cannot raise the dynamic LDS limit: %s", hipGetErrorString(rc)); return ICAP_ERR_HIP_BASE + (int)rc; }
-    hipLaunchKernelGGL((gemm_kernel<E, T, BM, BN, WM, WN, ST, EP>), dim3((unsigned)(p.tiles_m * p.tiles_n), p.ksplit), dim3(WM * WN * 64),
+    hipLaunchKernelGGL((gemm_kernel<E, T, BM, BN, WM, WN, ST, EP, AT, BT>), dim3((unsigned)(p.tiles_m * p.tiles_n), p.ksplit), dim3(WM * WN * 64),
                        (smem_bytes<BM, BN, ST>()), st, p);
     return launch_status("linear_ce");
 }
 
-template <typename E, typename T, int EP>
+template <typename E, typename T, int EP, bool AT = false, bool BT = false>
 int gemm(Gemm& p, const Shape& s, hipStream_t st) {
     p.tiles_m = s.tiles_m;
     p.tiles_n = s.tiles_n;
     p.ksplit = s.splits;
-    if (s.tile == 256) return go<E, T, 256, 256, 2, 4, 2, EP>(p, st);
-    if (s.tile == 128) return go<E, T, 128, 128, 2, 2, 2, EP>(p, st);
-    return go<E, T, 64, 64, 2, 1, 4, EP>(p, st);
+    if (s.tile == 256) return go<E, T, 256, 256, 2, 4, 2, EP, AT, BT>(p, st);
+    if (s.tile == 128) return go<E, T, 128, 128, 2, 2, 2, EP, AT, BT>(p, st);
+    return go<E, T, 64, 64, 2, 1, 4, EP, AT, BT>(p, st);
 }
 
 struct Call {
@@ -642,9 +616,10 @@ struct Call {
     long long ignore;
 };
 
-// bytes of D and D^T that a piece of the vocabulary may take: twice the last-level cache (half as many bytes
-// cost 12 % at 6756 words x 4864 rows, which then needed two pieces; twice as many gain 0.5 % at 65536 x 8192)
-constexpr long long PIECE_BYTES = 512ll << 20;
+// Bytes of D that a piece of the vocabulary may take.  The last-level cache holds 256 MB: up to there in one piece (131 MB at 4864 rows x 6756
+// words: 609 us, in two pieces 676), otherwise in pieces of half of it, beside which the operands stay (8192 x 65536, 1 GB: 8436 us,
+// with pieces of 256 MB 8740, of 512 MB 8700).
+constexpr long long WHOLE_BYTES = 256ll << 20, PIECE_BYTES = 128ll << 20;
 
 template <typename T> struct Of { typedef T E; static constexpr int planes = 1; };
 template <> struct Of<float> { typedef _Float16 E; static constexpr int planes = 2; };
@@ -653,47 +628,41 @@ template <> struct Of<float> { typedef _Float16 E; static constexpr int planes =
 template <typename T>
 bool direct(const void* x, long long ld, int C) { return sizeof(T) == 2 && C % 64 == 0 && ld % 8 == 0 && aligned16(x); }
 
+// the 16-bit planes of a matrix: row0, row1 for x; sum0, sum1 for the products that sum over its rows
 template <typename T>
 struct Operand {
-    typename Of<T>::E *row0 = nullptr, *row1 = nullptr, *col0 = nullptr, *col1 = nullptr;
-    long long ld = 0, ldc = 0;
+    typename Of<T>::E *row0 = nullptr, *row1 = nullptr, *sum0 = nullptr, *sum1 = nullptr;
+    long long ld = 0;
 };
 
-// room for the planes of a matrix (want_rows: as the GEMM's A or B in the logits; want_cols: transposed)
+// room for them; Rp: rows with those that are zeros
 template <typename T>
-Operand<T> room(Space& ws, const void* x, long long ld, int R, int C, bool want_cols, bool is_direct) {
+Operand<T> room(Space& ws, const void* x, long long ld, int Rp, int C, bool backward, bool is_direct) {
     typedef typename Of<T>::E E;
     Operand<T> o;
     o.ld = up(C, 64);
-    o.ldc = up(R, 64);
     if (is_direct) { o.row0 = (E*)const_cast<void*>(x); o.ld = ld; }
-    else {
-        o.row0 = ws.take<E>(R * o.ld);
-        if (Of<T>::planes == 2) o.row1 = ws.take<E>(R * o.ld);
-    }
-    if (want_cols) {
-        o.col0 = ws.take<E>(C * o.ldc);
-        if (Of<T>::planes == 2) o.col1 = ws.take<E>(C * o.ldc);
-    }
+    else o.row0 = ws.take<E>(Rp * o.ld);
+    if (Of<T>::planes == 2) o.row1 = ws.take<E>(Rp * o.ld);
+    o.sum0 = o.row0;
+    if (Of<T>::planes == 2 && backward) { o.sum0 = ws.take<E>(Rp * o.ld); o.sum1 = ws.take<E>(Rp * o.ld); }
     return o;
 }
 
 template <typename T>
-Turn turn_of(const Operand<T>& o, const void* x, long long ld, int R, int C, bool is_direct, float* u, const float* scale) {
-    Turn t{x, ld, R, C, (int)up(R, 64), (int)up(C, 64), (int)(up(C, 64) / 64), u, scale, nullptr, 0, 0, is_direct ? nullptr : (void*)o.row0, o.row1, o.col0, o.col1, 0};
-    if (!is_direct || o.col0) t.blocks = (int)(up(R, 64) / 64) * t.tiles_c;
-    return t;
+Planes planes_of(const Operand<T>& o, const void* x, long long ld, int R, int Rp, int C, bool is_direct, float* u, const float* scale) {
+    return {x, ld, R, C, is_direct ? 0 : Rp, (int)up(C, 64), u, scale, nullptr, 0, 0, o.row0, o.row1, o.sum0, o.sum1};
 }
 
 template <typename T>
 struct Plan {
-    bool dh_direct, dw_direct;
+    bool h_direct, w_direct;
     Operand<T> h, w;
     // forward
     float2* part; float* target_logit; int strips;
     // backward
-    int piece; long long ldd, ldt;
-    typename Of<T>::E *d0, *d1, *t0, *t1;
+    int piece; long long ldd;
+    typename Of<T>::E *d0, *d1;
     float *colpart, *acc_h, *acc_w;
     Shape s_logit, s_h, s_w;
     long long bytes;
@@ -701,11 +670,11 @@ struct Plan {
     Plan(const Call& c, bool backward, char* base) {
         typedef typename Of<T>::E E;
         Space ws{base};
-        dh_direct = direct<T>(c.h, c.ld_h, c.E);
-        dw_direct = direct<T>(c.w, c.ld_w, c.E);
-        if (!base) dh_direct = dw_direct = false;           // the size is asked for without pointers: the larger of the two
-        h = room<T>(ws, c.h, c.ld_h, c.R, c.E, backward, dh_direct);
-        w = room<T>(ws, c.w, c.ld_w, c.V, c.E, backward, dw_direct);
+        h_direct = !backward && direct<T>(c.h, c.ld_h, c.E);        // dW needs zeros in the rows that are left out
+        w_direct = direct<T>(c.w, c.ld_w, c.E) && (!backward || c.V % 64 == 0);          // dh reads whole K tiles of words
+        if (!base) h_direct = w_direct = false;             // the size is asked for without pointers: the larger of the two
+        h = room<T>(ws, c.h, c.ld_h, backward ? (int)up(c.R, 64) : c.R, c.E, backward, h_direct);
+        w = room<T>(ws, c.w, c.ld_w, backward ? (int)up(c.V, 64) : c.V, c.E, backward, w_direct);
         const int pairs = Of<T>::planes == 2 ? 3 : 1;
         if (!backward) {
             s_logit = shape_of(c.R, c.V, up(c.E, 64) / 64 * pairs, false);
@@ -714,20 +683,18 @@ struct Plan {
             target_logit = ws.take<float>(c.R);
         } else {
             const long long rp = up(c.R, 64);
-            long long v = PIECE_BYTES / (2 * rp * 2 * Of<T>::planes) / 256 * 256;
+            const long long word = rp * 2 * Of<T>::planes;
+            long long v = (word * c.V <= WHOLE_BYTES ? WHOLE_BYTES : PIECE_BYTES) / word / 256 * 256;
             if (v < 256) v = 256;
             if (v >= c.V) v = c.V;
             else v = up((c.V + (c.V + v - 1) / v - 1) / ((c.V + v - 1) / v), 256);      // pieces of about the same size
             piece = (int)v;
             ldd = up(piece, 64);
-            ldt = rp;
-            d0 = ws.take<E>(c.R * ldd);
-            t0 = ws.take<E>(piece * ldt);
-            d1 = t1 = nullptr;
-            if (Of<T>::planes == 2) { d1 = ws.take<E>(c.R * ldd); t1 = ws.take<E>(piece * ldt); }
+            d0 = ws.take<E>(rp * ldd);
+            d1 = Of<T>::planes == 2 ? ws.take<E>(rp * ldd) : nullptr;
             s_logit = shape_of(c.R, piece, up(c.E, 64) / 64 * pairs, false);
             s_h = shape_of(c.R, c.E, ldd / 64 * pairs, true);
-            s_w = shape_of(piece, c.E, ldt / 64 * pairs, true);
+            s_w = shape_of(piece, c.E, rp / 64 * pairs, true);
             colpart = ws.take<float>((long long)s_logit.tiles_m * 2 * c.V);
             acc_h = ws.take<float>((s_h.splits > 1 || piece < c.V) ? (long long)s_h.splits * c.R * c.E : 0);
             acc_w = ws.take<float>(s_w.splits > 1 ? (long long)s_w.splits * piece * c.E : 0);
@@ -745,12 +712,16 @@ template <typename T>
 void operands(const Call& c, Plan<T>& p, float* out, bool backward, hipStream_t st) {
     float *uh = nullptr, *uw = nullptr;
     if constexpr (sizeof(T) == 4) { uh = out + OUT_ROWS; uw = uh + up(c.R, 64); }
-    Turn a = turn_of<T>(p.h, c.h, c.ld_h, c.R, c.E, p.dh_direct, uh, uh ? out + 2 : nullptr), b = turn_of<T>(p.w, c.w, c.ld_w, c.V, c.E, p.dw_direct, uw, uw ? out + 4 : nullptr);
+    Planes a = planes_of<T>(p.h, c.h, c.ld_h, c.R, backward ? (int)up(c.R, 64) : c.R, c.E, p.h_direct, uh, uh && backward ? out + 2 : nullptr);
+    const Planes b = planes_of<T>(p.w, c.w, c.ld_w, c.V, backward ? (int)up(c.V, 64) : c.V, c.E, p.w_direct, uw, uw && backward ? out + 4 : nullptr);
     a.targets = c.targets;
     a.words = c.V;
     a.ignore = c.ignore;
-    if (sizeof(T) == 4 && !backward) hipLaunchKernelGGL(rows_kernel, dim3((unsigned)(((long long)c.R + c.V + 3) / 4)), dim3(256), 0, st, a, b);
-    else if (a.blocks + b.blocks > 0) hipLaunchKernelGGL((planes_kernel<T, typename Of<T>::E>), dim3(a.blocks + b.blocks), dim3(256), 0, st, a, b);
+    const long long rows = (long long)a.Rp + b.Rp;
+    if (rows == 0) return;
+    const dim3 grid((unsigned)((rows + 3) / 4));
+    if (sizeof(T) == 4 && !backward) hipLaunchKernelGGL((planes_kernel<T, typename Of<T>::E, sizeof(T) == 4>), grid, dim3(256), 0, st, a, b);
+    else hipLaunchKernelGGL((planes_kernel<T, typename Of<T>::E, false>), grid, dim3(256), 0, st, a, b);
 }
 
 template <typename T>
@@ -792,23 +763,24 @@ int bwd(const Call& c, const float* row_lse, const float* meta, const float* gra
         const int vn = c.V - v0 < p.piece ? c.V - v0 : p.piece;
         Gemm g = logits<T>(c, p, meta, v0, vn);
         g.lse = row_lse;
-        g.d0 = (unsigned short*)p.d0; g.d1 = (unsigned short*)p.d1; g.t0 = (unsigned short*)p.t0; g.t1 = (unsigned short*)p.t1;
-        g.ldd = p.ldd; g.ldt = p.ldt;
+        g.d0 = (unsigned short*)p.d0; g.d1 = (unsigned short*)p.d1;
+        g.ldd = p.ldd;
         g.rows_pad = (int)up(c.R, 64); g.cols_pad = (int)up(vn, 64);
         g.colpart = db ? p.colpart : nullptr; g.ldc = c.V;
         if (int rc = gemm<E, T, EP_GRAD>(g, resized(p.s_logit, c.R, vn), st)) return rc;
         if (dh) {
             Gemm q{};
             q.a0 = (const unsigned short*)p.d0; q.a1 = (const unsigned short*)p.d1;
-            q.b0 = (const unsigned short*)p.w.col0 + v0; q.b1 = p.w.col1 ? (const unsigned short*)p.w.col1 + v0 : nullptr;
-            q.lda = p.ldd; q.ldb = p.w.ldc;
+            q.b0 = (const unsigned short*)p.w.sum0 + v0 * p.w.ld; q.b1 = p.w.sum1 ? (const unsigned short*)p.w.sum1 + v0 * p.w.ld : nullptr;
+            q.lda = p.ldd; q.ldb = p.w.ld;
             q.M = c.R; q.N = c.E; q.K = (int)up(vn, 64);
+            q.b_cols = (int)up(c.E, 64);
             q.pairs = g.pairs;
             q.f0 = grad_out; q.f1 = meta + 1; q.f2 = sizeof(T) == 4 ? meta + 5 : nullptr; q.f = back;
             const bool whole = p.s_h.splits == 1 && p.piece >= c.V;
             if (whole) { q.out = dh; q.ldo = c.E; }
             else { q.acc = p.acc_h; q.accumulate = v0 > 0; }
-            if (int rc = gemm<E, T, EP_OUT>(q, p.s_h, st)) return rc;
+            if (int rc = gemm<E, T, EP_OUT, false, true>(q, p.s_h, st)) return rc;
             if (!whole && v0 + vn == c.V) {
                 const long long n = (long long)c.R * c.E;
                 hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(up(n, 1024) / 1024 > 4096 ? 4096 : up(n, 1024) / 1024)), dim3(256), 0, st, p.acc_h, p.s_h.splits, n,
@@ -817,16 +789,17 @@ int bwd(const Call& c, const float* row_lse, const float* meta, const float* gra
         }
         if (dw) {
             Gemm q{};
-            q.a0 = (const unsigned short*)p.t0; q.a1 = (const unsigned short*)p.t1;
-            q.b0 = (const unsigned short*)p.h.col0; q.b1 = (const unsigned short*)p.h.col1;
-            q.lda = p.ldt; q.ldb = p.h.ldc;
+            q.a0 = (const unsigned short*)p.d0; q.a1 = (const unsigned short*)p.d1;
+            q.b0 = (const unsigned short*)p.h.sum0; q.b1 = (const unsigned short*)p.h.sum1;
+            q.lda = p.ldd; q.ldb = p.h.ld;
             q.M = vn; q.N = c.E; q.K = (int)up(c.R, 64);
+            q.a_cols = (int)up(vn, 64); q.b_cols = (int)up(c.E, 64);
             q.pairs = g.pairs;
             q.f0 = grad_out; q.f1 = meta + 1; q.f2 = sizeof(T) == 4 ? meta + 3 : nullptr; q.f = back;
             T* dst = (T*)dw + (long long)v0 * c.E;
             if (p.s_w.splits == 1) { q.out = dst; q.ldo = c.E; }
             else q.acc = p.acc_w;
-            if (int rc = gemm<E, T, EP_OUT>(q, resized(p.s_w, vn, c.E), st)) return rc;
+            if (int rc = gemm<E, T, EP_OUT, true, true>(q, resized(p.s_w, vn, c.E), st)) return rc;
             if (p.s_w.splits > 1) {
                 const long long n = (long long)vn * c.E;
                 hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(up(n, 1024) / 1024 > 4096 ? 4096 : up(n, 1024) / 1024)), dim3(256), 0, st, p.acc_w, p.s_w.splits, n, dst, q);

@@ -863,8 +863,8 @@ int icap_attention_packed_bwd(int dtype, const void* dout, const void* q, const 
  * Backward: gradients of grad_out[0] (device scalar) * loss in the tensors' type, dense: dhidden [rows][width], dweight
  * [vocab][width], dbias [vocab]; each may be NULL.  fp32 products are fp32-accurate (a gradient to 2^-38 of the largest magnitude of
  * weight and hidden, too); magnitudes of fp32 hidden and weight below 2^74.
- * ws: icap_linear_ce_ws_bytes(dtype, rows, width, vocab, backward) bytes, 16-byte aligned: bounded by about
- * 512 MB, fp32 partial results and copies of hidden and weight, whatever the vocabulary. */
+ * ws: icap_linear_ce_ws_bytes(dtype, rows, width, vocab, backward) bytes, 16-byte aligned: at most 256 MB, fp32 partial results and
+ * copies of hidden and weight, whatever the vocabulary (but 256 words are worked on at once, however many rows). */
 long long icap_linear_ce_out_floats(int dtype, int rows, int vocab);
 long long icap_linear_ce_ws_bytes(int dtype, int rows, int width, int vocab, int backward);
 int icap_linear_ce_fwd(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,

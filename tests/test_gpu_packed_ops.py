@@ -384,7 +384,7 @@ def test_linear_ce_large_tiles_and_split_contraction(dtype):
 
 
 def test_linear_ce_in_several_pieces_of_the_vocabulary():
-    """So many rows that D of the whole vocabulary would pass the workspace's limit: three pieces, the last one shorter."""
+    """So many rows that D of the whole vocabulary would pass the workspace's limit: five pieces, the last one shorter."""
     from image_captioning_amd import _native as N
     R, E, V = 130000, 16, 2501
     assert N.load().icap_linear_ce_ws_bytes(1, R, E, V, 1) < 3 * R * V
