@@ -13,16 +13,23 @@
 // rescaling stay in the lane, and the eight values a lane half holds of 16 accumulator rows are the B operand of the next product as
 // they come (V^T is read in the same order of the contraction).  Rows that see no key get zeros (and a log-sum of -inf).
 //
-// What bounds it: at dim 128 a wave of 32 rows needs per 64 keys 1024 cycles of its SIMD's matrix core, about as many of
-// its vector unit (32 exponentials of 16 cycles) and a quarter of that of the CU's LDS (32 KB at 128 bytes a cycle).  So two waves a
+// Tiles are multiplied whole, so that a tile's products meet places that its rows do not see: those get the weight zero, and a row whose
+// result is not finite is formed once more from what it sees alone ("values that are not finite" below).
+//
+// What bounds it: at dim 128 a wave of 32 rows needs per 64 keys 1024 cycles of its SIMD's matrix core and about as many of
+// its vector unit (32 exponentials of 16 cycles), and the two overlap only in part: 872 TFLOP/s on six bf16 prompts of up to 8192 tokens
+// (354 us; a product of that many operations alone takes 252), matrix cores busy 47 % of the cycles, LDS without conflicts.  So two waves a
 // SIMD interleave (four-wave workgroups, two a CU: with one of eight waves all were in the same phase, 404 against 383 us on
-// 12k tokens of bf16 prompts), the scores of the next step are formed beside the exponentials of this one (353 us), and nothing
+// those prompts), the scores of the next step are formed beside the exponentials of this one (383 -> 353 us), and nothing
 // else stays in the loop:
 //   * tiles go global -> LDS without registers, double-buffered, one barrier a step;
-//   * LDS rows are not padded (the direct loads write linearly) but permuted in 16-byte slots by swizzle(), which spreads the 8
+//   * LDS rows are not padded (the direct loads write linearly) but permuted in 16-byte slots by swizzle(), which spreads the
 //     rows of a fragment read and the 4 rows of a transposing read over different banks;
 //   * the running maximum is only followed when it grows by more than 2^8 (weights stay below 256, sums in fp32, so nothing
 //     is lost), which leaves the accumulators alone in almost every step.
+// Backward, 8 bf16 sequences of up to 2048 tokens, dim 64: dK and dV 106 + 13, dQ 69 + 10 (the second part of dS), forward 61 us; the steps of
+// the longest sequence's first keys, one after another, are what they last.  Short texts (fp32 captions of up to 58 tokens: forward 35, dQ 45,
+// dK and dV 49 us) are bound by places of other texts in their tiles: a wave multiplies about three times what its rows see.
 #pragma once
 #include "packed.hpp"
 
@@ -656,7 +663,7 @@ __global__ __launch_bounds__(RW * KG * 64, DP == 128 && (RW < 4 || sizeof(T) == 
 // the B operands as they come (dV^T = dO^T P, dK^T = Q^T dS).
 // KW waves of 32 keys each, RG times: the row groups take every RG-th 32 rows and are added up in LDS at the end.  The first keys of
 // a long causal sequence meet all its rows, and that chain of steps - not the sum of the work - is what a launch of few sequences
-// lasts (167 -> 109 us with two groups, 8 bf16 sequences of up to 2048 tokens, dim 64).
+// lasts (167 -> 109 us with two groups, before dS had two parts, 8 bf16 sequences of up to 2048 tokens, dim 64).
 template <typename T, int DP, int KW, int RG>
 __global__ __launch_bounds__(KW * RG * 64, DP == 128 ? 1 : 2) void dkv_kernel(const AttnArgs a) {
     constexpr int NTHR = KW * RG * 64, BK = KW * 32, BR = 32 * RG, KK = DP / 16, ND = DP / 32;
@@ -798,8 +805,9 @@ void launch_dkv(const AttnArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((dkv_kernel<T, DP, KW, RG>), dim3(blocks_for(a, a.tokens_k, KW * 32)), dim3(KW * RG * 64), 0, st, a);
 }
 
-// Waves a workgroup: four where the average sequence fills them (they share each staged tile), two otherwise; split keys go
-// with one wave (attention_splits in capi.hip: few rows, long caches)
+// Waves a workgroup: four where the average sequence fills them, since they share each staged tile (two / four: bf16 prompts of up to 8192
+// tokens 574 / 361 us), two otherwise (fp32 captions of up to 58 tokens, forward and backward, 136 / 148); split keys go with one wave
+// (attention_splits in capi.hip: few rows, long caches)
 template <typename T, int DP>
 int fwd_dim(const AttnArgs& a, hipStream_t st) {
     if (a.splits > 1) return launch_fwd<T, DP, 1>(a, st);
@@ -807,16 +815,21 @@ int fwd_dim(const AttnArgs& a, hipStream_t st) {
     return launch_fwd<T, DP, 4>(a, st);
 }
 
+// Backward: a wave that walks alone over all a sequence's keys (rows) is what a launch lasts, as long as there are fewer workgroups than the
+// card takes at once (some 2048 of two waves); then two groups of waves share the walk.  16-bit types, dim 64, alone / shared: 8
+// sequences of 512 tokens, 8 heads 79 / 63 us; of up to 2048 324 / 239; but 64 of 200, 16 heads (3200 workgroups) 156 / 172, 16 of 1024 with
+// dim 128 (2048) 430 / 478.  Not where a walk is a few steps anyway: fp32 captions of up to 58 tokens 136 / 173.
 template <typename T, int DP>
 int bwd_dim(const AttnArgs& a, hipStream_t st) {
-    const long long rows = (long long)a.tokens_q * a.group / a.seqs;
+    const long long all = (long long)a.tokens_q * a.group;
+    const bool lengthy = all / a.seqs > 96;
     if (a.tokens_q > 0) {
-        if (rows <= 96) launch_dq<T, DP, 2, 1>(a, st);
-        else launch_dq<T, DP, 2, 2>(a, st);
+        if (lengthy && blocks_for(a, all, 64) < 2048) launch_dq<T, DP, 2, 2>(a, st);
+        else launch_dq<T, DP, 2, 1>(a, st);
     }
     if (a.tokens_k > 0) {
-        if (rows <= 96) launch_dkv<T, DP, 2, 1>(a, st);
-        else launch_dkv<T, DP, 2, 2>(a, st);
+        if (lengthy && blocks_for(a, a.tokens_k, 64) < 2048) launch_dkv<T, DP, 2, 2>(a, st);
+        else launch_dkv<T, DP, 2, 1>(a, st);
     }
     return launch_status("attention_packed_bwd");
 }

@@ -152,6 +152,13 @@ def test_attention_single_tokens_over_long_caches(dtype, H, K):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_attention_more_tiles_than_the_card_takes_at_once(dtype):
+    """Long sequences whose backward pass does not share a walk between groups of waves: there are enough workgroups."""
+    lens = [130] * 15 + [131]
+    compare_attention(dtype, lens, lens, 64, 64, 8, True, seed=11)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_attention_large_scores(dtype):
     compare_attention(dtype, [90, 31], [90, 31], 2, 1, 64, True, seed=9, big=20.0)
     compare_attention(dtype, [40], [40], 2, 1, 64, False, seed=10, scale=1e-3)
