@@ -13,6 +13,8 @@
 // repeated, and nothing is kept between calls.
 // Bound: HBM.  3 size(p) + 16 bytes a value with 32-bit states, 3 size(p) + 4 + 1/16 with 8-bit ones.  One wave owns 256 values at a
 // time (four a lane, 16 bytes of fp32), which is one scale's block: the largest magnitude is one wave reduction, no LDS, no barrier.
+// Measured: 20 fp32 tensors, 15.7 M values, fp32 states 118 us = 3.7 TB/s; 48 bf16 tensors, 176 M values, 8-bit states 444 us = 4.0 TB/s (a
+// large copy: 4.7); 250 fp32 tensors, 24 M values, 8-bit states 111 us in five launches.
 #include "packed.hpp"
 #include <math.h>
 
