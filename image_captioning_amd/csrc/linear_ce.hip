@@ -820,9 +820,12 @@ static int check(int dtype, const Call& c, const char* what) {
         set_error("%s: null tensor, empty size or overlapping rows", what);
         return ICAP_ERR_ARG;
     }
-    // tiles and blocks of 64 x 64 values are counted in 32 bits
-    if (c.R > 65535 * 64 || c.E > (1 << 20) || c.V > 65535 * 64 || up(c.R, 64) / 64 * (up(c.V, 64) / 64) > 0x7fffffffLL ||
-        (up(c.R, 64) + up(c.V, 64)) / 64 * (up(c.E, 64) / 64) > 0x7fffffffLL) {
+    // a launch has fewer than 2^32 threads
+    const auto fits = [&](long long m, long long n, long long k) {
+        const Shape t = shape_of(m, n, up(k, 64) / 64, false);
+        return (long long)t.tiles_m * t.tiles_n * (t.tile == 64 ? 128 : t.tile == 128 ? 256 : 512) < (1ll << 32);
+    };
+    if (c.R > 65535 * 64 || c.E > (1 << 20) || c.V > 65535 * 64 || !fits(c.R, c.V, dtype == DT_F32 ? 3ll * c.E : c.E) || !fits(c.R > c.V ? c.R : c.V, c.E, 1 << 16)) {
         set_error("%s: rows=%d width=%d vocabulary=%d too large", what, c.R, c.E, c.V);
         return ICAP_ERR_LIMIT;
     }

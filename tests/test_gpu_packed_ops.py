@@ -246,6 +246,25 @@ def test_attention_infinite_values_are_the_formulas(dtype):
     assert (got[:, :, 3] == math.inf).all()
 
 
+def test_attention_over_more_than_2_31_elements():
+    """Rows 2^23 elements apart: the last ones lie beyond 2^31 elements, whichever tensor they are of."""
+    n, H, K, dim = 290, 2, 1, 32
+    wide = torch.empty(n, 1 << 23, device=D, dtype=BF16)
+    packed = rnd(n, (2 * H + 2 * K) * dim, seed=1, dtype=BF16).to(D)
+    wide[:, -packed.size(1):] = packed
+
+    def parts(x):
+        return [t.unflatten(1, (-1, dim)) for t in x.split((H * dim, K * dim, K * dim, H * dim), 1)]
+    q, k, v, g = parts(packed)
+    far = parts(wide[:, -packed.size(1):])
+    assert far[1].stride(0) == 1 << 23
+    for lq in ([n], [1]):
+        near = run_attention(q[-sum(lq):], k, v, lq, [n], True, None, g[-sum(lq):])
+        got = run_attention(far[0][-sum(lq):], far[1], far[2], lq, [n], True, None, far[3][-sum(lq):])
+        for name in near:
+            assert torch.equal(got[name], near[name]), name
+
+
 def test_attention_offsets_beyond_the_tensors_are_cut_off():
     from image_captioning_amd import ops
     q, k, v = (rnd(40, 2, 32, seed=s).to(D) for s in (1, 2, 3))
@@ -382,6 +401,34 @@ def test_linear_ce_rows_do_not_touch_each_other(dtype, bad):
     others = torch.arange(R) != 33
     for n, x in (("row_loss", row), ("dh", dh)):
         within(x.cpu()[others], want[n][0][others], want[n][1][others], n)
+
+
+def test_linear_ce_over_more_than_2_31_elements():
+    """A weight of 2.2e9 elements, and hidden rows 2^23 elements apart."""
+    from image_captioning_amd import train_ops as T
+    R, E, V = 290, 8192, 268500
+    wide = torch.empty(R, 1 << 23, device=D, dtype=BF16)
+    h = wide[:, -E:]
+    h.copy_(rnd(R, E, seed=1, dtype=BF16))
+    w = torch.empty(V, E, device=D, dtype=BF16)
+    for i, rows in enumerate(w.split(65536)):
+        rows.copy_(torch.randn(rows.shape, device=D, generator=torch.Generator(D).manual_seed(i)).mul_(E ** -0.5))
+    t = torch.randint(0, V, (R,), generator=torch.Generator().manual_seed(2))
+    t[-3:] = V - 1
+    _, row, saved = T.linear_ce_fwd(h, w, None, t.to(D), -100, True)
+    dh, dw, _ = T.linear_ce_bwd(torch.tensor([1.0], device=D), saved)
+    hc = h.float()
+    x = torch.cat([hc @ rows.float().t() for rows in w.split(65536)], 1).double()
+    lse = torch.logsumexp(x, 1)
+    # exact products summed in fp32 on both sides: each x is off by at most E 2^-24 of its terms' magnitudes
+    e = 2 * E * E24 * float(max((hc.abs() @ rows.float().abs().t()).max() for rows in w.split(65536)))
+    assert ((row.double() - (lse - x.gather(1, t.to(D)[:, None])[:, 0])).abs() < 2 * e + 1e-5).all()
+    hot = (t.to(D)[:, None] == torch.arange(V - 500, V, device=D)).double()
+    d = torch.exp(x[:, -500:] - lse[:, None]) - hot
+    want = d.t() @ hc.double() / R
+    bound = (2.0 ** -8 + 2 * e) * 1.1 * ((d.abs() + hot).t() @ hc.double().abs() / R) + 2.0 ** -8 * want.abs()     # D and the result rounded
+    assert ((dw[-500:].double() - want).abs() <= bound).all()
+    assert torch.isfinite(dh).all() and dh.any()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -601,6 +648,20 @@ def test_adamw_tensors_more_than_one_launch_holds():
     for i in range(130):
         T.adamw_tensors([alone[i]], [gs[i]], [ma[i]], [va[i]], step=1, seed=9, lr=1e-2, index=[i])
         assert torch.equal(ps[i], alone[i]) and torch.equal(vs[i][0].view(torch.uint8), va[i][0].view(torch.uint8)) and torch.equal(ms[i][1], ma[i][1])
+
+
+def test_adamw_tensors_of_more_than_2_31_values():
+    from image_captioning_amd import train_ops as T
+    n, tail = (1 << 31) + 777, 3000
+    p, g = (torch.zeros(n, device=D, dtype=BF16) for _ in range(2))
+    m, v = (torch.zeros(n, device=D) for _ in range(2))
+    small = [rnd(tail, seed=1, dtype=BF16).to(D), rnd(tail, seed=2, dtype=BF16).to(D), rnd(tail, seed=3).to(D), rnd(tail, seed=4).to(D).abs()]
+    for x, y in zip((p, g, m, v), small):
+        x[-tail:] = y
+    T.adamw_tensors([p], [g], [m], [v], step=3, lr=1e-2)
+    T.adamw_tensors(small[:1], small[1:2], small[2:3], small[3:], step=3, lr=1e-2)
+    for x, y in zip((p, m, v), (small[0], small[2], small[3])):
+        assert torch.equal(x[-tail:], y) and not x[:1000].any()
 
 
 def test_adamw_tensors_refusals_on_the_device():

@@ -53,7 +53,7 @@ def ce_fwd(**kw):
 
 @pytest.mark.parametrize("kw,code", [(dict(dtype=7), 1), (dict(h=None), 1), (dict(t=None), 1), (dict(R=0), 1), (dict(V=0), 1), (dict(ldh=63), 1), (dict(ldw=10), 1),
                                      (dict(ws=None), 1), (dict(ws=24), 1), (dict(nbytes=8), 1), (dict(lse=None), 1), (dict(R=65535 * 64 + 1), 3), (dict(V=65535 * 64 + 1), 3),
-                                     (dict(E=(1 << 20) + 1, ldh=1 << 21, ldw=1 << 21), 3)])
+                                     (dict(E=(1 << 20) + 1, ldh=1 << 21, ldw=1 << 21), 3), (dict(R=1 << 22, V=1 << 21), 3), (dict(R=1 << 22, E=1 << 20, ldh=1 << 20, ldw=1 << 20), 3)])
 def test_linear_ce_forward_refuses(kw, code):
     assert ce_fwd(**kw) == code
 
