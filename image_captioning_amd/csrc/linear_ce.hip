@@ -416,6 +416,7 @@ __global__ __launch_bounds__(256) void lse_kernel(const float2* part, int strips
 // largest of n values >= 0, by 1024 threads
 __device__ __forceinline__ float block_max(const float* x, int n, float* red) {
     float m = 0.f;
+#pragma unroll 8
     for (int i = threadIdx.x; i < n; i += 1024) m = fmaxf(m, x[i]);
     m = wave_max(m);
     __syncthreads();
@@ -437,6 +438,7 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const
     }
     double s = 0.0;
     int c = 0;
+#pragma unroll 8
     for (int r = threadIdx.x; r < R; r += 1024) {
         s += row_loss[r];
         const long long t = targets[r];
@@ -531,25 +533,33 @@ __global__ __launch_bounds__(256) void planes_kernel(const Planes a, const Plane
     }
 }
 
-// out[i] = factor * sum over splits of acc[split][i], in order
-template <typename T>
+// out[i] = factor * sum over splits of acc[split][i], in order; V values a thread (n % V == 0)
+template <typename T, int V>
 __global__ __launch_bounds__(256) void join_kernel(const float* acc, int splits, long long n, T* out, const Gemm p) {
+    typedef float vec __attribute__((ext_vector_type(V)));
+    typedef T tvec __attribute__((ext_vector_type(V)));
     const float f = final_factor(p);
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        float s = acc[i];
-        for (int z = 1; z < splits; ++z) s += acc[z * n + i];
-        out[i] = (T)(s * f);
+    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * V; i < n; i += (long long)gridDim.x * 256 * V) {
+        vec s = *reinterpret_cast<const vec*>(acc + i);
+#pragma unroll 8
+        for (int z = 1; z < splits; ++z) s += *reinterpret_cast<const vec*>(acc + z * n + i);
+        *reinterpret_cast<tvec*>(out + i) = __builtin_convertvector(s * f, tvec);
     }
 }
 
+// 64 columns a workgroup, four parts of the row blocks each
 template <typename T>
 __global__ __launch_bounds__(256) void bias_kernel(const float* colpart, int blocks, int V, T* out, const float* f0, const float* f1) {
-    const int v = blockIdx.x * 256 + threadIdx.x;
-    if (v >= V) return;
+    __shared__ float part[4][64];
+    const int c = threadIdx.x & 63, v = blockIdx.x * 64 + c, q = threadIdx.x >> 6, per = (blocks + 3) / 4;
     float s = 0.f;
+    if (v < V) {
 #pragma unroll 16
-    for (int b = 0; b < blocks; ++b) s += colpart[(long long)b * V + v];
-    out[v] = (T)(s * (*f0 * *f1));
+        for (int b = q * per; b < min(q * per + per, blocks); ++b) s += colpart[(long long)b * V + v];
+    }
+    part[q][c] = s;
+    __syncthreads();
+    if (q == 0 && v < V) out[v] = (T)((((part[0][c] + part[1][c]) + part[2][c]) + part[3][c]) * (*f0 * *f1));
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -757,6 +767,14 @@ int fwd(const Call& c, int mean_over_valid, float* row_loss, float* row_lse, flo
 }
 
 template <typename T>
+void join(const float* acc, int splits, long long n, T* out, const Gemm& p, hipStream_t st) {
+    const long long blocks = up(n, n % 4 == 0 ? 1024 : 256) / (n % 4 == 0 ? 1024 : 256);
+    const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20));
+    if (n % 4 == 0) hipLaunchKernelGGL((join_kernel<T, 4>), grid, dim3(256), 0, st, acc, splits, n, out, p);
+    else hipLaunchKernelGGL((join_kernel<T, 1>), grid, dim3(256), 0, st, acc, splits, n, out, p);
+}
+
+template <typename T>
 int bwd(const Call& c, const float* row_lse, const float* meta, const float* grad_out, void* dh, void* dw, void* db, char* ws, hipStream_t st) {
     typedef typename Of<T>::E E;
     Plan<T> p(c, true, ws);
@@ -785,9 +803,7 @@ int bwd(const Call& c, const float* row_lse, const float* meta, const float* gra
             else { q.acc = p.acc_h; q.accumulate = v0 > 0; }
             if (int rc = gemm<E, T, EP_OUT, false, true>(q, p.s_h, st)) return rc;
             if (!whole && v0 + vn == c.V) {
-                const long long n = (long long)c.R * c.E;
-                hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(up(n, 1024) / 1024 > 4096 ? 4096 : up(n, 1024) / 1024)), dim3(256), 0, st, p.acc_h, p.s_h.splits, n,
-                                   (T*)dh, q);
+                join(p.acc_h, p.s_h.splits, (long long)c.R * c.E, (T*)dh, q, st);
             }
         }
         if (dw) {
@@ -804,13 +820,12 @@ int bwd(const Call& c, const float* row_lse, const float* meta, const float* gra
             else q.acc = p.acc_w;
             if (int rc = gemm<E, T, EP_OUT, true, true>(q, resized(p.s_w, vn, c.E), st)) return rc;
             if (p.s_w.splits > 1) {
-                const long long n = (long long)vn * c.E;
-                hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(up(n, 1024) / 1024 > 4096 ? 4096 : up(n, 1024) / 1024)), dim3(256), 0, st, p.acc_w, p.s_w.splits, n, dst, q);
+                join(p.acc_w, p.s_w.splits, (long long)vn * c.E, dst, q, st);
             }
         }
     }
     if (db)
-        hipLaunchKernelGGL((bias_kernel<T>), dim3((c.V + 255) / 256), dim3(256), 0, st, p.colpart, p.s_logit.tiles_m * 2, c.V, (T*)db, grad_out, meta + 1);
+        hipLaunchKernelGGL((bias_kernel<T>), dim3((c.V + 63) / 64), dim3(256), 0, st, p.colpart, p.s_logit.tiles_m * 2, c.V, (T*)db, grad_out, meta + 1);
     return launch_status("linear_ce_bwd");
 }
 
