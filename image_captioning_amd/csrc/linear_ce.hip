@@ -20,7 +20,7 @@
 // Bound: the matrix cores (2 R E V flops a product; one forward, three backward of which the logits are repeated).
 // Measured: 8192 rows x 65536 words x 2048, bf16: logits 1984 us (1108 TFLOP/s), a piece of 8192 words: D 266, dh 280, dW 257 (1033, 981, 1068);
 // a library product reaches 1270.  4864 x 6756 x 512, fp32 as three fp16 products: logits 141 us (716), D 166, dh 135, dW 143.  684 x 81 x
-// 512: 72 us in ten launches.
+// 512: 68 us in ten launches.
 #include "packed.hpp"
 
 namespace icap {
