@@ -705,6 +705,35 @@ def test_packed_ops_refusals_on_the_device():
             T.linear_ce_fwd(*args)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_empty_and_smallest_calls(dtype):
+    from image_captioning_amd import ops, train_ops as T, training
+    for lq, lk in (([0], [0]), ([0, 0], [0, 5]), ([3, 0], [0, 0]), ([1], [1])):
+        compare_attention(dtype, lq, lk, 2, 1, 8, True, seed=1)
+        compare_attention(dtype, lq, lk, 2, 1, 8, False, seed=2)
+    for R, E, V in ((1, 1, 1), (2, 1, 300), (65, 3, 2)):
+        compare_ce(dtype, R, E, V, seed=R)
+    p = torch.nn.Parameter(rnd(5, seed=1, dtype=dtype).to(D))
+    none = torch.nn.Parameter(torch.zeros(0, 4, device=D, dtype=dtype))
+    for bits in (8, 32):
+        opt = training.AdamWTensors([p, none], lr=1e-2, state_bits=bits)
+        opt.step()                                            # no gradients: nothing to do
+        p.grad, none.grad = torch.ones_like(p), torch.zeros_like(none)
+        before = p.detach().clone()
+        opt.step()
+        assert opt.param_steps == [1, 1] and (p < before).all()
+        opt.zero_grad()
+    T.adamw_tensors([], [], [], [], step=1, lr=1e-3)
+    # a key head for every query head's own copy: what is expanded is read in place, and its gradient is the copies'
+    q, k = rnd(20, 4, 16, seed=3, dtype=dtype).to(D), rnd(20, 1, 16, seed=4, dtype=dtype).to(D)
+    wide = k.expand(20, 4, 16)
+    cu = offsets([13, 7]).to(D)
+    out, lse = ops.attention_packed(q, wide, wide, cu, want_lse=True)
+    assert torch.equal(out, ops.attention_packed(q, wide.contiguous(), wide.contiguous(), cu))
+    for x, y in zip(T.attention_packed_bwd(out, q, wide, wide, out, lse, cu), T.attention_packed_bwd(out, q, wide.contiguous(), wide.contiguous(), out, lse, cu)):
+        assert torch.equal(x, y)
+
+
 # ------------------------------------------------------------------------------------------------ as they are used
 class Decoder(torch.nn.Module):
     """One attention layer over packed captions and an output layer."""
