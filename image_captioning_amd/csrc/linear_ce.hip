@@ -15,12 +15,17 @@
 //   2^14; the products hi hi + hi lo + lo hi drop 2^-22 of each term: as exact as an fp32 dot product, at three fp16
 //   products for one (the fp32 matrix instruction takes sixteen times a 16-bit product).  For the logits every row of hidden and
 //   every word of the weight has a scale of its own, so that no row touches another; as the contraction of dh and dW runs over words
-//   and rows, those take one scale for all.
+//   and rows, those take one scale for all.  fp16 ends at 2^-24, so D 2^14 alone would hold 22 bits only of probabilities above 2^-17, and none
+//   below 2^-39: the row of dW of a word that is no row's target (its probabilities may all be 1e-10) would be lost.  So each word's
+//   column of D is multiplied by a power of two, its `lift`, that brings its largest value to 1; dW's row leaves it again in its epilogue, and for
+//   dh the word's row of W is divided by it.  The largest probability of a word over all rows comes from a product of the high parts
+//   alone, rounded up by what these may lack: 2^-10 of both rows' lengths (EP_TOP; 63 us at 4864 x 6756 x 512), where dW is wanted.  The values
+//   may be up to 2^-17 below 1 then and still have their 22 bits.
 // Rows that are left out are zeros in every operand that sums over rows, whatever they hold (NaN, infinities).
 // Bound: the matrix cores (2 R E V flops a product; one forward, three backward of which the logits are repeated).
 // Measured: 8192 rows x 65536 words x 2048, bf16: logits 1984 us (1108 TFLOP/s), a piece of 8192 words: D 266, dh 280, dW 257 (1033, 981, 1068);
-// a library product reaches 1270.  4864 x 6756 x 512, fp32 as three fp16 products: logits 141 us (716), D 166, dh 135, dW 143.  684 x 81 x
-// 512: 68 us in ten launches.
+// a library product reaches 1270.  4864 x 6756 x 512, fp32 as three fp16 products: logits 138 us (731), largest values 63,
+// D 160, dh 132, dW 139.  684 x 81 x 512: 80 us in twelve launches.
 #include "packed.hpp"
 
 namespace icap {
@@ -31,7 +36,7 @@ constexpr int STRIP = 64;                           // columns that share one (m
 constexpr float D_SCALE = 16384.0f;                 // fp16 D
 constexpr float LOG2E = 1.4426950408889634f;
 
-enum Epilogue { EP_LSE, EP_GRAD, EP_OUT };
+enum Epilogue { EP_LSE, EP_GRAD, EP_OUT, EP_TOP };
 
 struct Gemm {
     const unsigned short *a0, *a1, *b0, *b1;        // planes: high and (fp32 tensors) low parts
@@ -39,17 +44,20 @@ struct Gemm {
     int M, N, K, pairs, ksplit, tiles_m, tiles_n;   // K % 64 == 0; pairs 1 or 3
     int a_cols, b_cols;                             // operands whose rows are k (K of them): columns there are (% 8 == 0)
     const float *urow, *ucol;                       // fp32: factors 2^-s of the logits' rows and columns
-    // EP_LSE and EP_GRAD
+    // EP_LSE, EP_GRAD and EP_TOP
     const void* bias;                               // type of the tensors
     const long long* targets;
     long long ignore;
     int V, v0;                                      // column 0 of this product is word v0; words end at V
     float2* part; int strips; float* target_logit;  // EP_LSE
-    const float* lse;                               // EP_GRAD
+    const float* lse;                               // EP_GRAD, EP_TOP
     unsigned short *d0, *d1;                        // D [rows_pad][ldd], planes
     long long ldd;
     int rows_pad, cols_pad;                         // D is written (zeros) up to these multiples of 64
-    float* colpart; long long ldc;                  // [row blocks][ldc]
+    float* colpart; long long ldc;                  // [row blocks][ldc]; EP_TOP: log2 of the largest magnitudes of D there
+    const float* lift;                              // fp32: factors of D's columns (null: 1); EP_OUT: what the result's rows are divided by
+    const float *nrow, *ncol;                       // EP_TOP: lengths of A's and B's rows, of which a product may lack their product times
+    float lack;                                     // this
     // EP_OUT
     void* out; long long ldo;                       // final results (type of the tensors)
     float* acc; int accumulate;                     // or fp32 partial results [ksplit][M][N], added to what is there
@@ -85,6 +93,16 @@ __device__ __forceinline__ float final_factor(const Gemm& p) {
     if (p.f1) f *= *p.f1;
     if (p.f2) f *= *p.f2;
     return f;
+}
+
+// op over the 32 lanes of a half
+template <typename F>
+__device__ __forceinline__ float half_wave(float v, F op) {
+    v = op(v, dpp_f<DPP_QUAD_SWAP1>(v));
+    v = op(v, dpp_f<DPP_QUAD_SWAP2>(v));
+    v = op(v, dpp_f<DPP_HALF_MIRROR>(v));
+    v = op(v, dpp_f<DPP_ROW_MIRROR>(v));
+    return op(v, __shfl_xor(v, 16));
 }
 
 // high and low 16-bit parts of a value
@@ -217,7 +235,46 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
     unsigned char* img = smem + wave * IMG;
     const int nb = n0 + wn * TN;                                // the wave's first column
     const bool edge = nb + TN > p.N;                            // some columns do not exist
-    if constexpr (EP != EP_OUT) {
+    // A column's 32 rows are spread over the 32 lanes of a half.  What they make of it is kept by one lane, the half's lr-th column by lane
+    // lr, and stored at once (a store for each column: 89 us where this took 61, EP_TOP of 4864 x 6756 x 512)
+    const int mine = nb + (lr >> 4) * 32 + ((lr >> 2) & 3) * 8 + 4 * lh + (lr & 3);
+    if constexpr (EP == EP_TOP) {
+        const float b = (p.bias && mine < p.N) ? (float)((const T*)p.bias)[p.v0 + mine] * LOG2E : 0.f;
+        int t[RM];
+        float ur[RM], nr[RM], lse2[RM], most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < RM; ++i) {
+            const int m = m0 + wm * TM + i * 32 + lr, mm = min(m, p.M - 1);
+            const long long target = p.targets[mm];
+            const bool on = m < p.M && target >= 0 && target < p.V && target != p.ignore;
+            t[i] = on ? (int)target - p.v0 - nb - 4 * lh : -1;
+            ur[i] = p.urow[mm] * LOG2E;
+            nr[i] = p.nrow[mm] * p.lack * ur[i];
+            lse2[i] = on ? p.lse[mm] * LOG2E : INFINITY;
+        }
+        f32x4 uc[RN][4], nc[RN][4];
+#pragma unroll
+        for (int j = 0; j < RN; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                uc[j][g] = *reinterpret_cast<const f32x4*>(p.ucol + nb + j * 32 + 8 * g + 4 * lh);
+                nc[j][g] = *reinterpret_cast<const f32x4*>(p.ncol + nb + j * 32 + 8 * g + 4 * lh) * uc[j][g];
+            }
+#pragma unroll
+        for (int j = 0; j < RN; ++j)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                float v = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < RM; ++i) {
+                    const float l = fmaf(acc[i][j][k], uc[j][k >> 2][k & 3] * ur[i], fmaf(nc[j][k >> 2][k & 3], nr[i], -lse2[i]));
+                    v = fmaxf(v, t[i] == j * 32 + acc_row(k) ? INFINITY : l);               // a target's |D| may be 1
+                }
+                v = half_wave(v, [](float a, float c) { return fmaxf(a, c); });
+                most = lr == j * 16 + k ? v : most;
+            }
+        if (mine < p.N) p.colpart[(long long)(tile_m * WM + wm) * p.ldc + p.v0 + mine] = most + b;
+    } else if constexpr (EP != EP_OUT) {
         f32x4 bias[RN][4];
 #pragma unroll
         for (int j = 0; j < RN; ++j)
@@ -292,13 +349,16 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
                         typename Vec<E>::x4 h4, l4;
+                        f32x4 up = {D_SCALE, D_SCALE, D_SCALE, D_SCALE};
+                        if constexpr (sizeof(T) == 4)
+                            if (p.lift) up *= *reinterpret_cast<const f32x4*>(p.lift + nb + j * 32 + 8 * g + 4 * lh);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             float d = __builtin_amdgcn_exp2f(fmaf(x[j][4 * g + e], LOG2E, -lse2));
                             if (here && t == j * 32 + 8 * g + 4 * lh + e) d -= 1.0f;
                             d = on ? d : 0.f;
                             colsum[j][g][e] += d;
-                            if constexpr (!__is_same(E, __bf16)) d *= D_SCALE;
+                            if constexpr (!__is_same(E, __bf16)) d *= up[e];
                             E h, l;
                             split<E>(d, h, l);
                             h4[e] = h;
@@ -323,22 +383,15 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
         }
         if constexpr (EP == EP_GRAD) {
             if (p.colpart) {
-                // 32 rows of each column are spread over 32 lanes
+                float sum = 0.f;
 #pragma unroll
                 for (int j = 0; j < RN; ++j)
 #pragma unroll
-                    for (int g = 0; g < 4; ++g)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float v = colsum[j][g][e];
-                            v += dpp_f<DPP_QUAD_SWAP1>(v);
-                            v += dpp_f<DPP_QUAD_SWAP2>(v);
-                            v += dpp_f<DPP_HALF_MIRROR>(v);
-                            v += dpp_f<DPP_ROW_MIRROR>(v);
-                            v += __shfl_xor(v, 16);
-                            const int n = nb + j * 32 + 8 * g + 4 * lh + e;
-                            if (lr == 0 && n < p.N) p.colpart[(long long)(tile_m * WM + wm) * p.ldc + p.v0 + n] = v;
-                        }
+                    for (int k = 0; k < 16; ++k) {
+                        const float v = half_wave(colsum[j][k >> 2][k & 3], [](float a, float c) { return a + c; });
+                        sum = lr == j * 16 + k ? v : sum;
+                    }
+                if (mine < p.N) p.colpart[(long long)(tile_m * WM + wm) * p.ldc + p.v0 + mine] = sum;
             }
         }
     } else {
@@ -348,12 +401,15 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_kernel(const Gemm p) {
             const int mb = m0 + wm * TM + i * 32;
             if (sizeof(T) == 4 || p.acc) {
                 float* im = reinterpret_cast<float*>(img);
+                float fr = f;
+                if constexpr (sizeof(T) == 4)
+                    if (p.lift) fr = f / p.lift[min(mb + lr, p.M - 1)];         // powers of two
 #pragma unroll
                 for (int j = 0; j < RN; ++j)
 #pragma unroll
                     for (int g = 0; g < 4; ++g)
                         *reinterpret_cast<f32x4*>(im + lr * LD4 + j * 32 + 8 * g + 4 * lh) =
-                            f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]} * f;
+                            f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]} * fr;
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     const int row = q * 4 + (lane >> 4), c = (lane & 15) * 4, m = mb + row, n = nb + c;
@@ -467,12 +523,15 @@ __device__ __forceinline__ float unscale_of(float m) {
 
 // One matrix [R][C] (rows ld apart) and the 16-bit planes wanted of it, [.][Cp] with zeros from C on: r0, r1 for x (fp32: u the rows' factors
 // 2^-s, found by the forward call), c0, c1 for the products that sum over rows (fp32: scale the whole tensor's 2^s), with zeros in rows R to
-// Rp.  targets: rows left out are zeros.
+// Rp.  targets: rows left out are zeros.  Planes that are null are not wanted.  top (fp32): log2 of the largest magnitude of a word's column of
+// D in each block of rows, of which the word's lift is made; its row of c0, c1 is divided by it.
 struct Planes {
     const void* src; long long ld; int R, C, Rp, Cp;
     float* u; const float* scale;
     const long long* targets; int words; long long ignore;
     void *r0, *r1, *c0, *c1;
+    const float* top; int blocks;
+    float *lift, *norm;                             // norm: wanted lengths of r0, r1's rows
 };
 
 // the rows of both matrices, one wave a row; FIND: the rows' factors are found first
@@ -511,8 +570,19 @@ __global__ __launch_bounds__(256) void planes_kernel(const Planes a, const Plane
         }
         u = unscale_of(wave_max(m));
         if (lane == 0 && r < p.R) p.u[r] = u;
-    } else if (sizeof(T) == 4 && r < p.R) u = p.u[r];
-    const float f[2] = {1.0f / u, p.scale ? *p.scale : 1.0f};
+    } else if (sizeof(T) == 4 && p.u && r < p.R) u = p.u[r];
+    float f[2] = {1.0f / u, p.scale ? *p.scale : 1.0f};
+    if (sizeof(T) == 4 && !FIND && p.lift) {
+        float m = -INFINITY;
+        if (r < p.R)
+            for (int b = lane; b < p.blocks; b += 64) m = fmaxf(m, p.top[(long long)b * p.R + r]);
+        m = wave_max(m);
+        // to at most 1; not beyond 2^100, so that its inverse stays a factor; a column of zeros (and words that do not exist): 1
+        const float lift = (m < 0.f && m > -INFINITY) ? ldexpf(1.0f, (int)fminf(-ceilf(m), 100.0f)) : 1.0f;
+        if (lane == 0) p.lift[r] = lift;
+        f[1] /= lift;
+    }
+    float squares = 0.f;
 #pragma unroll 4
     for (int c = lane * V; c < p.Cp; c += 64 * V) {
         const long long to = (long long)r * p.Cp + c;
@@ -523,13 +593,21 @@ __global__ __launch_bounds__(256) void planes_kernel(const Planes a, const Plane
             E h[V], l[V];
 #pragma unroll
             for (int k = 0; k < (FIND ? 1 : 2); ++k) {
-                if (k == 0 && r >= p.R) continue;
+                if (k == 0 ? r >= p.R || !p.r0 : !p.c0) continue;
 #pragma unroll
-                for (int e = 0; e < V; ++e) split<E>(x[e] * f[k], h[e], l[e]);
+                for (int e = 0; e < V; ++e) {
+                    const float y = x[e] * f[k];
+                    split<E>(y, h[e], l[e]);
+                    if (!FIND && k == 0) squares = fmaf(y, y, squares);
+                }
                 *reinterpret_cast<u32x2*>((E*)(k ? p.c0 : p.r0) + to) = *reinterpret_cast<u32x2*>(h);
                 *reinterpret_cast<u32x2*>((E*)(k ? p.c1 : p.r1) + to) = *reinterpret_cast<u32x2*>(l);
             }
         }
+    }
+    if (sizeof(T) == 4 && !FIND && p.norm) {
+        squares = wave_sum(squares);
+        if (lane == 0 && r < p.R) p.norm[r] = sqrtf(squares);
     }
 }
 
@@ -664,7 +742,7 @@ Operand<T> room(Space& ws, const void* x, long long ld, int Rp, int C, bool back
 
 template <typename T>
 Planes planes_of(const Operand<T>& o, const void* x, long long ld, int R, int Rp, int C, bool is_direct, float* u, const float* scale) {
-    return {x, ld, R, C, is_direct ? 0 : Rp, (int)up(C, 64), u, scale, nullptr, 0, 0, o.row0, o.row1, o.sum0, o.sum1};
+    return {x, ld, R, C, is_direct ? 0 : Rp, (int)up(C, 64), u, scale, nullptr, 0, 0, o.row0, o.row1, o.sum0, o.sum1, nullptr, 0, nullptr, nullptr};
 }
 
 template <typename T>
@@ -676,8 +754,8 @@ struct Plan {
     // backward
     int piece; long long ldd;
     typename Of<T>::E *d0, *d1;
-    float *colpart, *acc_h, *acc_w;
-    Shape s_logit, s_h, s_w;
+    float *colpart, *acc_h, *acc_w, *lift, *norm_h, *norm_w;
+    Shape s_top, s_logit, s_h, s_w;
     long long bytes;
 
     Plan(const Call& c, bool backward, char* base) {
@@ -708,7 +786,17 @@ struct Plan {
             s_logit = shape_of(c.R, piece, up(c.E, 64) / 64 * pairs, false);
             s_h = shape_of(c.R, c.E, ldd / 64 * pairs, true);
             s_w = shape_of(piece, c.E, rp / 64 * pairs, true);
-            colpart = ws.take<float>((long long)s_logit.tiles_m * 2 * c.V);
+            // the largest values of D's columns, once they have become factors, make room for the columns' sums
+            int blocks = s_logit.tiles_m * 2;
+            lift = norm_h = norm_w = nullptr;
+            if (Of<T>::planes == 2) {
+                s_top = shape_of(c.R, c.V, up(c.E, 64) / 64, false);
+                if (s_top.tiles_m * 2 > blocks) blocks = s_top.tiles_m * 2;
+                lift = ws.take<float>(up(c.V, 64) + 256);       // these are read up to 256 behind the last, too
+                norm_h = ws.take<float>(up(c.R, 64));
+                norm_w = ws.take<float>(up(c.V, 64) + 256);
+            }
+            colpart = ws.take<float>((long long)blocks * c.V);
             acc_h = ws.take<float>((s_h.splits > 1 || piece < c.V) ? (long long)s_h.splits * c.R * c.E : 0);
             acc_w = ws.take<float>(s_w.splits > 1 ? (long long)s_w.splits * piece * c.E : 0);
         }
@@ -721,12 +809,14 @@ struct Plan {
 constexpr int OUT_ROWS = 8;
 inline long long out_floats(int dtype, int R, int V) { return OUT_ROWS + (dtype == DT_F32 ? up(R, 64) + up(V, 64) + 256 : 0); }
 
+// lifted: the sums' planes of the weight come later (words)
 template <typename T>
-void operands(const Call& c, Plan<T>& p, float* out, bool backward, hipStream_t st) {
+void operands(const Call& c, Plan<T>& p, float* out, bool backward, bool lifted, hipStream_t st) {
     float *uh = nullptr, *uw = nullptr;
     if constexpr (sizeof(T) == 4) { uh = out + OUT_ROWS; uw = uh + up(c.R, 64); }
     Planes a = planes_of<T>(p.h, c.h, c.ld_h, c.R, backward ? (int)up(c.R, 64) : c.R, c.E, p.h_direct, uh, uh && backward ? out + 2 : nullptr);
-    const Planes b = planes_of<T>(p.w, c.w, c.ld_w, c.V, backward ? (int)up(c.V, 64) : c.V, c.E, p.w_direct, uw, uw && backward ? out + 4 : nullptr);
+    Planes b = planes_of<T>(p.w, c.w, c.ld_w, c.V, backward ? (int)up(c.V, 64) : c.V, c.E, p.w_direct, uw, uw && backward ? out + 4 : nullptr);
+    if (lifted) { b.Rp = c.V; b.c0 = b.c1 = nullptr; a.norm = p.norm_h; b.norm = p.norm_w; }
     a.targets = c.targets;
     a.words = c.V;
     a.ignore = c.ignore;
@@ -735,6 +825,18 @@ void operands(const Call& c, Plan<T>& p, float* out, bool backward, hipStream_t 
     const dim3 grid((unsigned)((rows + 3) / 4));
     if (sizeof(T) == 4 && !backward) hipLaunchKernelGGL((planes_kernel<T, typename Of<T>::E, sizeof(T) == 4>), grid, dim3(256), 0, st, a, b);
     else hipLaunchKernelGGL((planes_kernel<T, typename Of<T>::E, false>), grid, dim3(256), 0, st, a, b);
+}
+
+// fp32: the words' lifts, from what EP_TOP found, and with them (dh wanted) the planes of the weight for dh
+template <typename T>
+void words(const Call& c, Plan<T>& p, const float* meta, bool dh, hipStream_t st) {
+    Planes a = planes_of<T>(p.w, c.w, c.ld_w, c.V, (int)up(c.V, 64), c.E, false, nullptr, meta + 4), none{};
+    a.r0 = a.r1 = nullptr;
+    if (!dh) { a.c0 = a.c1 = nullptr; a.Cp = 0; }
+    a.top = p.colpart;
+    a.blocks = p.s_top.tiles_m * 2;
+    a.lift = p.lift;
+    hipLaunchKernelGGL((planes_kernel<T, typename Of<T>::E, false>), dim3((unsigned)((a.Rp + 3) / 4)), dim3(256), 0, st, a, none);
 }
 
 template <typename T>
@@ -757,7 +859,7 @@ template <typename T>
 int fwd(const Call& c, int mean_over_valid, float* row_loss, float* row_lse, float* out, char* ws, hipStream_t st) {
     typedef typename Of<T>::E E;
     Plan<T> p(c, false, ws);
-    operands<T>(c, p, out, false, st);
+    operands<T>(c, p, out, false, false, st);
     Gemm g = logits<T>(c, p, out, 0, c.V);
     g.part = p.part; g.strips = p.strips; g.target_logit = p.target_logit;
     if (int rc = gemm<E, T, EP_LSE>(g, p.s_logit, st)) return rc;
@@ -778,7 +880,19 @@ template <typename T>
 int bwd(const Call& c, const float* row_lse, const float* meta, const float* grad_out, void* dh, void* dw, void* db, char* ws, hipStream_t st) {
     typedef typename Of<T>::E E;
     Plan<T> p(c, true, ws);
-    operands<T>(c, p, const_cast<float*>(meta), true, st);         // which only reads it here
+    const bool lifted = sizeof(T) == 4 && dw;
+    operands<T>(c, p, const_cast<float*>(meta), true, lifted, st);         // which only reads it here
+    if constexpr (sizeof(T) == 4)
+        if (lifted) {
+            Gemm g = logits<T>(c, p, meta, 0, c.V);
+            g.lse = row_lse;
+            g.pairs = 1;
+            g.nrow = p.norm_h; g.ncol = p.norm_w;
+            g.lack = 0x1.04p-10f + (float)c.E * 0x1p-24f;           // both sides' low parts, and the sum's own roundings
+            g.colpart = p.colpart; g.ldc = c.V;
+            if (int rc = gemm<E, T, EP_TOP>(g, p.s_top, st)) return rc;
+            words<T>(c, p, meta, dh, st);
+        }
     const float back = __is_same(E, _Float16) ? 1.0f / D_SCALE : 1.0f;
     for (int v0 = 0; v0 < c.V; v0 += p.piece) {
         const int vn = c.V - v0 < p.piece ? c.V - v0 : p.piece;
@@ -788,6 +902,7 @@ int bwd(const Call& c, const float* row_lse, const float* meta, const float* gra
         g.ldd = p.ldd;
         g.rows_pad = (int)up(c.R, 64); g.cols_pad = (int)up(vn, 64);
         g.colpart = db ? p.colpart : nullptr; g.ldc = c.V;
+        g.lift = lifted ? p.lift + v0 : nullptr;
         if (int rc = gemm<E, T, EP_GRAD>(g, resized(p.s_logit, c.R, vn), st)) return rc;
         if (dh) {
             Gemm q{};
@@ -815,6 +930,7 @@ int bwd(const Call& c, const float* row_lse, const float* meta, const float* gra
             q.a_cols = (int)up(vn, 64); q.b_cols = (int)up(c.E, 64);
             q.pairs = g.pairs;
             q.f0 = grad_out; q.f1 = meta + 1; q.f2 = sizeof(T) == 4 ? meta + 3 : nullptr; q.f = back;
+            q.lift = g.lift;
             T* dst = (T*)dw + (long long)v0 * c.E;
             if (p.s_w.splits == 1) { q.out = dst; q.ldo = c.E; }
             else q.acc = p.acc_w;

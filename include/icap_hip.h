@@ -861,8 +861,10 @@ int icap_attention_packed_bwd(int dtype, const void* dout, const void* q, const 
  * icap_linear_ce_out_floats(dtype, rows, vocab) values: out[0] = loss, out[1] = the scale every row was weighted with, as in
  * icap_ce_loss_fwd_f32 (mean_over_valid likewise), the others are for the backward call; row_loss, row_lse [rows] fp32.
  * Backward: gradients of grad_out[0] (device scalar) * loss in the tensors' type, dense: dhidden [rows][width], dweight
- * [vocab][width], dbias [vocab]; each may be NULL.  fp32 products are fp32-accurate (a gradient to 2^-38 of the largest magnitude of
- * weight and hidden, too); magnitudes of fp32 hidden and weight below 2^74.
+ * [vocab][width], dbias [vocab]; each may be NULL.  fp32 operands are multiplied with 22 bits of each value, less below 2^-17 of the largest
+ * they are scaled by (down to 2^-39 of it): a row of hidden and of weight by its own largest value for the logits, all of them by one for
+ * the gradients; a word's softmax values by their own largest for dweight, so that a word of small probability everywhere keeps its gradient.
+ * Magnitudes of fp32 hidden and weight below 2^74.
  * ws: icap_linear_ce_ws_bytes(dtype, rows, width, vocab, backward) bytes, 16-byte aligned: at most 256 MB, fp32 partial results and
  * copies of hidden and weight, whatever the vocabulary (but 256 words are worked on at once, however many rows). */
 long long icap_linear_ce_out_floats(int dtype, int rows, int vocab);
