@@ -171,7 +171,7 @@ __device__ __forceinline__ typename Vec<T>::x8 acc_frag(const f32x16& a, int hal
     else return __builtin_convertvector(x, typename Vec<T>::x8);
 }
 
-// dS in two parts, high and low (16-bit types; 16 bits and more of each value): its terms differ in sign, so that one rounded part made
+// dS in two parts, high and low (16-bit types; 16 bits and more of each value, of bf16; of fp16 see lift below): its terms differ in sign, so that one rounded part made
 // dQ and dK 1.53 times as far off as rounding the exact results does; two: 1.17 times, the rest from O's own rounding in delta.  The
 // second product costs 8 % of a training pass (222 -> 241 us, 8 bf16 sequences of up to 2048 tokens, dim 64) to 19 % (dim 128).
 template <typename T>
@@ -189,6 +189,31 @@ __device__ __forceinline__ void acc_parts(const f32x16& a, int half, typename Ve
         y = __builtin_convertvector(hi, f32x8);
     }
     lo = __builtin_convertvector(x - y, typename Vec<T>::x8);
+}
+
+// fp16 ends at 2^-24 and at 65504, and dS, a weight times an output gradient, at neither: over 4096 keys and gradients of 1e-3 it is some 2e-6, of
+// which the two parts held 5 bits.  So a column's dS (its row's in dQ, its key's in dK) are multiplied by a power of two, which the
+// column's accumulators then have, too.  It starts at 2^100 and is lowered when a value would pass 2^15: the largest so far is at 2^8
+// and above, and values down to 2^-11 of it have all 22 bits.  Backward pass of 8 fp16 sequences of up to 2048 tokens, dim 64: 155 -> 164 us, dim 128
+// up to 9 %; with a loss scale under which dS passed 65504, and every such row was formed once more (below), 13.5 ms -> 165 us.
+constexpr float LIFT0 = 0x1p100f;
+__device__ __forceinline__ float inverse_of(float f) { return __uint_as_float((254u << 23) - __float_as_uint(f)); }         // of a power of two
+template <int ND>
+__device__ __forceinline__ void lift(f32x16& s, float& f, f32x16 (&acc)[ND]) {
+    float most = fabsf(s[0]);
+#pragma unroll
+    for (int e = 1; e < 16; ++e) most = fmaxf(most, fabsf(s[e]));
+    const f32x2 halves = both_halves(most);
+    most = fmaxf(halves[0], halves[1]);
+    if (__any(most * f > 32768.0f)) {
+        // 2^8 over most's power of two, within 2^-119 .. 2^100
+        const float to = most * f > 32768.0f ? __uint_as_float((unsigned)cut(262 - (int)(__float_as_uint(most) >> 23), 8, 227) << 23) : f;
+        const float by = to * inverse_of(f);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] *= by;
+        f = to;
+    }
+    s *= f;
 }
 
 // fragment of a row in memory: columns 16 kk + 8 (lane / 32) .. + 7, zeros from dim on and when !ok (p stays readable)
@@ -316,7 +341,7 @@ __device__ __forceinline__ Span tile_rows(const AttnArgs& a, int key0, int key, 
 // ------------------------------------------------------------------------------------------------ values that are not finite
 // What a row does not see has the weight zero, but zero times an infinity or a NaN is not zero, and a tile's products meet the keys of
 // all its rows.  So a row (key) whose results are not all finite is formed once more, by its two lanes, from what it sees and nothing
-// else.  Slow, and never reached by finite tensors whose results are finite.
+// else.  Slow, and not reached by finite tensors whose scores, weights, dO V^T and sums are finite in fp32.
 template <int ND>
 __device__ __forceinline__ bool finite_row(const f32x16 (&x)[ND]) {
     float z = 0.f;
@@ -599,6 +624,7 @@ __global__ __launch_bounds__(RW * KG * 64, DP == 128 && (RW < 4 || sizeof(T) == 
     f32x16 dq[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) dq[d] = zeros16();
+    float factor = LIFT0;
     int buf = 0;
     for (int n0 = keys.lo; n0 < keys.hi; n0 += BN, buf ^= 1) {
         landed();
@@ -621,6 +647,7 @@ __global__ __launch_bounds__(RW * KG * 64, DP == 128 && (RW < 4 || sizeof(T) == 
                 for (int e = 0; e < 16; ++e)
                     if (acc_row(e) < lo || acc_row(e) >= hi) s[e] = 0.f;
             }
+            if constexpr (__is_same(T, _Float16)) lift(s, factor, dq);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 if constexpr (sizeof(T) == 4) {
@@ -638,6 +665,11 @@ __global__ __launch_bounds__(RW * KG * 64, DP == 128 && (RW < 4 || sizeof(T) == 
                 }
             }
         }
+    }
+    if constexpr (__is_same(T, _Float16)) {
+        factor = inverse_of(factor);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) dq[d] *= factor;
     }
     if constexpr (KG > 1) {
         join_waves<ND, KG>(dq, reinterpret_cast<float*>(staged) + rw * (64 * ND * 16) + lane, kg);
@@ -707,6 +739,7 @@ __global__ __launch_bounds__(KW * RG * 64, DP == 128 ? 1 : 2) void dkv_kernel(co
 #pragma unroll
     for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zeros16();
     const float c2 = a.scale * LOG2E;
+    float factor = LIFT0;
     int buf = 0;
     for (int r0 = rows.lo; r0 < rows.hi; r0 += BR, buf ^= 1) {
         landed();
@@ -735,6 +768,7 @@ __global__ __launch_bounds__(KW * RG * 64, DP == 128 ? 1 : 2) void dkv_kernel(co
             for (int e = 0; e < 16; ++e)
                 if (acc_row(e) < lo || acc_row(e) >= hi) s[e] = dp[e] = 0.f;
         }
+        if constexpr (__is_same(T, _Float16)) lift(dp, factor, dk);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const auto pf = acc_frag<T>(s, j);
@@ -749,6 +783,11 @@ __global__ __launch_bounds__(KW * RG * 64, DP == 128 ? 1 : 2) void dkv_kernel(co
                 if constexpr (sizeof(T) == 2) dk[d] = mma32(qt, lo, dk[d]);
             }
         }
+    }
+    if constexpr (__is_same(T, _Float16)) {
+        factor = inverse_of(factor);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) dk[d] *= factor;
     }
     if constexpr (RG > 1) {
         float* at = reinterpret_cast<float*>(tiles) + kw * (64 * ND * 16) + lane;

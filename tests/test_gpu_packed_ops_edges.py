@@ -3,7 +3,7 @@ strides, losses changed in place, gradients far from 1, words of small probabili
 import pytest
 import torch
 
-from .test_gpu_packed_ops import D, E24, rnd, within
+from .test_gpu_packed_ops import D, E24, F16, F32, TYPES, half_step, offsets, rnd, within
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +80,88 @@ def test_linear_ce_gradients_of_rare_words_one_at_a_time():
     # two sums of the same products: 3 V roundings of fp32 each, and 22 bits of every operand
     size = float((saved[1].abs().max(0)[0]).max()) / 200
     assert float((alone - dh).abs().max()) <= 2 * (3 * 400 * E24 + 2.0 ** -20) * size
+
+
+# ------------------------------------------------------------------------------------------------ gradients far from 1
+def backward_oracle(q, k, v, g, out, lse, causal, scale):
+    """The backward formula in 64 bits from the forward call's own results (their rounding is not the backward call's), one text.
+    Bounds: P rounded once, 16 bits of each dS, fp32 sums; nothing that grows with the text but the sums' own roundings."""
+    u = half_step(q.dtype)
+    up, uds = (0.0, 0.0) if q.dtype == F32 else (u, 2.0 ** -16)
+    tiny = 2.0 ** -25 if q.dtype == F16 else 0.0
+    n, H, dim = q.shape
+    K = k.shape[1]
+    r = {"dq": torch.zeros(q.shape, dtype=torch.float64), "dk": torch.zeros(k.shape, dtype=torch.float64), "dv": torch.zeros(k.shape, dtype=torch.float64)}
+    b = {m: torch.zeros_like(x) for m, x in r.items()}
+    q, k, v, g, out, lse = (x.double() for x in (q, k, v, g, out, lse))
+    for h in range(H):
+        c = h // (H // K)
+        Q, KK, V, G, O = q[:, h], k[:, c], v[:, c], g[:, h], out[:, h]
+        s = scale * Q @ KK.t()
+        P = torch.exp(s - lse[:, h:h + 1])
+        if causal:
+            P = P.tril()
+        e_s = float(scale * (dim + 8) * E24 * (Q.abs() @ KK.abs().t()).max()) + 2.0 ** -21 + 4 * E24 * float(lse[:, h].abs().max())
+        dS = P * (G @ V.t() - (G * O).sum(1, keepdim=True))
+        E = (uds + 3 * e_s + 4 * E24) * dS.abs() + P * (dim + 8) * E24 * (G.abs() @ V.abs().t() + (G.abs() * O.abs()).sum(1, keepdim=True))
+        f = (n + 16) * E24
+        r["dq"][:, h] = scale * dS @ KK
+        b["dq"][:, h] = scale * ((E + f * dS.abs() + 2.0 ** -32 * dS.abs().amax(1, keepdim=True)) @ KK.abs()) * 1.01
+        f = (n * (H // K) + 16) * E24
+        r["dk"][:, c] += scale * dS.t() @ Q
+        b["dk"][:, c] += scale * ((E + f * dS.abs() + 2.0 ** -32 * dS.abs().amax(0)).t() @ Q.abs()) * 1.01
+        r["dv"][:, c] += P.t() @ G
+        # weights of fp16 keep their 11 bits down to 2^-28
+        b["dv"][:, c] += ((up + f + 3 * e_s) * P + (2.0 ** -39 if tiny else 0.0)).t() @ G.abs() * 1.01
+    return {m: (r[m], b[m] + u * r[m].abs() * (1 + 2.0 ** -6) + tiny * 1.01 + 1e-30) for m in r}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,causal", [(1500, False), (1500, True), (70, True), (4096, False)])
+@pytest.mark.parametrize("size", [1e-3, 1.0])
+def test_attention_gradients_of_small_weights(dtype, n, causal, size):
+    """Attention spread over a long text, and small output gradients: every weight, and every dS, is far below 1."""
+    from image_captioning_amd import ops, train_ops as T
+    H, K, dim = (2, 1, 64) if n < 4000 else (1, 1, 32)
+    q, k, v, g = (rnd(n, h, dim, seed=s, scale=c, dtype=dtype) for h, s, c in ((H, 1, 0.5), (K, 2, 0.5), (K, 3, 1.0), (H, 4, size)))
+    dev, cu = [x.to(D) for x in (q, k, v)], offsets([n]).to(D)
+    out, lse = ops.attention_packed(*dev, cu, causal=causal, want_lse=True)
+    got = T.attention_packed_bwd(g.to(D), *dev, out, lse, cu, causal=causal)
+    want = backward_oracle(q, k, v, g, out.cpu(), lse.cpu(), causal, dim ** -0.5)
+    for name, x in zip(("dq", "dk", "dv"), got):
+        within(x, *want[name], name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [70, 1100])
+def test_attention_gradients_of_large_values(dtype, n):
+    """A large loss scale: dS passes fp16's largest value, the gradients do not."""
+    from image_captioning_amd import ops, train_ops as T
+    q, k, v, g = (rnd(n, 2, 64, seed=s, scale=c, dtype=dtype) for s, c in ((1, 0.02), (2, 0.02), (3, 4.0), (4, 8e3)))
+    dev, cu = [x.to(D) for x in (q, k, v)], offsets([n]).to(D)
+    out, lse = ops.attention_packed(*dev, cu, want_lse=True)
+    got = T.attention_packed_bwd(g.to(D), *dev, out, lse, cu)
+    want = backward_oracle(q, k, v, g, out.cpu(), lse.cpu(), True, 0.125)
+    dP = g[:, 0].double() @ v[:, 0].double().t()
+    assert float((dP / torch.arange(1, n + 1, dtype=torch.float64)[:, None]).tril().abs().max()) > 65504
+    assert max(float(w.abs().max()) for w, _ in want.values()) < 65504
+    for name, x in zip(("dq", "dk", "dv"), got):
+        within(x, *want[name], name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_gradients_that_grow_along_a_text(dtype):
+    """Output gradients from 1e-6 to 1e3 within one text, and rows that are zeros: what a row or key adds up spans the whole range."""
+    from image_captioning_amd import ops, train_ops as T
+    n = 700
+    q, k, v, g = (rnd(n, 2, 64, seed=s, scale=c, dtype=F32) for s, c in ((1, 0.3), (2, 0.3), (3, 1.0), (4, 1.0)))
+    g = g * torch.logspace(-6, 3, n)[:, None, None]
+    g[::50] = 0.0
+    for order in (torch.arange(n), torch.arange(n - 1, -1, -1)):
+        x = [t[order].to(dtype) if i == 3 else t.to(dtype) for i, t in enumerate((q, k, v, g))]
+        dev, cu = [t.to(D) for t in x[:3]], offsets([n]).to(D)
+        out, lse = ops.attention_packed(*dev, cu, want_lse=True)
+        got = T.attention_packed_bwd(x[3].to(D), *dev, out, lse, cu)
+        want = backward_oracle(*x, out.cpu(), lse.cpu(), True, 0.125)
+        for name, y in zip(("dq", "dk", "dv"), got):
+            within(y, *want[name], name)
