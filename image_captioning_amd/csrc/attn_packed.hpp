@@ -696,9 +696,12 @@ __global__ __launch_bounds__(RW * KG * 64, DP == 128 && (RW < 4 || sizeof(T) == 
 // KW waves of 32 keys each, RG times: the row groups take every RG-th 32 rows and are added up in LDS at the end.  The first keys of
 // a long causal sequence meet all its rows, and that chain of steps - not the sum of the work - is what a launch of few sequences
 // lasts (167 -> 109 us with two groups, before dS had two parts, 8 bf16 sequences of up to 2048 tokens, dim 64).
+// fp16: P 2^14 is rounded, which keeps 11 bits of a weight down to 2^-28 (of P itself down to 2^-14: keys that are hardly seen by many rows lost
+// their dV, 170 times its bound at weights of 1e-8); the factor comes with the row's log-sum and leaves after the loop.
 template <typename T, int DP, int KW, int RG>
 __global__ __launch_bounds__(KW * RG * 64, DP == 128 ? 1 : 2) void dkv_kernel(const AttnArgs a) {
     constexpr int NTHR = KW * RG * 64, BK = KW * 32, BR = 32 * RG, KK = DP / 16, ND = DP / 32;
+    constexpr float P_BITS = __is_same(T, _Float16) ? 14.0f : 0.0f;
     __shared__ __attribute__((aligned(1024))) T tiles[4][BR * DP];
     static_assert(RG == 1 || sizeof(tiles) >= KW * 64 * ND * 16 * 4, "one of dK, dV of a row group fits the tiles");
     T (*const sq)[BR * DP] = tiles;
@@ -719,7 +722,7 @@ __global__ __launch_bounds__(KW * RG * 64, DP == 128 ? 1 : 2) void dkv_kernel(co
         if (threadIdx.x < BR) {
             const int r = min(r0 + (int)threadIdx.x, rows.hi - 1), t = r / a.group;
             const long long at = (long long)t * a.heads + kvh * a.group + (r - t * a.group);
-            srow[buf][0][threadIdx.x] = a.lse[at] * LOG2E;
+            srow[buf][0][threadIdx.x] = a.lse[at] * LOG2E - P_BITS;
             srow[buf][1][threadIdx.x] = a.delta[at];
         }
     };
@@ -785,9 +788,10 @@ __global__ __launch_bounds__(KW * RG * 64, DP == 128 ? 1 : 2) void dkv_kernel(co
         }
     }
     if constexpr (__is_same(T, _Float16)) {
-        factor = inverse_of(factor);
+        const float p_factor = __builtin_amdgcn_exp2f(-P_BITS);
+        factor = inverse_of(factor) * p_factor;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) dk[d] *= factor;
+        for (int d = 0; d < ND; ++d) { dk[d] *= factor; dv[d] *= p_factor; }
     }
     if constexpr (RG > 1) {
         float* at = reinterpret_cast<float*>(tiles) + kw * (64 * ND * 16) + lane;

@@ -165,3 +165,22 @@ def test_attention_gradients_that_grow_along_a_text(dtype):
         want = backward_oracle(*x, out.cpu(), lse.cpu(), True, 0.125)
         for name, y in zip(("dq", "dk", "dv"), got):
             within(y, *want[name], name)
+
+
+# ------------------------------------------------------------------------------------------------ keys that are hardly seen
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [40, 512, 1500])
+def test_attention_gradients_of_keys_that_are_hardly_seen(dtype, n):
+    """Weights down to some 1e-10, in every row, and output gradients of 100: these keys' values get all of their small gradient."""
+    from image_captioning_amd import ops, train_ops as T
+    q, k, v, g = (rnd(n, 2, 64, seed=s, scale=c, dtype=dtype) for s, c in ((1, 0.3), (2, 0.3), (3, 1.0), (4, 100.0)))
+    q[:, :, 0] = 4.0
+    k[3::7, :, 0] = -8.0
+    k[4::7, :, 0] = -16.0
+    k[5::7, :, 0] = -26.0
+    dev, cu = [x.to(D) for x in (q, k, v)], offsets([n]).to(D)
+    out, lse = ops.attention_packed(*dev, cu, causal=False, want_lse=True)
+    got = T.attention_packed_bwd(g.to(D), *dev, out, lse, cu, causal=False)
+    want = backward_oracle(q, k, v, g, out.cpu(), lse.cpu(), False, 0.125)
+    for name, x in zip(("dq", "dk", "dv"), got):
+        within(x, *want[name], name)
