@@ -171,7 +171,7 @@ __device__ __forceinline__ typename Vec<T>::x8 acc_frag(const f32x16& a, int hal
     else return __builtin_convertvector(x, typename Vec<T>::x8);
 }
 
-// dS in two parts, high and low (16-bit types; 16 bits and more of each value, of bf16; of fp16 see lift below): its terms differ in sign, so that one rounded part made
+// dS in two parts, high and low (16-bit types; 16 bits and more of each value, of bf16; of fp16 see lower below): its terms differ in sign, so that one rounded part made
 // dQ and dK 1.53 times as far off as rounding the exact results does; two: 1.17 times, the rest from O's own rounding in delta.  The
 // second product costs 8 % of a training pass (222 -> 241 us, 8 bf16 sequences of up to 2048 tokens, dim 64) to 19 % (dim 128).
 template <typename T>
@@ -192,28 +192,31 @@ __device__ __forceinline__ void acc_parts(const f32x16& a, int half, typename Ve
 }
 
 // fp16 ends at 2^-24 and at 65504, and dS, a weight times an output gradient, at neither: over 4096 keys and gradients of 1e-3 it is some 2e-6, of
-// which the two parts held 5 bits.  So a column's dS (its row's in dQ, its key's in dK) are multiplied by a power of two, which the
-// column's accumulators then have, too.  It starts at 2^100 and is lowered when a value would pass 2^15: the largest so far is at 2^8
-// and above, and values down to 2^-11 of it have all 22 bits.  Backward pass of 8 fp16 sequences of up to 2048 tokens, dim 64: 155 -> 164 us, dim 128
-// up to 9 %; with a loss scale under which dS passed 65504, and every such row was formed once more (below), 13.5 ms -> 165 us.
-constexpr float LIFT0 = 0x1p100f;
-__device__ __forceinline__ float inverse_of(float f) { return __uint_as_float((254u << 23) - __float_as_uint(f)); }         // of a power of two
+// which the two parts held 5 bits.  So a column's dS (its row's in dQ, its key's in dK) are formed with a power of two, which the
+// column's accumulators then have, too.  It starts at 2^40 and is lowered when a value would pass 2^15: the largest so far is at 2^8
+// and above (or below 2^-25), and values down to 2^-11 of it have all 22 bits.  Backward pass of 8
+// fp16 sequences of up to 2048 tokens, dim 64: 155 -> 163 us, 16 of 1024, dim 128: 623 -> 707; under a loss scale with which dS passed 65504, and
+// every such row was formed once more (below), 13.5 ms -> 163 us.
+constexpr int LIFT0 = 40;
+__device__ __forceinline__ float power_of(int b) { return __uint_as_float((unsigned)(b + 127) << 23); }
+// s: dS 2^bits of 16 places
 template <int ND>
-__device__ __forceinline__ void lift(f32x16& s, float& f, f32x16 (&acc)[ND]) {
-    float most = fabsf(s[0]);
+__device__ __forceinline__ void lower(f32x16& s, int& bits, f32x16 (&acc)[ND]) {
+    float most = fabsf(s[0]), other = fabsf(s[8]);
 #pragma unroll
-    for (int e = 1; e < 16; ++e) most = fmaxf(most, fabsf(s[e]));
-    const f32x2 halves = both_halves(most);
-    most = fmaxf(halves[0], halves[1]);
-    if (__any(most * f > 32768.0f)) {
-        // 2^8 over most's power of two, within 2^-119 .. 2^100
-        const float to = most * f > 32768.0f ? __uint_as_float((unsigned)cut(262 - (int)(__float_as_uint(most) >> 23), 8, 227) << 23) : f;
-        const float by = to * inverse_of(f);
+    for (int e = 1; e < 8; ++e) { most = fmaxf(most, fabsf(s[e])); other = fmaxf(other, fabsf(s[e + 8])); }
+    most = fmaxf(most, other);
+    if (__builtin_expect(__any(most > 32768.0f), 0)) {
+        const f32x2 halves = both_halves(most);
+        most = fmaxf(halves[0], halves[1]);
+        // to 2^8 (from 2^127 at most; what is not finite stays that)
+        const int by = most > 32768.0f ? max(8 - ((int)(__float_as_uint(most) >> 23) - 127), -100 - bits) : 0;
+        const float f = power_of(by);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) acc[d] *= by;
-        f = to;
+        for (int d = 0; d < ND; ++d) acc[d] *= f;
+        s *= f;
+        bits += by;
     }
-    s *= f;
 }
 
 // fragment of a row in memory: columns 16 kk + 8 (lane / 32) .. + 7, zeros from dim on and when !ok (p stays readable)
@@ -624,7 +627,7 @@ __global__ __launch_bounds__(RW * KG * 64, DP == 128 && (RW < 4 || sizeof(T) == 
     f32x16 dq[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) dq[d] = zeros16();
-    float factor = LIFT0;
+    int bits = __is_same(T, _Float16) ? LIFT0 : 0;
     int buf = 0;
     for (int n0 = keys.lo; n0 < keys.hi; n0 += BN, buf ^= 1) {
         landed();
@@ -640,14 +643,14 @@ __global__ __launch_bounds__(RW * KG * 64, DP == 128 && (RW < 4 || sizeof(T) == 
                 dp = mma32(row_frag<T, DP>(sv[buf], kt * 32, c), gf[c], dp);
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -lse2)) * (dp[e] - delta);
+            for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, (float)bits - lse2)) * (dp[e] - delta);
             if (n1 < me.all.lo || n1 + 32 > me.all.hi) {
                 const int lo = me.mine.lo - n1 - 4 * lh, hi = me.mine.hi - n1 - 4 * lh;
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                     if (acc_row(e) < lo || acc_row(e) >= hi) s[e] = 0.f;
             }
-            if constexpr (__is_same(T, _Float16)) lift(s, factor, dq);
+            if constexpr (__is_same(T, _Float16)) lower(s, bits, dq);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 if constexpr (sizeof(T) == 4) {
@@ -667,9 +670,8 @@ __global__ __launch_bounds__(RW * KG * 64, DP == 128 && (RW < 4 || sizeof(T) == 
         }
     }
     if constexpr (__is_same(T, _Float16)) {
-        factor = inverse_of(factor);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) dq[d] *= factor;
+        for (int d = 0; d < ND; ++d) dq[d] *= power_of(-bits);
     }
     if constexpr (KG > 1) {
         join_waves<ND, KG>(dq, reinterpret_cast<float*>(staged) + rw * (64 * ND * 16) + lane, kg);
@@ -742,7 +744,7 @@ __global__ __launch_bounds__(KW * RG * 64, DP == 128 ? 1 : 2) void dkv_kernel(co
 #pragma unroll
     for (int d = 0; d < ND; ++d) dk[d] = dv[d] = zeros16();
     const float c2 = a.scale * LOG2E;
-    float factor = LIFT0;
+    int bits = __is_same(T, _Float16) ? LIFT0 : 0;
     int buf = 0;
     for (int r0 = rows.lo; r0 < rows.hi; r0 += BR, buf ^= 1) {
         landed();
@@ -755,6 +757,7 @@ __global__ __launch_bounds__(KW * RG * 64, DP == 128 ? 1 : 2) void dkv_kernel(co
             s = mma32(row_frag<T, DP>(sq[buf], mine, c), kf[c], s);
             dp = mma32(row_frag<T, DP>(sg[buf], mine, c), vf[c], dp);
         }
+        const float factor = power_of(bits);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const f32x4 l4 = *reinterpret_cast<const f32x4*>(&srow[buf][0][mine + 8 * g + 4 * lh]), d4 = *reinterpret_cast<const f32x4*>(&srow[buf][1][mine + 8 * g + 4 * lh]);
@@ -762,7 +765,8 @@ __global__ __launch_bounds__(KW * RG * 64, DP == 128 ? 1 : 2) void dkv_kernel(co
             for (int i = 0; i < 4; ++i) {
                 const int e = 4 * g + i;
                 s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c2, -l4[i]));
-                dp[e] = s[e] * (dp[e] - d4[i]);
+                if constexpr (__is_same(T, _Float16)) dp[e] = s[e] * fmaf(dp[e], factor, -d4[i] * factor);
+                else dp[e] = s[e] * (dp[e] - d4[i]);
             }
         }
         if (r1 < me.all.lo || r1 + 32 > me.all.hi) {
@@ -771,7 +775,7 @@ __global__ __launch_bounds__(KW * RG * 64, DP == 128 ? 1 : 2) void dkv_kernel(co
             for (int e = 0; e < 16; ++e)
                 if (acc_row(e) < lo || acc_row(e) >= hi) s[e] = dp[e] = 0.f;
         }
-        if constexpr (__is_same(T, _Float16)) lift(dp, factor, dk);
+        if constexpr (__is_same(T, _Float16)) lower(dp, bits, dk);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const auto pf = acc_frag<T>(s, j);
@@ -789,7 +793,7 @@ __global__ __launch_bounds__(KW * RG * 64, DP == 128 ? 1 : 2) void dkv_kernel(co
     }
     if constexpr (__is_same(T, _Float16)) {
         const float p_factor = __builtin_amdgcn_exp2f(-P_BITS);
-        factor = inverse_of(factor) * p_factor;
+        const float factor = power_of(-bits) * p_factor;
 #pragma unroll
         for (int d = 0; d < ND; ++d) { dk[d] *= factor; dv[d] *= p_factor; }
     }
