@@ -575,7 +575,8 @@ def adamw_tensors(params, grads, exp_avg, exp_avg_sq, step, lr, beta1=0.9, beta2
     and the place, so a step can be repeated).  All states are of one kind.
     step: from 1, one for all or a list; step_dev: int32 [1] on the device, added to step by the kernel (a step recorded in a HIP
     graph: step = 0 and the count kept there).  index: the tensors' numbers for the generator (their places in the list).
-    No parameter or state may appear twice.  A gradient that is not finite spoils its value's states, with 8 bits its block's."""
+    No parameter or state may appear twice.  The parameters' version counters advance, as after any operation in place: the backward pass of a
+    graph that holds one of them from before raises.  A gradient that is not finite spoils its value's states, with 8 bits its block's."""
     n = len(params)
     if not (len(grads) == len(exp_avg) == len(exp_avg_sq) == n):
         raise N.IcapError("adamw_tensors: as many gradients and states as parameters are wanted")
@@ -636,7 +637,9 @@ def adamw_tensors(params, grads, exp_avg, exp_avg_sq, step, lr, beta1=0.9, beta2
                                        float(eps), float(weight_decay), float(grad_scale), int(seed) & (2 ** 64 - 1), _p(step_dev), _stream()),
                 "adamw_tensors")
         span.done()
-    ops.bump_weights_generation()       # the kernel writes the parameters by raw pointer: eval-mode weight caches must rebuild
+    # the kernel writes the parameters by raw pointer: eval-mode weight caches must rebuild, and a graph that has saved one must not go back
+    ops.bump_weights_generation()
+    torch.autograd.graph.increment_version(params)
 
 
 # ---------------------------------------------------------------------------- convolutional encoder

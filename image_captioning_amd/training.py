@@ -344,6 +344,7 @@ class AdamWTensors:
 
     def advance_recorded(self, replays: int) -> None:
         ops.bump_weights_generation()
+        torch.autograd.graph.increment_version([p for p in self.params if p.grad is not None])
         self.param_steps = [s + replays * (p.grad is not None) for s, p in zip(self.param_steps, self.params)]
 
     def state_dict(self):

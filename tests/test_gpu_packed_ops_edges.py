@@ -184,3 +184,23 @@ def test_attention_gradients_of_keys_that_are_hardly_seen(dtype, n):
     want = backward_oracle(q, k, v, g, out.cpu(), lse.cpu(), False, 0.125)
     for name, x in zip(("dq", "dk", "dv"), got):
         within(x, *want[name], name)
+
+
+# ------------------------------------------------------------------------------------------------ the graph knows of the update
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_tensors_tells_autograd_that_parameters_changed(bits):
+    """A graph kept across a step holds values that are no longer there: its backward pass is refused, as after torch's optimizers."""
+    from image_captioning_amd import training
+    w, left = (torch.nn.Parameter(rnd(8, 64, seed=s).to(D)) for s in (1, 2))
+    opt = training.AdamWTensors([w, left], lr=1e-2, state_bits=bits)
+    h, t = rnd(5, 64, seed=3).to(D), torch.tensor([0, 1, 2, 3, 4], device=D)
+    kept, other = training.linear_cross_entropy(h, w, None, t), (left * left).sum()
+    w.grad = torch.ones_like(w)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.backward()
+    other.backward()                                         # it had no gradient and was left alone
+    kept = training.linear_cross_entropy(h, w, None, t)
+    opt.advance_recorded(1)                                  # a replay has written the parameters
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.backward()
