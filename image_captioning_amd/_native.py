@@ -201,6 +201,7 @@ SIGNATURES = {
     "icap_linear_ce_ws_bytes": (_ll, [_i] * 5),
     "icap_linear_ce_out_floats": (_ll, [_i] * 3),
     "icap_linear_ce_fwd": (_i, [_i, _p, _ll, _p, _ll, _p, _p, _i, _i, _i, _ll, _i, _p, _p, _p, _p, _ll, _p]),
+    "icap_linear_ce_loss_fwd": (_i, [_i, _p, _ll, _p, _ll, _p, _p, _i, _i, _i, _ll, _i, _p, _p, _p, _p, _p, _ll, _p]),
     "icap_linear_ce_bwd": (_i, [_i, _p, _ll, _p, _ll, _p, _p, _i, _i, _i, _ll] + [_p] * 7 + [_ll, _p]),
     "icap_adamw_tensors": (_i, [_i] + [_p] * 9 + [_i] * 3 + [_d] * 6 + [C.c_ulonglong, _p, _p]),
 }

@@ -205,7 +205,7 @@ static inline long long align4(long long n) { return (n + 3) & ~3LL; }
 long long linear_ce_ws_bytes(int, int, int, int, int);
 long long linear_ce_out_floats(int, int, int);
 int linear_ce_fwd(int, const void*, long long, const void*, long long, const void*, const long long*, int, int, int, long long, int, float*, float*,
-                  float*, void*, long long, hipStream_t);
+                  float*, float*, void*, long long, hipStream_t);
 int linear_ce_bwd(int, const void*, long long, const void*, long long, const void*, const long long*, int, int, int, long long, const float*,
                   const float*, const float*, void*, void*, void*, void*, long long, hipStream_t);
 int adamw_tensors(int, void* const*, const void* const*, void* const*, void* const*, float* const*, float* const*, const long long*, const int*,
@@ -1151,8 +1151,16 @@ long long icap_linear_ce_ws_bytes(int dtype, int rows, int width, int vocab, int
 int icap_linear_ce_fwd(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias, const long long* targets,
                        int rows, int width, int vocab, long long ignore_index, int mean_over_valid, float* row_loss, float* row_lse, float* out,
                        void* ws, long long ws_bytes, void* stream) {
-    return linear_ce_fwd(dtype, hidden, ld_h, weight, ld_w, bias, targets, rows, width, vocab, ignore_index, mean_over_valid, row_loss, row_lse, out, ws,
-                         ws_bytes, (hipStream_t)stream);
+    return linear_ce_fwd(dtype, hidden, ld_h, weight, ld_w, bias, targets, rows, width, vocab, ignore_index, mean_over_valid, row_loss, row_lse, nullptr,
+                         out, ws, ws_bytes, (hipStream_t)stream);
+}
+
+int icap_linear_ce_loss_fwd(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
+                            const long long* targets, int rows, int width, int vocab, long long ignore_index, int mean_over_valid,
+                            float* row_loss, float* row_lse, float* loss, float* out, void* ws, long long ws_bytes, void* stream) {
+    if (!loss) { set_error("linear_ce_loss_fwd: null loss"); return ICAP_ERR_ARG; }
+    return linear_ce_fwd(dtype, hidden, ld_h, weight, ld_w, bias, targets, rows, width, vocab, ignore_index, mean_over_valid, row_loss, row_lse, loss,
+                         out, ws, ws_bytes, (hipStream_t)stream);
 }
 
 int icap_linear_ce_bwd(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias, const long long* targets,

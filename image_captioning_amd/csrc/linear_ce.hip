@@ -484,7 +484,7 @@ __device__ __forceinline__ float block_max(const float* x, int n, float* red) {
 
 // loss (its sum in 64 bits) and the scale of every row; fp32 (urow, ucol): the scales of whole tensors, from those of their rows
 __global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const long long* targets, int R, int V, long long ignore, int mean_over_valid,
-                                                    const float* urow, const float* ucol, float* out) {
+                                                    const float* urow, const float* ucol, float* loss, float* out) {
     __shared__ double ss[16];
     __shared__ int sc[16];
     if (urow) {
@@ -509,6 +509,7 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* row_loss, const
         for (int i = 0; i < 16; ++i) { sum += ss[i]; cnt += sc[i]; }
         const int over = mean_over_valid ? cnt : R;
         out[0] = over > 0 ? (float)(sum / over) : 0.f;
+        if (loss) *loss = out[0];
         out[1] = over > 0 ? 1.0f / (float)over : 0.f;
     }
 }
@@ -856,7 +857,7 @@ Gemm logits(const Call& c, const Plan<T>& p, const float* out, int v0, int vn) {
 }
 
 template <typename T>
-int fwd(const Call& c, int mean_over_valid, float* row_loss, float* row_lse, float* out, char* ws, hipStream_t st) {
+int fwd(const Call& c, int mean_over_valid, float* row_loss, float* row_lse, float* loss, float* out, char* ws, hipStream_t st) {
     typedef typename Of<T>::E E;
     Plan<T> p(c, false, ws);
     operands<T>(c, p, out, false, false, st);
@@ -864,7 +865,7 @@ int fwd(const Call& c, int mean_over_valid, float* row_loss, float* row_lse, flo
     g.part = p.part; g.strips = p.strips; g.target_logit = p.target_logit;
     if (int rc = gemm<E, T, EP_LSE>(g, p.s_logit, st)) return rc;
     hipLaunchKernelGGL(lse_kernel, dim3((c.R + 3) / 4), dim3(256), 0, st, p.part, p.strips, p.target_logit, c.targets, c.R, c.V, c.ignore, row_loss, row_lse);
-    hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, c.targets, c.R, c.V, c.ignore, mean_over_valid, g.urow, g.ucol, out);
+    hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(1024), 0, st, row_loss, c.targets, c.R, c.V, c.ignore, mean_over_valid, g.urow, g.ucol, loss, out);
     return launch_status("linear_ce_fwd");
 }
 
@@ -975,7 +976,7 @@ long long linear_ce_ws_bytes(int dtype, int R, int E, int V, int backward) {
 long long linear_ce_out_floats(int dtype, int R, int V) { return R <= 0 || V <= 0 ? 0 : lce::out_floats(dtype, R, V); }
 
 int linear_ce_fwd(int dtype, const void* h, long long ld_h, const void* w, long long ld_w, const void* bias, const long long* targets, int R, int E,
-                  int V, long long ignore, int mean_over_valid, float* row_loss, float* row_lse, float* out, void* ws, long long ws_bytes,
+                  int V, long long ignore, int mean_over_valid, float* row_loss, float* row_lse, float* loss, float* out, void* ws, long long ws_bytes,
                   hipStream_t st) {
     const lce::Call c{h, w, bias, ld_h, ld_w, targets, R, E, V, ignore};
     if (int rc = lce::check(dtype, c, "linear_ce_fwd")) return rc;
@@ -983,9 +984,9 @@ int linear_ce_fwd(int dtype, const void* h, long long ld_h, const void* w, long 
         set_error("linear_ce_fwd: null result, results or a workspace that are unaligned, or a workspace that is null or too small");
         return ICAP_ERR_ARG;
     }
-    if (dtype == DT_F32) return lce::fwd<float>(c, mean_over_valid, row_loss, row_lse, out, (char*)ws, st);
-    if (dtype == DT_BF16) return lce::fwd<__bf16>(c, mean_over_valid, row_loss, row_lse, out, (char*)ws, st);
-    return lce::fwd<_Float16>(c, mean_over_valid, row_loss, row_lse, out, (char*)ws, st);
+    if (dtype == DT_F32) return lce::fwd<float>(c, mean_over_valid, row_loss, row_lse, loss, out, (char*)ws, st);
+    if (dtype == DT_BF16) return lce::fwd<__bf16>(c, mean_over_valid, row_loss, row_lse, loss, out, (char*)ws, st);
+    return lce::fwd<_Float16>(c, mean_over_valid, row_loss, row_lse, loss, out, (char*)ws, st);
 }
 
 int linear_ce_bwd(int dtype, const void* h, long long ld_h, const void* w, long long ld_w, const void* bias, const long long* targets, int R, int E,

@@ -499,15 +499,17 @@ def linear_ce_fwd(hidden, weight, bias, targets, ignore_index=-100, mean_over_va
         raise N.IcapError("linear_ce: targets must be contiguous")
     lib, dev, code = N.load(), hidden.device, DTYPE_CODES[hidden.dtype]
     rows = torch.empty((2, R), device=dev, dtype=torch.float32)
+    # the loss is no part of what the backward call reads: its owner may change it in place, and does not keep the rest alive with it
+    value = torch.empty((), device=dev, dtype=torch.float32)
     out = torch.empty(lib.icap_linear_ce_out_floats(code, R, V), device=dev, dtype=torch.float32)
     nbytes = lib.icap_linear_ce_ws_bytes(code, R, E, V, 0)
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
     span = _Span("linear_ce_fwd", (R, E, V, str(hidden.dtype)))
-    N.check(lib.icap_linear_ce_fwd(code, hidden.data_ptr(), ld_h, weight.data_ptr(), ld_w, _p(bias), targets.data_ptr(), R, E, V, int(ignore_index),
-                                   int(bool(mean_over_valid)), rows[0].data_ptr(), rows[1].data_ptr(), out.data_ptr(), ws.data_ptr(), nbytes,
-                                   _stream()), "linear_ce_fwd")
+    N.check(lib.icap_linear_ce_loss_fwd(code, hidden.data_ptr(), ld_h, weight.data_ptr(), ld_w, _p(bias), targets.data_ptr(), R, E, V,
+                                        int(ignore_index), int(bool(mean_over_valid)), rows[0].data_ptr(), rows[1].data_ptr(), value.data_ptr(),
+                                        out.data_ptr(), ws.data_ptr(), nbytes, _stream()), "linear_ce_fwd")
     span.done()
-    return out[0], rows[0], (hidden, weight, bias, targets, int(ignore_index), rows, out) if want_grad else None
+    return value, rows[0], (hidden, weight, bias, targets, int(ignore_index), rows, out) if want_grad else None
 
 
 def linear_ce_bwd(grad_out, saved, need=(True, True, True)):

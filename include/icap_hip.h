@@ -872,6 +872,10 @@ long long icap_linear_ce_ws_bytes(int dtype, int rows, int width, int vocab, int
 int icap_linear_ce_fwd(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
                        const long long* targets, int rows, int width, int vocab, long long ignore_index, int mean_over_valid,
                        float* row_loss, float* row_lse, float* out, void* ws, long long ws_bytes, void* stream);
+/* The same with the loss written to *loss as well: a value of its own, which its owner may change or keep whatever becomes of out. */
+int icap_linear_ce_loss_fwd(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
+                            const long long* targets, int rows, int width, int vocab, long long ignore_index, int mean_over_valid,
+                            float* row_loss, float* row_lse, float* loss, float* out, void* ws, long long ws_bytes, void* stream);
 int icap_linear_ce_bwd(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,
                        const long long* targets, int rows, int width, int vocab, long long ignore_index, const float* row_lse,
                        const float* out, const float* grad_out, void* dhidden, void* dweight, void* dbias, void* ws,

@@ -204,3 +204,23 @@ def test_adamw_tensors_tells_autograd_that_parameters_changed(bits):
     opt.advance_recorded(1)                                  # a replay has written the parameters
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         kept.backward()
+
+
+# ------------------------------------------------------------------------------------------------ the loss as a tensor of its own
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_cross_entropy_changed_in_place(dtype):
+    """loss /= steps, loss *= and loss += before the backward pass, as accumulation loops write them."""
+    from image_captioning_amd import training
+    h, w = rnd(30, 64, seed=1, dtype=dtype).to(D).requires_grad_(), rnd(90, 64, seed=2, scale=0.2, dtype=dtype).to(D).requires_grad_()
+    t = torch.randint(0, 90, (30,), generator=torch.Generator().manual_seed(3)).to(D)
+    want = torch.autograd.grad(training.linear_cross_entropy(h, w, None, t) * 0.25, (h, w))
+    value = training.linear_cross_entropy(h, w, None, t)
+    before = float(value.detach())
+    value /= 4
+    value += 1.0
+    value -= 1.0
+    assert abs(float(value.detach()) - before / 4) <= 4 * E24 * (before + 1)
+    for x, y in zip(torch.autograd.grad(value, (h, w)), want):
+        assert torch.equal(x, y)
+    # what a training loop collects keeps one value alive, not what the backward call reads
+    assert training.linear_cross_entropy(h, w, None, t).detach().untyped_storage().nbytes() <= 64
