@@ -66,7 +66,7 @@ class _MaskedCE(torch.autograd.Function):
                                               out.data_ptr(), _stream()), "ce_loss_fwd")
         ctx.save_for_backward(pred, tg, row_lse, out)
         ctx.geom = (R, V, ld, gr, gs, int(ignore_index))
-        return out[0]
+        return out[0].data          # no view of what is saved: `loss /= n` changes out[0], which the backward call does not read
 
     @staticmethod
     def backward(ctx, grad_out):
