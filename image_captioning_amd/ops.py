@@ -1031,13 +1031,19 @@ def _ckd(t, name, dtype=None, shape=None):
 
 def _packed_rows(t):
     """t [tokens, heads, dim] as the attention kernels read it (last axis contiguous, 16-byte aligned rows; a slice of a fused
-    projection is), a contiguous copy otherwise."""
+    projection is), a dense copy otherwise."""
     per = 16 // t.element_size()
-    if (t.stride(2) == 1 and t.stride(0) % per == 0 and t.stride(1) % per == 0 and t.data_ptr() % 16 == 0 and t.stride(0) <= 1 << 24
-            and t.stride(1) * t.size(1) <= 1 << 30):
-        return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+    def read_in_place(a, b):
+        return a % per == 0 and b % per == 0 and a <= 1 << 24 and b * t.size(1) <= 1 << 30
+    if t.stride(2) == 1 and t.data_ptr() % 16 == 0:
+        if read_in_place(t.stride(0), t.stride(1)):
+            return t
+        # nobody steps along an axis of size 1, whatever its stride
+        a, b = (t.stride(i) if t.size(i) > 1 else 0 for i in (0, 1))
+        if read_in_place(a, b):
+            return t.as_strided(t.shape, (a, b, 1))
+    return torch.empty(t.shape, device=t.device, dtype=t.dtype).copy_(t)        # contiguous() keeps such a stride
 
 
 def _packed_args(q, k, v, cu_q, cu_k, what):

@@ -236,3 +236,38 @@ def test_loss_on_stored_logits_changed_in_place():
         value /= 4
         got, = torch.autograd.grad(value, x)
         assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------------------------------------ strides of axes of size one
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("at", [slice(0, 1), slice(1, 2), slice(7, 8)])
+def test_attention_of_one_token_of_an_odd_projection(dtype, at):
+    """One token sliced from rows of an odd width: its token stride is no multiple of 16 bytes, and belongs to an axis of size 1."""
+    from image_captioning_amd import ops, train_ops as T
+    H, K, dim = 4, 2, 32
+    buf = rnd(8, (H + 2 * K) * dim + 3, seed=1, dtype=dtype).to(D)
+    q, k, v = (t.unflatten(1, (-1, dim)) for t in buf[:, :(H + 2 * K) * dim].split((H * dim, K * dim, K * dim), 1))
+    g = rnd(8, H * dim + 5, seed=2, dtype=dtype).to(D)[:, :H * dim].unflatten(1, (H, dim))
+    one, all8 = offsets([1]).to(D), offsets([8]).to(D)
+    for args, cu in (((q[at], k[at], v[at]), (one, one)), ((q[at], k, v), (one, all8))):
+        dense = [torch.empty(t.shape, device=D, dtype=dtype).copy_(t) for t in args]
+        got, want = ops.attention_packed(*args, *cu, want_lse=True), ops.attention_packed(*dense, *cu, want_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        for x, y in zip(T.attention_packed_bwd(g[at], *args, *got, *cu), T.attention_packed_bwd(g[at].clone(memory_format=torch.contiguous_format), *dense, *want, *cu)):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_of_one_head_and_of_rows_far_apart(dtype):
+    """One key head of a tensor with an odd head stride; the last token of a text whose rows lie further apart than a stride may be."""
+    from image_captioning_amd import ops
+    dim, n = 16, 9
+    heads = rnd(n * dim + 8, seed=3, dtype=dtype).to(D)
+    q = heads.as_strided((n, 1, dim), (dim, dim + 1, 1))
+    cu = offsets([n]).to(D)
+    dense = torch.empty(q.shape, device=D, dtype=dtype).copy_(q)
+    assert torch.equal(ops.attention_packed(q, q, q, cu), ops.attention_packed(dense, dense, dense, cu))
+    far = rnd(dim, seed=4, dtype=dtype).to(D).as_strided((1, 1, dim), ((1 << 24) + 16, dim, 1))
+    one = offsets([1]).to(D)
+    dense = torch.empty(far.shape, device=D, dtype=dtype).copy_(far)
+    assert torch.equal(ops.attention_packed(far, far, far, one), ops.attention_packed(dense, dense, dense, one))

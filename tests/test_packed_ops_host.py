@@ -1,6 +1,9 @@
 """CPU: what the packed attention, the vocabulary loss and the many-tensor update do before anything touches a device, at the edges of
 what they take."""
-from image_captioning_amd import _native as N
+import pytest
+import torch
+
+from image_captioning_amd import _native as N, ops
 
 
 def test_linear_ce_loss_forward_refuses():
@@ -8,3 +11,22 @@ def test_linear_ce_loss_forward_refuses():
     good = dict(dtype=1, h=16, ldh=64, w=16, ldw=64, b=None, t=16, R=4, E=64, V=100, ign=-100, mean=1, rl=16, lse=16, loss=16, out=16, ws=16, nbytes=1 << 40)
     for kw, code in ((dict(loss=None), 1), (dict(out=None), 1), (dict(out=24), 1), (dict(ws=None), 1), (dict(R=0), 1), (dict(dtype=5), 1), (dict(V=65535 * 64 + 1), 3)):
         assert lib.icap_linear_ce_loss_fwd(*{**good, **kw}.values(), None) == code, kw
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_packed_rows_are_readable_whatever_the_layout(dtype):
+    """Strides that are multiples of 16 bytes and within the limits, an aligned address, the same values; in place where that is possible."""
+    per = 16 // torch.empty((), dtype=dtype).element_size()
+    base = torch.arange(8 * 131 + 64).to(dtype)
+    base = base[(-base.data_ptr() % 16) // base.element_size():]
+    odd = base[:8 * 131].view(8, 131)[:, :128].unflatten(1, (4, 32))
+    wide = base[:8 * 128].view(8, 4, 32)
+    cases = [(odd, False), (odd[:3], False), (odd[:1], True), (odd[1:2], False), (odd[4:5], False), (odd.split([1, 7])[0], True), (wide, True), (wide[:, 1:3], True),
+             (wide[2:3, 1:2], True), (wide[:0], True), (wide.transpose(0, 1), True), (wide[:, :, ::2], False), (wide[:, :, per // 2:per // 2 + 24], False), (wide[:, :, 8:24], True),
+             (base.as_strided((9, 1, 16), (16, 17, 1)), True), (base.as_strided((1, 2, 16), ((1 << 24) + 16, 16, 1)), True),
+             (base.as_strided((1, 1, 16), (3, 5, 1)), True), (wide[:, :1].expand(8, 6, 32), True), (base[:1].expand(4, 2, 8), False)]
+    for t, in_place in cases:
+        got = ops._packed_rows(t)
+        assert torch.equal(got, t) and (got.data_ptr() == t.data_ptr()) == in_place
+        assert got.stride(2) == 1 and got.data_ptr() % 16 == 0 and all(x % per == 0 for x in got.stride()[:2])
+        assert got.stride(0) <= 1 << 24 and got.stride(1) * got.size(1) <= 1 << 30
