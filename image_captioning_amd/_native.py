@@ -199,6 +199,7 @@ SIGNATURES = {
     "icap_attention_packed_fwd": (_i, [_i] + [_p] * 7 + [_i] * 6 + [_ll] * 6 + [_f, _i, _p, _ll, _p]),
     "icap_attention_packed_bwd": (_i, [_i] + [_p] * 11 + [_i] * 6 + [_ll] * 8 + [_f, _i, _p, _p]),
     "icap_linear_ce_ws_bytes": (_ll, [_i] * 5),
+    "icap_linear_ce_ws_bytes_for": (_ll, [_i, _p, _ll, _p, _ll] + [_i] * 4),
     "icap_linear_ce_out_floats": (_ll, [_i] * 3),
     "icap_linear_ce_fwd": (_i, [_i, _p, _ll, _p, _ll, _p, _p, _i, _i, _i, _ll, _i, _p, _p, _p, _p, _ll, _p]),
     "icap_linear_ce_loss_fwd": (_i, [_i, _p, _ll, _p, _ll, _p, _p, _i, _i, _i, _ll, _i, _p, _p, _p, _p, _p, _ll, _p]),

@@ -203,6 +203,7 @@ static inline long long align4(long long n) { return (n + 3) & ~3LL; }
     } while (0)
 
 long long linear_ce_ws_bytes(int, int, int, int, int);
+long long linear_ce_ws_bytes_for(int, const void*, long long, const void*, long long, int, int, int, int);
 long long linear_ce_out_floats(int, int, int);
 int linear_ce_fwd(int, const void*, long long, const void*, long long, const void*, const long long*, int, int, int, long long, int, float*, float*,
                   float*, float*, void*, long long, hipStream_t);
@@ -1146,6 +1147,11 @@ long long icap_linear_ce_out_floats(int dtype, int rows, int vocab) { return lin
 
 long long icap_linear_ce_ws_bytes(int dtype, int rows, int width, int vocab, int backward) {
     return linear_ce_ws_bytes(dtype, rows, width, vocab, backward);
+}
+
+long long icap_linear_ce_ws_bytes_for(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, int rows, int width, int vocab,
+                                      int need) {
+    return linear_ce_ws_bytes_for(dtype, hidden, ld_h, weight, ld_w, rows, width, vocab, need);
 }
 
 int icap_linear_ce_fwd(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias, const long long* targets,

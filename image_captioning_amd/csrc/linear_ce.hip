@@ -706,7 +706,9 @@ struct Call {
     const long long* targets;
     int R, E, V;
     long long ignore;
+    int need = 0;                       // the backward call's results that are wanted; 0: the forward call
 };
+enum { NEED_DH = 1, NEED_DW = 2, NEED_DB = 4 };
 
 // Bytes of D that a piece of the vocabulary may take.  The last-level cache holds 256 MB: up to there in one piece (131 MB at 4864 rows x 6756
 // words: 609 us, in two pieces 676), otherwise in pieces of half of it, beside which the operands stay (8192 x 65536, 1 GB: 8436 us,
@@ -727,9 +729,9 @@ struct Operand {
     long long ld = 0;
 };
 
-// room for them; Rp: rows with those that are zeros
+// room for them; Rp: rows with those that are zeros; sums: those planes are wanted
 template <typename T>
-Operand<T> room(Space& ws, const void* x, long long ld, int Rp, int C, bool backward, bool is_direct) {
+Operand<T> room(Space& ws, const void* x, long long ld, int Rp, int C, bool sums, bool is_direct) {
     typedef typename Of<T>::E E;
     Operand<T> o;
     o.ld = up(C, 64);
@@ -737,7 +739,8 @@ Operand<T> room(Space& ws, const void* x, long long ld, int Rp, int C, bool back
     else o.row0 = ws.take<E>(Rp * o.ld);
     if (Of<T>::planes == 2) o.row1 = ws.take<E>(Rp * o.ld);
     o.sum0 = o.row0;
-    if (Of<T>::planes == 2 && backward) { o.sum0 = ws.take<E>(Rp * o.ld); o.sum1 = ws.take<E>(Rp * o.ld); }
+    if (Of<T>::planes == 2) o.sum0 = nullptr;
+    if (Of<T>::planes == 2 && sums) { o.sum0 = ws.take<E>(Rp * o.ld); o.sum1 = ws.take<E>(Rp * o.ld); }
     return o;
 }
 
@@ -759,14 +762,16 @@ struct Plan {
     Shape s_top, s_logit, s_h, s_w;
     long long bytes;
 
-    Plan(const Call& c, bool backward, char* base) {
+    // any: whatever the addresses and row distances
+    Plan(const Call& c, char* base, bool any = false) {
         typedef typename Of<T>::E E;
+        const bool backward = c.need != 0, dh = c.need & NEED_DH, dw = c.need & NEED_DW;
         Space ws{base};
         h_direct = !backward && direct<T>(c.h, c.ld_h, c.E);        // dW needs zeros in the rows that are left out
         w_direct = direct<T>(c.w, c.ld_w, c.E) && (!backward || c.V % 64 == 0);          // dh reads whole K tiles of words
-        if (!base) h_direct = w_direct = false;             // the size is asked for without pointers: the larger of the two
-        h = room<T>(ws, c.h, c.ld_h, backward ? (int)up(c.R, 64) : c.R, c.E, backward, h_direct);
-        w = room<T>(ws, c.w, c.ld_w, backward ? (int)up(c.V, 64) : c.V, c.E, backward, w_direct);
+        if (any) h_direct = w_direct = false;
+        h = room<T>(ws, c.h, c.ld_h, backward ? (int)up(c.R, 64) : c.R, c.E, dw, h_direct);
+        w = room<T>(ws, c.w, c.ld_w, backward ? (int)up(c.V, 64) : c.V, c.E, dh, w_direct);
         const int pairs = Of<T>::planes == 2 ? 3 : 1;
         if (!backward) {
             s_logit = shape_of(c.R, c.V, up(c.E, 64) / 64 * pairs, false);
@@ -788,9 +793,9 @@ struct Plan {
             s_h = shape_of(c.R, c.E, ldd / 64 * pairs, true);
             s_w = shape_of(piece, c.E, rp / 64 * pairs, true);
             // the largest values of D's columns, once they have become factors, make room for the columns' sums
-            int blocks = s_logit.tiles_m * 2;
+            int blocks = c.need & NEED_DB ? s_logit.tiles_m * 2 : 0;
             lift = norm_h = norm_w = nullptr;
-            if (Of<T>::planes == 2) {
+            if (Of<T>::planes == 2 && dw) {
                 s_top = shape_of(c.R, c.V, up(c.E, 64) / 64, false);
                 if (s_top.tiles_m * 2 > blocks) blocks = s_top.tiles_m * 2;
                 lift = ws.take<float>(up(c.V, 64) + 256);       // these are read up to 256 behind the last, too
@@ -798,8 +803,8 @@ struct Plan {
                 norm_w = ws.take<float>(up(c.V, 64) + 256);
             }
             colpart = ws.take<float>((long long)blocks * c.V);
-            acc_h = ws.take<float>((s_h.splits > 1 || piece < c.V) ? (long long)s_h.splits * c.R * c.E : 0);
-            acc_w = ws.take<float>(s_w.splits > 1 ? (long long)s_w.splits * piece * c.E : 0);
+            acc_h = ws.take<float>(dh && (s_h.splits > 1 || piece < c.V) ? (long long)s_h.splits * c.R * c.E : 0);
+            acc_w = ws.take<float>(dw && s_w.splits > 1 ? (long long)s_w.splits * piece * c.E : 0);
         }
         bytes = ws.at;
     }
@@ -859,7 +864,7 @@ Gemm logits(const Call& c, const Plan<T>& p, const float* out, int v0, int vn) {
 template <typename T>
 int fwd(const Call& c, int mean_over_valid, float* row_loss, float* row_lse, float* loss, float* out, char* ws, hipStream_t st) {
     typedef typename Of<T>::E E;
-    Plan<T> p(c, false, ws);
+    Plan<T> p(c, ws);
     operands<T>(c, p, out, false, false, st);
     Gemm g = logits<T>(c, p, out, 0, c.V);
     g.part = p.part; g.strips = p.strips; g.target_logit = p.target_logit;
@@ -880,7 +885,7 @@ void join(const float* acc, int splits, long long n, T* out, const Gemm& p, hipS
 template <typename T>
 int bwd(const Call& c, const float* row_lse, const float* meta, const float* grad_out, void* dh, void* dw, void* db, char* ws, hipStream_t st) {
     typedef typename Of<T>::E E;
-    Plan<T> p(c, true, ws);
+    Plan<T> p(c, ws);
     const bool lifted = sizeof(T) == 4 && dw;
     operands<T>(c, p, const_cast<float*>(meta), true, lifted, st);         // which only reads it here
     if constexpr (sizeof(T) == 4)
@@ -966,11 +971,18 @@ static int check(int dtype, const Call& c, const char* what) {
 
 }  // namespace lce
 
+static long long plan_bytes(int dtype, const lce::Call& c, bool any) {
+    if (c.R <= 0 || c.E <= 0 || c.V <= 0) return 0;
+    if (dtype == DT_F32) return lce::Plan<float>(c, nullptr, any).bytes;
+    return lce::Plan<_Float16>(c, nullptr, any).bytes;
+}
+
 long long linear_ce_ws_bytes(int dtype, int R, int E, int V, int backward) {
-    lce::Call c{nullptr, nullptr, nullptr, E, E, nullptr, R, E, V, 0};
-    if (R <= 0 || E <= 0 || V <= 0) return 0;
-    if (dtype == DT_F32) return lce::Plan<float>(c, backward, nullptr).bytes;
-    return lce::Plan<_Float16>(c, backward, nullptr).bytes;
+    return plan_bytes(dtype, lce::Call{nullptr, nullptr, nullptr, E, E, nullptr, R, E, V, 0, backward ? 7 : 0}, true);
+}
+
+long long linear_ce_ws_bytes_for(int dtype, const void* h, long long ld_h, const void* w, long long ld_w, int R, int E, int V, int need) {
+    return plan_bytes(dtype, lce::Call{h, w, nullptr, ld_h, ld_w, nullptr, R, E, V, 0, need & 7}, false);
 }
 
 long long linear_ce_out_floats(int dtype, int R, int V) { return R <= 0 || V <= 0 ? 0 : lce::out_floats(dtype, R, V); }
@@ -980,7 +992,7 @@ int linear_ce_fwd(int dtype, const void* h, long long ld_h, const void* w, long 
                   hipStream_t st) {
     const lce::Call c{h, w, bias, ld_h, ld_w, targets, R, E, V, ignore};
     if (int rc = lce::check(dtype, c, "linear_ce_fwd")) return rc;
-    if (!row_loss || !row_lse || !out || !aligned16(out) || !ws || !aligned16(ws) || ws_bytes < linear_ce_ws_bytes(dtype, R, E, V, 0)) {
+    if (!row_loss || !row_lse || !out || !aligned16(out) || !ws || !aligned16(ws) || ws_bytes < plan_bytes(dtype, c, false)) {
         set_error("linear_ce_fwd: null result, results or a workspace that are unaligned, or a workspace that is null or too small");
         return ICAP_ERR_ARG;
     }
@@ -992,9 +1004,10 @@ int linear_ce_fwd(int dtype, const void* h, long long ld_h, const void* w, long 
 int linear_ce_bwd(int dtype, const void* h, long long ld_h, const void* w, long long ld_w, const void* bias, const long long* targets, int R, int E,
                   int V, long long ignore, const float* row_lse, const float* meta, const float* grad_out, void* dh, void* dw, void* db, void* ws,
                   long long ws_bytes, hipStream_t st) {
-    const lce::Call c{h, w, bias, ld_h, ld_w, targets, R, E, V, ignore};
+    const lce::Call c{h, w, bias, ld_h, ld_w, targets, R, E, V, ignore, (dh ? lce::NEED_DH : 0) | (dw ? lce::NEED_DW : 0) | (db ? lce::NEED_DB : 0)};
     if (int rc = lce::check(dtype, c, "linear_ce_bwd")) return rc;
-    if (!row_lse || !meta || !aligned16(meta) || !grad_out || !ws || !aligned16(ws) || ws_bytes < linear_ce_ws_bytes(dtype, R, E, V, 1)) {
+    if (c.need == 0) return ICAP_OK;
+    if (!row_lse || !meta || !aligned16(meta) || !grad_out || !ws || !aligned16(ws) || ws_bytes < plan_bytes(dtype, c, false)) {
         set_error("linear_ce_bwd: null tensor, or a workspace that is null, unaligned or too small");
         return ICAP_ERR_ARG;
     }

@@ -502,7 +502,7 @@ def linear_ce_fwd(hidden, weight, bias, targets, ignore_index=-100, mean_over_va
     # the loss is no part of what the backward call reads: its owner may change it in place, and does not keep the rest alive with it
     value = torch.empty((), device=dev, dtype=torch.float32)
     out = torch.empty(lib.icap_linear_ce_out_floats(code, R, V), device=dev, dtype=torch.float32)
-    nbytes = lib.icap_linear_ce_ws_bytes(code, R, E, V, 0)
+    nbytes = lib.icap_linear_ce_ws_bytes_for(code, hidden.data_ptr(), ld_h, weight.data_ptr(), ld_w, R, E, V, 0)
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
     span = _Span("linear_ce_fwd", (R, E, V, str(hidden.dtype)))
     N.check(lib.icap_linear_ce_loss_fwd(code, hidden.data_ptr(), ld_h, weight.data_ptr(), ld_w, _p(bias), targets.data_ptr(), R, E, V,
@@ -527,10 +527,12 @@ def linear_ce_bwd(grad_out, saved, need=(True, True, True)):
     if dh is None and dw is None and db is None:
         return None, None, None
     lib, code = N.load(), DTYPE_CODES[dtype]
-    nbytes = lib.icap_linear_ce_ws_bytes(code, R, E, V, 1)
+    ld_h, ld_w = _ce_rows(hidden, "linear_ce_bwd: hidden"), _ce_rows(weight, "linear_ce_bwd: weight", dtype)
+    nbytes = lib.icap_linear_ce_ws_bytes_for(code, hidden.data_ptr(), ld_h, weight.data_ptr(), ld_w, R, E, V,
+                                             (dh is not None) + 2 * (dw is not None) + 4 * (db is not None))
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
     span = _Span("linear_ce_bwd", (R, E, V, str(dtype)))
-    N.check(lib.icap_linear_ce_bwd(code, hidden.data_ptr(), _ce_rows(hidden, "hidden"), weight.data_ptr(), _ce_rows(weight, "weight"), _p(bias),
+    N.check(lib.icap_linear_ce_bwd(code, hidden.data_ptr(), ld_h, weight.data_ptr(), ld_w, _p(bias),
                                    targets.data_ptr(), R, E, V, ignore_index, rows[1].data_ptr(), out.data_ptr(), g.data_ptr(), _p(dh), _p(dw), _p(db),
                                    ws.data_ptr(), nbytes, _stream()), "linear_ce_bwd")
     span.done()

@@ -865,8 +865,15 @@ int icap_attention_packed_bwd(int dtype, const void* dout, const void* q, const 
  * they are scaled by (down to 2^-39 of it): a row of hidden and of weight by its own largest value for the logits, all of them by one for
  * the gradients; a word's softmax values by their own largest for dweight, so that a word of small probability everywhere keeps its gradient.
  * Magnitudes of fp32 hidden and weight below 2^74.
- * ws: icap_linear_ce_ws_bytes(dtype, rows, width, vocab, backward) bytes, 16-byte aligned: at most 256 MB, fp32 partial results and
- * copies of hidden and weight, whatever the vocabulary (but 256 words are worked on at once, however many rows). */
+ * ws: 16-byte aligned, icap_linear_ce_ws_bytes_for(...) bytes for these very tensors (need: 0 for the forward call, otherwise the sum of 1 for
+ * dhidden, 2 for dweight, 4 for dbias), or icap_linear_ce_ws_bytes(dtype, rows, width, vocab, backward), which is enough whatever their
+ * addresses, ld_h and ld_w, and whichever gradients are wanted.  It holds: forward, 8 bytes for 64 logits; backward, the gradient of the
+ * logits of a piece of the vocabulary (256 MB at most, but of 256 words at least, however many rows), fp32 partial results, 4 bytes a word for every 32 rows or more
+ * where dbias or an fp32 dweight is wanted; and, of hidden and weight where they cannot be read as they are, copies: one of a
+ * 16-bit weight whose rows are not whole multiples of 64 values, 16-byte aligned (backward: or whose words are not a multiple of 64), one of 16-bit hidden
+ * (backward, and forward under the same condition), and of fp32 tensors 16-bit parts as large as they are (backward: up to twice that). */
+long long icap_linear_ce_ws_bytes_for(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, int rows, int width,
+                                      int vocab, int need);
 long long icap_linear_ce_out_floats(int dtype, int rows, int vocab);
 long long icap_linear_ce_ws_bytes(int dtype, int rows, int width, int vocab, int backward);
 int icap_linear_ce_fwd(int dtype, const void* hidden, long long ld_h, const void* weight, long long ld_w, const void* bias,

@@ -1,9 +1,11 @@
 """GPU: calls of the packed attention, the vocabulary loss and the many-tensor AdamW at the edges of what they take: sizes of one with odd
 strides, losses changed in place, gradients far from 1, words of small probability, memory that a call takes."""
+import math
+
 import pytest
 import torch
 
-from .test_gpu_packed_ops import D, E24, F16, F32, TYPES, half_step, offsets, rnd, within
+from .test_gpu_packed_ops import BF16, D, E24, F16, F32, TYPES, half_step, offsets, rnd, within
 
 pytestmark = pytest.mark.gpu
 
@@ -271,3 +273,26 @@ def test_attention_of_one_head_and_of_rows_far_apart(dtype):
     one = offsets([1]).to(D)
     dense = torch.empty(far.shape, device=D, dtype=dtype).copy_(far)
     assert torch.equal(ops.attention_packed(far, far, far, one), ops.attention_packed(dense, dense, dense, one))
+
+
+# ------------------------------------------------------------------------------------------------ memory of the loss
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_linear_ce_takes_no_memory_for_copies_that_it_does_not_make(dtype):
+    """A weight that is read where it lies is not allocated again: one row scored over it takes kilobytes."""
+    from image_captioning_amd import train_ops as T
+    V, E = 65536, 1024
+    w = torch.zeros(V, E, device=D, dtype=dtype)
+    h, t = torch.zeros(3, E, device=D, dtype=dtype), torch.tensor([5, 0, V - 1], device=D)
+    T.linear_ce_fwd(h, w, None, t, want_grad=False)
+    torch.cuda.synchronize()
+    used = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    value, _, saved = T.linear_ce_fwd(h, w, None, t)
+    assert torch.cuda.max_memory_allocated() - used < 1 << 20
+    assert abs(float(value) - math.log(V)) < 1e-5
+    used = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    dh, _, _ = T.linear_ce_bwd(torch.ones(1, device=D), saved, need=(True, False, False))
+    # D of 64 rows (8 MB), partial results of dhidden; no copy of the weight (128 MB)
+    assert torch.cuda.max_memory_allocated() - used < 32 << 20
+    assert not dh.any()

@@ -30,3 +30,26 @@ def test_packed_rows_are_readable_whatever_the_layout(dtype):
         assert torch.equal(got, t) and (got.data_ptr() == t.data_ptr()) == in_place
         assert got.stride(2) == 1 and got.data_ptr() % 16 == 0 and all(x % per == 0 for x in got.stride()[:2])
         assert got.stride(0) <= 1 << 24 and got.stride(1) * got.size(1) <= 1 << 30
+
+
+def test_linear_ce_workspace_for_the_tensors_of_a_call():
+    """What is read where it lies takes no room, results that are not wanted take none, and nothing takes more than any call of that size."""
+    ws, of = N.load().icap_linear_ce_ws_bytes, N.load().icap_linear_ce_ws_bytes_for
+    at = 1 << 20
+    for dtype in (0, 1, 2):
+        for R, E, V in ((1, 8, 1), (3, 2048, 65536), (684, 512, 81), (4864, 512, 6756), (8192, 2048, 65536), (20000, 16, 4100)):
+            for h, ld_h, w, ld_w in ((at, E, at, E), (at, E + 3, at + 2, E + 5), (at + 4, E, at, E + 64)):
+                assert 0 < of(dtype, h, ld_h, w, ld_w, R, E, V, 0) <= ws(dtype, R, E, V, 0)
+                every = of(dtype, h, ld_h, w, ld_w, R, E, V, 7)
+                assert every <= ws(dtype, R, E, V, 1)
+                for need in range(1, 7):
+                    assert 0 < of(dtype, h, ld_h, w, ld_w, R, E, V, need) <= every
+    # one row scored over a weight that is read where it lies: its strips; a copy of the weight alone is 268 MB
+    assert of(1, at, 2048, at, 2048, 1, 2048, 65536, 0) < 1 << 14 and of(1, at, 2048, at + 2, 2048, 1, 2048, 65536, 0) > 1 << 28
+    assert of(1, at, 2048, at, 2048, 8192, 2048, 65536, 7) <= of(1, at, 2048, at, 2049, 8192, 2048, 65536, 7) - (1 << 28)
+    assert of(1, at, 8, at, 8, 0, 8, 8, 0) == 0
+    # too small by one piece of the workspace: refused
+    n = of(0, at, 64, at, 64, 4, 64, 100, 2)
+    good = dict(dtype=0, h=16, ldh=64, w=16, ldw=64, b=None, t=16, R=4, E=64, V=100, ign=-100, lse=16, out=16, g=16, dh=None, dw=16, db=None, ws=16, nbytes=n - 256)
+    assert N.load().icap_linear_ce_bwd(*good.values(), None) == 1
+    assert N.load().icap_linear_ce_bwd(*{**good, "dw": None, "nbytes": 0, "ws": None}.values(), None) == 0          # nothing is wanted
