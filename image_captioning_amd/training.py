@@ -141,16 +141,21 @@ class _LinearCE(torch.autograd.Function):
         return (*T.linear_ce_bwd(g, (hidden, weight, bias, targets, ctx.ignore_index, rows, out), need=ctx.needs_input_grad[:3]), None, None, None)
 
 
+def _ce_matrix(t):
+    """t where its rows lie one after another, a copy otherwise (an expanded row, a turned weight)."""
+    return t if (t.size(1) == 1 or t.stride(1) == 1) and (t.size(0) <= 1 or t.stride(0) >= t.size(1)) else t.contiguous()
+
+
 def linear_cross_entropy(hidden, weight, bias, targets, ignore_index: int = -100, mean_over_valid: bool = True) -> torch.Tensor:
     """The loss of an output layer and its criterion in one: cross entropy of hidden @ weight.T + bias, without the logits in
     memory (train_ops.linear_ce_fwd).  hidden [..., width] fp32, bf16 or fp16, targets [...] int64, weight [vocab, width] and bias
     [vocab] or None (an nn.Linear's) of the same type.  mean_over_valid: the mean over the rows that are not ignored, as
-    CrossEntropyLoss above; otherwise over all rows, as compute_loss."""
+    CrossEntropyLoss above; otherwise over all rows, as compute_loss.  hidden and weight whose rows do not lie one after another are copied."""
     if hidden.dim() < 2 or hidden.shape[:-1] != targets.shape:
         raise N.IcapError(f"linear_cross_entropy: hidden {tuple(hidden.shape)} and targets {tuple(targets.shape)} do not belong together")
-    hidden, targets = hidden.reshape(-1, hidden.size(-1)), targets.reshape(-1).contiguous()
-    if hidden.numel() and hidden.stride(-1) != 1:
-        hidden = hidden.contiguous()
+    hidden, targets = _ce_matrix(hidden.reshape(-1, hidden.size(-1))), targets.reshape(-1).contiguous()
+    if weight.dim() == 2:
+        weight = _ce_matrix(weight)
     return _LinearCE.apply(hidden, weight, bias, targets, int(ignore_index), bool(mean_over_valid))
 
 

@@ -296,3 +296,14 @@ def test_linear_ce_takes_no_memory_for_copies_that_it_does_not_make(dtype):
     # D of 64 rows (8 MB), partial results of dhidden; no copy of the weight (128 MB)
     assert torch.cuda.max_memory_allocated() - used < 32 << 20
     assert not dh.any()
+
+
+# ------------------------------------------------------------------------------------------------ tensors as programs have them
+def test_linear_cross_entropy_of_rows_that_share_memory_and_of_turned_weights():
+    from image_captioning_amd import training
+    h, w = rnd(1, 64, seed=1).to(D).requires_grad_(), rnd(64, 90, seed=2, scale=0.2).to(D).requires_grad_()
+    t = torch.randint(0, 90, (40,), generator=torch.Generator().manual_seed(3)).to(D)
+    got = torch.autograd.grad(training.linear_cross_entropy(h.expand(40, 64), w.t(), None, t), (h, w))
+    want = torch.autograd.grad(training.linear_cross_entropy(h.repeat(40, 1), w.t().contiguous(), None, t), (h, w))
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
