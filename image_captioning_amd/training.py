@@ -150,9 +150,13 @@ def linear_cross_entropy(hidden, weight, bias, targets, ignore_index: int = -100
     """The loss of an output layer and its criterion in one: cross entropy of hidden @ weight.T + bias, without the logits in
     memory (train_ops.linear_ce_fwd).  hidden [..., width] fp32, bf16 or fp16, targets [...] int64, weight [vocab, width] and bias
     [vocab] or None (an nn.Linear's) of the same type.  mean_over_valid: the mean over the rows that are not ignored, as
-    CrossEntropyLoss above; otherwise over all rows, as compute_loss.  hidden and weight whose rows do not lie one after another are copied."""
+    CrossEntropyLoss above; otherwise over all rows, as compute_loss.  hidden and weight whose rows do not lie one after another are copied.
+    Under torch.autocast tensors of different types (hidden of 16 bits, fp32 parameters) are taken in autocast's type, as nn.Linear takes them;
+    their gradients come in their own."""
     if hidden.dim() < 2 or hidden.shape[:-1] != targets.shape:
         raise N.IcapError(f"linear_cross_entropy: hidden {tuple(hidden.shape)} and targets {tuple(targets.shape)} do not belong together")
+    if torch.is_autocast_enabled("cuda") and any(t is not None and t.dtype != hidden.dtype for t in (weight, bias)):
+        hidden, weight, bias = (t if t is None else t.to(torch.get_autocast_dtype("cuda")) for t in (hidden, weight, bias))
     hidden, targets = _ce_matrix(hidden.reshape(-1, hidden.size(-1))), targets.reshape(-1).contiguous()
     if weight.dim() == 2:
         weight = _ce_matrix(weight)

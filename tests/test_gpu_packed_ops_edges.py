@@ -307,3 +307,20 @@ def test_linear_cross_entropy_of_rows_that_share_memory_and_of_turned_weights():
     want = torch.autograd.grad(training.linear_cross_entropy(h.repeat(40, 1), w.t().contiguous(), None, t), (h, w))
     for x, y in zip(got, want):
         assert torch.equal(x, y)
+
+
+# ------------------------------------------------------------------------------------------------ types of one program
+def test_linear_cross_entropy_under_autocast():
+    """hidden in 16 bits from an autocast layer, weight and bias in fp32: taken as nn.Linear takes them; gradients reach the fp32 leaves."""
+    from image_captioning_amd import _native as N, training
+    h, w, b = rnd(40, 64, seed=1).to(D).requires_grad_(), rnd(90, 64, seed=2, scale=0.2).to(D).requires_grad_(), rnd(90, seed=3).to(D).requires_grad_()
+    t = torch.randint(0, 90, (40,), generator=torch.Generator().manual_seed(3)).to(D)
+    for dtype in (BF16, F16):
+        with torch.autocast("cuda", dtype=dtype):
+            value = training.linear_cross_entropy(h.to(dtype), w, b, t)
+        want = training.linear_cross_entropy(h.to(dtype), w.to(dtype), b.to(dtype), t)
+        assert torch.equal(value.detach(), want.detach())
+        for x, y in zip(torch.autograd.grad(value, (h, w, b)), torch.autograd.grad(want, (h, w, b))):
+            assert x.dtype == F32 and torch.equal(x, y)
+    with pytest.raises(N.IcapError):
+        training.linear_cross_entropy(h.to(BF16), w, b, t)
