@@ -417,6 +417,8 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && (NW < 4 || sizeof(T) == 4) ? 
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = zeros16();
     float m = -INFINITY, l = 0.f;
+    // fp16 ends at 2^-24: weights (up to 2^8, see above) are taken 2^7 times, as their sum then is; 11 bits down to 2^-21 of the largest
+    constexpr float P_BITS = __is_same(T, _Float16) ? 7.0f : 0.0f;
     const float c2 = a.scale * LOG2E;
     // The scores of the next 32 keys are formed while the exponentials of these run, so K is staged 32 keys ahead of V: a step of
     // V's keys n0 .. n0 + BN goes with K's n0 + 32 .. n0 + BN + 32
@@ -454,7 +456,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && (NW < 4 || sizeof(T) == 4) ? 
             for (int d = 0; d < ND; ++d) o[d] *= alpha;
         }
         const f32x16 next = scores(kt, kr);
-        const float base = m == -INFINITY ? 0.f : m;
+        const float base = (m == -INFINITY ? 0.f : m) - P_BITS;
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -484,6 +486,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && (NW < 4 || sizeof(T) == 4) ? 
         }
     }
     float sum = l + __shfl_xor(l, 32);
+    m -= P_BITS;
     if (!finite_row(o)) {
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] = zeros16();

@@ -324,3 +324,31 @@ def test_linear_cross_entropy_under_autocast():
             assert x.dtype == F32 and torch.equal(x, y)
     with pytest.raises(N.IcapError):
         training.linear_cross_entropy(h.to(BF16), w, b, t)
+
+
+# ------------------------------------------------------------------------------------------------ large values of keys that are hardly seen
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [40, 700])
+def test_attention_of_large_values_that_are_hardly_seen(dtype, n):
+    """Weights of some 1e-7 of values of 6e4: what they add to a row is far above a rounding of it."""
+    from image_captioning_amd import ops
+    q, k, v = (rnd(n, 2, 64, seed=s, scale=c, dtype=dtype) for s, c in ((1, 0.1), (2, 0.1), (3, 0.01)))
+    q[:, :, 0] = 4.0
+    k[3::7, :, 0] = torch.linspace(-24.0, -32.0, len(k[3::7]))[:, None].to(dtype)
+    v[3::7] = 6e4
+    for causal in (False, True):
+        cu = offsets([n]).to(D)
+        out, lse = ops.attention_packed(*(x.to(D) for x in (q, k, v)), cu, causal=causal, want_lse=True)
+        u = half_step(dtype)
+        for h in range(2):
+            Q, KK, V = (x[:, h].double() for x in (q, k, v))
+            s = 0.125 * Q @ KK.t()
+            if causal:
+                s = s.masked_fill(torch.ones(n, n, dtype=torch.bool).triu(1), -math.inf)
+            want = torch.logsumexp(s, 1)
+            P = torch.exp(s - want[:, None])
+            e_s = float(0.125 * 72 * E24 * (Q.abs() @ KK.abs().t()).max()) + 2.0 ** -21
+            # each weight rounded once, and no further than 2^-32 of the row's largest
+            bound = ((0.0 if dtype == F32 else u) + (n + 16) * E24 + 3 * e_s) * (P @ V.abs()) + (2.0 ** -32 * V.abs().sum(0) if dtype == F16 else 0.0)
+            within(out[:, h], P @ V, bound + u * (P @ V).abs() * (1 + 2.0 ** -6) + (2.0 ** -25 if dtype == F16 else 0.0) + 1e-30, "out")
+            within(lse[:, h], want, 2 * e_s + 4 * E24 * want.abs() + (n + 16) * E24, "lse")
