@@ -115,7 +115,7 @@ def backward_oracle(q, k, v, g, out, lse, causal, scale):
         r["dv"][:, c] += P.t() @ G
         # weights of fp16 keep their 11 bits down to 2^-28
         b["dv"][:, c] += ((up + f + 3 * e_s) * P + (2.0 ** -39 if tiny else 0.0)).t() @ G.abs() * 1.01
-    return {m: (r[m], b+ u * r[m].abs() * (1 + 2.0 ** -6) + tiny * 1.01 + 1e-30) for m in r}
+    return {m: (r[m], b[m] + u * r[m].abs() * (1 + 2.0 ** -6) + tiny * 1.01 + 1e-30) for m in r}
 
 
 @pytest.mark.parametrize("dtype", TYPES)
