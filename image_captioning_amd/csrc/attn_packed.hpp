@@ -17,9 +17,9 @@
 // result is not finite is formed once more from what it sees alone ("values that are not finite" below).
 //
 // What bounds it: at dim 128 a wave of 32 rows needs per 64 keys 1024 cycles of its SIMD's matrix core and about as many of
-// its vector unit (32 exponentials of 16 cycles), and the two overlap only in part: 872 TFLOP/s on six bf16 prompts of up to 8192 tokens
-// (354 us; a product of that many operations alone takes 252), matrix cores busy 47 % of the cycles, LDS without conflicts.  So two waves a
-// SIMD interleave (four-wave workgroups, two a CU: with one of eight waves all were in the same phase, 404 against 383 us on
+// its vector unit (32 exponentials of 16 cycles), and the two overlap only in part: 874 TFLOP/s on six bf16 prompts of up to 8192 tokens
+// (366 us; a product of that many operations alone takes 252), matrix cores busy 47 % of the cycles, LDS without conflicts.  About 13 % of
+// them are a tail, as the longest text's tiles do not start first (fwd_kernel).  Two waves a SIMD interleave (four-wave workgroups, two a CU: with one of eight waves all were in the same phase, 404 against 383 us on
 // those prompts), the scores of the next step are formed beside the exponentials of this one (383 -> 353 us), and nothing
 // else stays in the loop:
 //   * tiles go global -> LDS without registers, double-buffered, one barrier a step;
@@ -27,9 +27,10 @@
 //     rows of a fragment read and the 4 rows of a transposing read over different banks;
 //   * the running maximum is only followed when it grows by more than 2^8 (weights stay below 256, sums in fp32, so nothing
 //     is lost), which leaves the accumulators alone in almost every step.
-// Backward, 8 bf16 sequences of up to 2048 tokens, dim 64: dK and dV 106 + 13, dQ 69 + 10 (the second part of dS), forward 61 us; the steps of
-// the longest sequence's first keys, one after another, are what they last.  Short texts (fp32 captions of up to 58 tokens: forward 35, dQ 45,
-// dK and dV 49 us) are bound by places of other texts in their tiles: a wave multiplies about three times what its rows see.
+// Backward, 8 bf16 sequences of up to 2048 tokens, dim 64: dK and dV 117, dQ 78, forward 60 us; the steps of the longest sequence's first
+// keys, one after another, are what they last.  Short texts (fp32 captions of up to 58 tokens: forward 34, dQ 44, dK and dV 49 us) are
+// bound by places of other texts in their tiles: 6.1 times the pairs that are seen are multiplied in the forward pass, 4.6 (dQ) and
+// 4.1 (dK, dV) times in the backward pass.
 #pragma once
 #include "packed.hpp"
 
@@ -160,8 +161,9 @@ __device__ __forceinline__ typename Vec<T>::x8 col_frag(const T* lds, int row0, 
     }
 }
 
-// eight registers of an accumulator (16 of its rows) as an operand: the one rounding of P to a 16-bit type (2^-9 / 2^-12 of
-// each value, as much as the result's own rounding; the sum of P itself is taken from the unrounded values)
+// eight registers of an accumulator (16 of its rows) as an operand: the one rounding of P to a 16-bit type (2^-8 / 2^-11 of
+// each value, as much as the result's own rounding: O is up to 1.3 times as far off as a rounding of the exact result; a second
+// part would double the product with V; the sum of P itself is taken from the unrounded values)
 template <typename T>
 __device__ __forceinline__ typename Vec<T>::x8 acc_frag(const f32x16& a, int half) {
     f32x8 x;
@@ -171,9 +173,9 @@ __device__ __forceinline__ typename Vec<T>::x8 acc_frag(const f32x16& a, int hal
     else return __builtin_convertvector(x, typename Vec<T>::x8);
 }
 
-// dS in two parts, high and low (16-bit types; 16 bits and more of each value, of bf16; of fp16 see lower below): its terms differ in sign, so that one rounded part made
-// dQ and dK 1.53 times as far off as rounding the exact results does; two: 1.17 times, the rest from O's own rounding in delta.  The
-// second product costs 8 % of a training pass (222 -> 241 us, 8 bf16 sequences of up to 2048 tokens, dim 64) to 19 % (dim 128).
+// dS in two parts, high and low (16-bit types; 16 bits and more of each value, of fp16 with the power of two of lower() below): its terms
+// differ in sign, so that one rounded part made dQ and dK 1.53 times as far off as rounding the exact results does; two: 1.17 times, the
+// rest from O's own rounding in delta.  The second product costs 8 % of a training pass (222 -> 241 us, 8 bf16 sequences of up to 2048 tokens, dim 64) to 19 % (dim 128).
 template <typename T>
 __device__ __forceinline__ void acc_parts(const f32x16& a, int half, typename Vec<T>::x8& hi, typename Vec<T>::x8& lo) {
     f32x8 x, y;
@@ -194,9 +196,9 @@ __device__ __forceinline__ void acc_parts(const f32x16& a, int half, typename Ve
 // fp16 ends at 2^-24 and at 65504, and dS, a weight times an output gradient, at neither: over 4096 keys and gradients of 1e-3 it is some 2e-6, of
 // which the two parts held 5 bits.  So a column's dS (its row's in dQ, its key's in dK) are formed with a power of two, which the
 // column's accumulators then have, too.  It starts at 2^40 and is lowered when a value would pass 2^15: the largest so far is at 2^8
-// and above (or below 2^-25), and values down to 2^-11 of it have all 22 bits.  Backward pass of 8
-// fp16 sequences of up to 2048 tokens, dim 64: 155 -> 163 us, 16 of 1024, dim 128: 623 -> 707; under a loss scale with which dS passed 65504, and
-// every such row was formed once more (below), 13.5 ms -> 163 us.
+// and above (or below 2^-25), and values down to 2^-11 of it have all 22 bits.  Backward pass of 8 fp16 sequences of up to 2048 tokens, dim 64:
+// 155 -> 163 us, 16 of 1024, dim 128: 623 -> 707; under a loss scale with which dS passed 65504, and every such row was formed once
+// more ("values that are not finite" below), 13.5 ms -> 163 us.
 constexpr int LIFT0 = 40;
 __device__ __forceinline__ float power_of(int b) { return __uint_as_float((unsigned)(b + 127) << 23); }
 // s: dS 2^bits of 16 places
@@ -392,7 +394,8 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && (NW < 4 || sizeof(T) == 4) ? 
     __shared__ __attribute__((aligned(1024))) T sk[2][BN * DP];
     __shared__ __attribute__((aligned(1024))) T sv[2][BN * DP];
     const int kvh = blockIdx.x % a.kv_heads, tiles = gridDim.x / a.kv_heads, lane = threadIdx.x & 63, lh = lane >> 5;
-    // causal: the rows of a sequence's end see most keys and start first
+    // causal: later rows of a sequence see more keys and start first.  Sequences go in the order they are given, the last one first (507,
+    // 112, 4, 8192, 301 and 3254 tokens: 187 steps one after another, 162 if the longest tiles started first)
     const int tile = a.causal ? tiles - 1 - (int)(blockIdx.x / a.kv_heads) : blockIdx.x / a.kv_heads;
     const int row0 = tile * BM, row = row0 + (threadIdx.x >> 6) * 32 + (lane & 31), total = a.tokens_q * a.group;
     const int tok = min(row, total - 1) / a.group, head = kvh * a.group + min(row, total - 1) - tok * a.group;

@@ -9,7 +9,7 @@
 // All products are one GEMM kernel: C[m][n] = sum_k A[m][k] B[n][k] on the 16-bit matrix cores, fp32 accumulation.  An operand's k is
 // contiguous (x), or its rows are k (W in dh, D and h in dW): those tiles pass the LDS's transposing read on their way to the matrix cores, and
 // nothing is transposed in memory.
-//   bf16: D is rounded to bf16 (2^-9 of each value, as much as the result's own rounding).
+//   bf16: D is rounded to bf16 (2^-8 of each value, as much as the result's own rounding).
 //   fp16: D 2^14 is rounded to fp16, so that a probability of 1e-8 still has full precision; the factor leaves again exactly.
 //   fp32: every operand is the sum of two fp16 values (22 bits), scaled by a power of two so that its largest magnitude is near
 //   2^14; the products hi hi + hi lo + lo hi drop 2^-22 of each term: as exact as an fp32 dot product, at three fp16

@@ -575,8 +575,8 @@ def adamw_tensors(params, grads, exp_avg, exp_avg_sq, step, lr, beta1=0.9, beta2
 
     params: fp32, bf16 or fp16, contiguous; grads: their gradients, of the same type or fp32 (None: the tensor is left alone).
     exp_avg, exp_avg_sq: fp32 tensors (states of 32 bits), or (codes, scales) pairs (states of 8 bits: adamw_state8; the second one
-    holds the SQUARE ROOT of the second moment, rounded at random - with the right mean - from `seed`, the step, the tensor's index
-    and the place, so a step can be repeated).  All states are of one kind.
+    holds the SQUARE ROOT of the second moment, rounded at random - with the right mean, but never from above zero to zero - from `seed`,
+    the step, the tensor's index and the place, so a step can be repeated).  All states are of one kind.
     step: from 1, one for all or a list; step_dev: int32 [1] on the device, added to step by the kernel (a step recorded in a HIP
     graph: step = 0 and the count kept there).  index: the tensors' numbers for the generator (their places in the list).
     No parameter or state may appear twice.  The parameters' version counters advance, as after any operation in place: the backward pass of a
