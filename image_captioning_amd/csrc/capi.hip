@@ -234,9 +234,9 @@ static int attention_check(const char* what, int dtype, const AttnArgs& a) {
         set_error("%s: strides beyond 2^24 elements a token", what);
         return ICAP_ERR_LIMIT;
     }
-    // a launch has fewer than 2^32 threads, and rows (tokens x heads) take eight of them each
-    if ((long long)a.tokens_q * a.heads > (1ll << 28) || (long long)a.tokens_k * a.kv_heads > (1ll << 28) || a.seqs > (1 << 24)) {
-        set_error("%s: tokens x heads beyond 2^28, or more than 2^24 sequences", what);
+    // a launch has fewer than 2^32 threads: rows (tokens x heads) take eight of them each, and every key head a workgroup of up to 256
+    if ((long long)a.tokens_q * a.heads > (1ll << 28) || (long long)a.tokens_k * a.kv_heads > (1ll << 28) || a.kv_heads > (1 << 23) || a.seqs > (1 << 24)) {
+        set_error("%s: tokens x heads beyond 2^28, more than 2^23 key heads, or more than 2^24 sequences", what);
         return ICAP_ERR_LIMIT;
     }
     return ICAP_OK;

@@ -53,3 +53,14 @@ def test_linear_ce_workspace_for_the_tensors_of_a_call():
     good = dict(dtype=0, h=16, ldh=64, w=16, ldw=64, b=None, t=16, R=4, E=64, V=100, ign=-100, lse=16, out=16, g=16, dh=None, dw=16, db=None, ws=16, nbytes=n - 256)
     assert N.load().icap_linear_ce_bwd(*good.values(), None) == 1
     assert N.load().icap_linear_ce_bwd(*{**good, "dw": None, "nbytes": 0, "ws": None}.values(), None) == 0          # nothing is wanted
+
+
+def test_attention_refuses_more_key_heads_than_a_launch_takes():
+    """One token has no stride that would bound its heads."""
+    lib = N.load()
+    fwd = dict(dtype=1, q=16, k=16, v=16, out=16, lse=None, cu_q=4, cu_k=4, seqs=1, tq=1, tk=1, h=(1 << 23) + 1, kv=(1 << 23) + 1, d=8, qt=0, qh=8, kt=0, kh=8, vt=0, vh=8,
+               scale=0.1, causal=1, ws=None, nbytes=0)
+    assert lib.icap_attention_packed_fwd(*fwd.values(), None) == 3 and b"key heads" in lib.icap_last_error()
+    bwd = dict(dtype=1, dout=16, q=16, k=16, v=16, out=16, lse=16, dq=16, dk=16, dv=16, cu_q=4, cu_k=4, seqs=1, tq=1, tk=1, h=1 << 24, kv=1 << 24, d=8, gt=0, gh=8,
+               qt=0, qh=8, kt=0, kh=8, vt=0, vh=8, scale=0.1, causal=1, ws=16)
+    assert lib.icap_attention_packed_bwd(*bwd.values(), None) == 3
