@@ -214,6 +214,8 @@ def test_attention_of_large_values_that_are_hardly_seen(dtype, n):
             bound = ((0.0 if dtype == F32 else u) + (n + 16) * E24 + 3 * e_s) * (P @ V.abs()) + (2.0 ** -32 * V.abs().sum(0) if dtype == F16 else 0.0)
             within(out[:, h], P @ V, bound + u * (P @ V).abs() * (1 + 2.0 ** -6) + (2.0 ** -25 if dtype == F16 else 0.0) + 1e-30, "out")
             within(lse[:, h], want, 2 * e_s + 4 * E24 * want.abs() + (n + 16) * E24, "lse")
+
+
 # ------------------------------------------------------------------------------------------------ the graph knows of the update
 @pytest.mark.parametrize("bits", [8, 32])
 def test_adamw_tensors_tells_autograd_that_parameters_changed(bits):
@@ -376,3 +378,63 @@ def test_linear_cross_entropy_under_autocast():
             assert x.dtype == F32 and torch.equal(x, y)
     with pytest.raises(N.IcapError):
         training.linear_cross_entropy(h.to(BF16), w, b, t)
+
+
+# ------------------------------------------------------------------------------------------------ recorded, and two at once
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_captured_gradients_replay_with_new_inputs(dtype):
+    """Loss and attention with their gradients in a HIP graph, replayed with inputs whose sizes differ by powers of ten, eager work between."""
+    from image_captioning_amd import ops, train_ops as T
+    H, dim, V, lens = 4, 32, 301, [9, 40, 15]
+    n, E = sum(lens), H * dim
+    cu = offsets(lens).to(D)
+    w, b = rnd(V, E, seed=100, scale=E ** -0.5, dtype=dtype).to(D), (rnd(V, seed=101) - torch.linspace(0, 20, V)).to(dtype).to(D)
+
+    def inputs(i):
+        return rnd(n, 3 * H, dim, seed=i, dtype=dtype).to(D), torch.randint(0, 100, (n,), generator=torch.Generator().manual_seed(i)).to(D), torch.full((1,), 10.0 ** (2 * i - 3), device=D)
+
+    def step(x, t, g):
+        q, k, v = x.split((H, H, H), 1)
+        out, lse = ops.attention_packed(q, k, v, cu, want_lse=True)
+        value, row, saved = T.linear_ce_fwd(out.view(n, E), w, b, t)
+        dh, dw, db = T.linear_ce_bwd(g, saved)
+        return (value, row, dh, dw, db, *T.attention_packed_bwd(dh.view(n, H, dim), q, k, v, out, lse, cu))
+    x, t, g = inputs(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, t, g)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        recorded = step(x, t, g)
+    for i in (1, 3, 0, 2):
+        new = inputs(i)
+        for a, c in zip((x, t, g), new):
+            a.copy_(c)
+        graph.replay()
+        eager = step(*new)
+        torch.cuda.synchronize()
+        for a, c in zip(recorded, eager):
+            assert torch.equal(a, c), f"inputs {i}"
+
+
+def test_loss_gradients_on_two_streams_at_once():
+    from image_captioning_amd import train_ops as T
+    h, w, t = rnd(700, 64, seed=4).to(D), rnd(2000, 64, seed=5, scale=0.1).to(D), torch.arange(700, device=D)
+    h2, w2, t2 = rnd(300, 128, seed=6).to(D), rnd(900, 128, seed=7, scale=0.1).to(D), torch.arange(300, device=D)
+    one = torch.ones(1, device=D)
+
+    def go(*x):
+        return T.linear_ce_bwd(one, T.linear_ce_fwd(x[0], x[1], None, x[2])[2])[:2]
+    want = go(h, w, t), go(h2, w2, t2)
+    torch.cuda.synchronize()
+    a, c = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(a):
+            x = go(h, w, t)
+        with torch.cuda.stream(c):
+            y = go(h2, w2, t2)
+        torch.cuda.synchronize()
+        for got, ref in zip((*x, *y), (*want[0], *want[1])):
+            assert torch.equal(got, ref)
